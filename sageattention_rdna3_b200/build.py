@@ -18,6 +18,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -25,11 +26,10 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_ABI = PKG_DIR / "libsage_b200.so"
 LIB_OPS = PKG_DIR / "_C.so"
+OBJ_DIR = PKG_DIR / "build"
 
-NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC", "--cudart", "shared",
-]
+NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
+LINK_FLAGS = ["-shared", "--cudart", "shared"]
 
 
 def _nvcc() -> str:
@@ -63,16 +63,33 @@ def _run(cmd) -> None:
         raise RuntimeError("build command failed:\n  " + " ".join(map(str, cmd)) + "\n" + proc.stdout)
 
 
+def _compile(jobs, force: bool, extra: str = "") -> list:
+    """Objects of (command, source, headers), each in a process of its own and only where something changed."""
+    OBJ_DIR.mkdir(exist_ok=True)
+    objects = [OBJ_DIR / (unit.name + ".o") for _, unit, _ in jobs]
+
+    def one(job, obj):
+        cmd, unit, headers = job
+        if force or not _up_to_date(obj, [unit, *headers], extra):
+            _run([*cmd, "-c", "-o", str(obj), str(unit)])
+            _write_stamp(obj, [unit, *headers], extra)
+
+    with ThreadPoolExecutor(len(jobs)) as pool:
+        list(pool.map(one, jobs, objects))
+    return objects
+
+
 def build_abi(force: bool = False, verbose: bool = False) -> Path:
-    sources = [CSRC / "sage_abi.cu", CSRC / "attn_kernel.cuh", CSRC / "prep_kernels.cuh", CSRC / "merge_kernels.cuh",
-               CSRC / "pair_kernel.cuh",
-               CSRC / "ptx_sm100.cuh", CSRC / "internal.h",
-               REPO_DIR / "include" / "sage_b200.h"]
+    common = [CSRC / "ptx_sm100.cuh", CSRC / "host_common.h", REPO_DIR / "include" / "sage_b200.h"]
+    attn = [*common, CSRC / "attn_kernel.cuh", CSRC / "prep_kernels.cuh", CSRC / "merge_kernels.cuh", CSRC / "pair_kernel.cuh",
+            CSRC / "internal.h"]
+    paged = [*common, CSRC / "paged_common.cuh", CSRC / "rotary_kernels.cuh", REPO_DIR / "include" / "sage_paged_b200.h"]
+    units = [(CSRC / "sage_abi.cu", attn), (CSRC / "paged_abi.cu", paged)]
+    sources = sorted({f for unit, headers in units for f in (unit, *headers)})
     if force or not _up_to_date(LIB_ABI, sources):
-        cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(LIB_ABI), str(CSRC / "sage_abi.cu")]
-        if verbose:
-            cmd.insert(1, "-Xptxas=-v")
-        _run(cmd)
+        nvcc = [_nvcc(), *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS]
+        objects = _compile([(nvcc, unit, headers) for unit, headers in units], force)
+        _run([_nvcc(), *NVCC_FLAGS, *LINK_FLAGS, "-o", str(LIB_ABI), *map(str, objects)])
         _write_stamp(LIB_ABI, sources)
     return LIB_ABI
 
@@ -81,21 +98,23 @@ def build_ops(force: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    sources = [CSRC / "torch_ops.cpp", CSRC / "internal.h", REPO_DIR / "include" / "sage_b200.h"]
+    units = [(CSRC / "torch_ops.cpp", [CSRC / "internal.h", REPO_DIR / "include" / "sage_b200.h"]),
+             (CSRC / "torch_paged_ops.cpp", [REPO_DIR / "include" / "sage_b200.h", REPO_DIR / "include" / "sage_paged_b200.h"])]
+    sources = sorted({f for unit, headers in units for f in (unit, *headers)})
     extra = torch.__version__
     if force or not _up_to_date(LIB_OPS, sources, extra):
         torch_lib = Path(torch.__file__).parent / "lib"
         includes = cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]
-        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+        gxx = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                "-DTORCH_EXTENSION_NAME=_C"]
         for inc in includes:
-            cmd += ["-isystem", str(inc)]
-        cmd += [str(CSRC / "torch_ops.cpp"), "-o", str(LIB_OPS),
-                f"-L{PKG_DIR}", "-l:libsage_b200.so", f"-L{torch_lib}",
-                "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda", "-ltorch_python",
-                "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
-        _run(cmd)
+            gxx += ["-isystem", str(inc)]
+        objects = _compile([(gxx, unit, headers) for unit, headers in units], force, extra)
+        _run(["g++", "-shared", *map(str, objects), "-o", str(LIB_OPS),
+              f"-L{PKG_DIR}", "-l:libsage_b200.so", f"-L{torch_lib}",
+              "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda", "-ltorch_python",
+              "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
         _write_stamp(LIB_OPS, sources, extra)
     return LIB_OPS
 

@@ -23,7 +23,8 @@ _LAYOUT_CODE = {"NHD": 0, "HND": 1}   # csrc/attn_gfx11.cu:32-33
 _status_words: Dict[int, torch.Tensor] = {}
 _status_mirrors: Dict[int, tuple] = {}
 _STATUS_MESSAGE = ("sageattn: the attention kernel reported device status {code} "
-                   "(1 = shared memory misaligned, 2+16*k = bounded wait k timed out)")
+                   "(1 = shared memory misaligned, 2+16*k = bounded wait k timed out; paged cache: 3 = page index outside "
+                   "the cache, 4 = lengths that do not fit the page table or the new tokens)")
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
@@ -90,6 +91,24 @@ def check_status(device: Union[torch.device, int, str, None] = None) -> None:
         if _MIRROR_ON:
             _status_mirror(device)[1][0] = 0
         raise RuntimeError(_STATUS_MESSAGE.format(code=code))
+
+
+def _prepare_status(device: torch.device) -> None:
+    """Makes the status word of ``device`` and its mirror, which cannot be done inside a stream capture."""
+    _status_word(device)
+    if _MIRROR_ON:
+        _status_mirror(device)
+
+
+def _raise_pending(device: torch.device) -> None:
+    """Raises what an earlier call on ``device`` left in the mirror of the status word."""
+    if _MIRROR_ON:
+        _, seen = _status_mirror(device)
+        if seen[0] != 0:
+            code = int(seen[0])
+            seen[0] = 0
+            _status_word(device).zero_()
+            raise RuntimeError(_STATUS_MESSAGE.format(code=code) + "; reported by the call after the one that failed")
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -262,13 +281,7 @@ def sageattn(
         # or the INT8 branch ([K mean,] quantise Q / K and convert a bf16 V in one launch, attention).
         direct = _pick_direct(kwargs.get("kernel"), headdim, tensor_layout, is_causal, q_len, kv_len)
         smooth = bool(smooth_k) and not direct          # the un-quantised branch has no use for the mean
-        if _MIRROR_ON:
-            _, seen = _status_mirror(q.device)
-            if seen[0] != 0:                            # an earlier call on this device gave up
-                code = int(seen[0])
-                seen[0] = 0
-                _status_word(q.device).zero_()
-                raise RuntimeError(_STATUS_MESSAGE.format(code=code) + "; reported by the call after the one that failed")
+        _raise_pending(q.device)                        # an earlier call on this device gave up
         _register(q.device)
         out = ops.sageattn_fwd(q, k, v, layout, int(is_causal), sm_scale, int(smooth), int(direct),
                                _status_word(q.device), lse if want_lse else None, out_arg,

@@ -1,0 +1,140 @@
+"""Rotary positions with one or several axes, in front of ``sageattn``.
+
+Text has one axis, a picture two or three (frame, row, column), a video three: each axis turns some of the pairs of a
+head.  The reference leaves the rotation to the model; here q and k take one launch together, and the
+gradient another:
+
+    rope = rotary_axes(128, (32, 48, 48), interleaved=True)       # kept: the frequencies on the device
+    q, k = apply_rotary(q, k, positions, rope, tensor_layout="NHD")     # positions: [S, 3]
+    o = sageattn(q, k, v, tensor_layout="NHD")
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _native
+from .core import _LAYOUT_CODE
+
+MAX_AXES = 4
+
+
+@dataclass
+class RotaryAxes:
+    """The frequencies of every pair on a device, made by :func:`rotary_axes`."""
+    head_dim: int
+    axes: Tuple[int, ...]       # widths: values of a head that each axis turns
+    interleaved: bool
+    freq: torch.Tensor          # [pairs] int64: turns per position in units of 2^-64
+    axis: torch.Tensor          # [pairs] int32
+
+    @property
+    def n_axes(self) -> int:
+        return len(self.axes)
+
+    @property
+    def rotary_dim(self) -> int:
+        return sum(self.axes)
+
+
+def rotary_axes(head_dim: int, axes: Union[int, Sequence[int]], base: Union[float, Sequence[float]] = 10000.0,
+                interleaved: bool = False, inv_freq: Optional[Sequence[float]] = None,
+                device: Union[torch.device, int, str, None] = None) -> RotaryAxes:
+    """The table of :func:`apply_rotary` and ``paged_kv_append``.
+
+    axes: how many values of a head each axis turns, e.g. ``(32, 48, 48)`` (even numbers, 1 to 4 of them; their sum is a
+    multiple of 16 and at most ``head_dim``; the values behind them stay as they are).  Pair i of an axis of width w has the
+    frequency ``base ** (-2 i / w)`` radians per position; ``base`` may be one number per axis, and ``inv_freq`` (one
+    number per pair, the pairs of axis 0 first) takes its place.  Pairs are ``(x[i], x[i + rotary_dim / 2])``, or
+    neighbours ``(x[2i], x[2i + 1])`` with ``interleaved``.  The frequencies keep 64 bits, so that positions
+    far from zero lose nothing."""
+    widths = (axes,) if isinstance(axes, int) else tuple(int(w) for w in axes)
+    assert head_dim in (64, 128), f"head_dim must be 64 or 128, got {head_dim}."
+    assert 1 <= len(widths) <= MAX_AXES, f"1 to {MAX_AXES} axes, got {len(widths)}."
+    assert all(w > 0 and w % 2 == 0 for w in widths), f"axes must be positive even widths, got {widths}."
+    total = sum(widths)
+    assert total % 16 == 0 and total <= head_dim, (
+        f"the axes must add up to a multiple of 16 that is at most head_dim, got {total}.")
+    if inv_freq is None:
+        bases = [float(base)] * len(widths) if isinstance(base, (int, float)) else [float(b) for b in base]
+        assert len(bases) == len(widths) and all(b > 0 for b in bases), "base must be positive: one number, or one per axis."
+        inv_freq = [b ** (-2.0 * i / w) for b, w in zip(bases, widths) for i in range(w // 2)]
+    else:
+        inv_freq = [float(f) for f in inv_freq]
+        assert len(inv_freq) == total // 2, f"inv_freq must have one number per pair ({total // 2}), got {len(inv_freq)}."
+    assert all(math.isfinite(f) for f in inv_freq), "frequencies must be finite."
+    freq = []
+    for f in inv_freq:
+        turns = f / (2.0 * math.pi)
+        units = int((turns - math.floor(turns)) * 2.0 ** 64) % 2 ** 64
+        freq.append(units - 2 ** 64 if units >= 2 ** 63 else units)
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else (
+        torch.device("cuda", device) if isinstance(device, int) else torch.device(device))
+    return RotaryAxes(head_dim, widths, bool(interleaved), torch.tensor(freq, dtype=torch.int64).to(dev),
+                      torch.tensor([a for a, w in enumerate(widths) for _ in range(w // 2)], dtype=torch.int32).to(dev))
+
+
+def _vector_aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy of it that 16-byte loads can read."""
+    unit = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, rotary, layout, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.args = (rotary, layout, inverse)
+        out = _native.load_ops().rotary(_vector_aligned(q), None if k is None else _vector_aligned(k), positions, rotary.freq,
+                                        rotary.axis, int(rotary.interleaved), layout, int(inverse))
+        return (out[0], None) if k is None else (out[0], out[1])
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        (positions,) = ctx.saved_tensors
+        rotary, layout, inverse = ctx.args
+        if grad_q is not None:                   # a rotation: the gradient is turned the other way
+            grad_q, grad_k = _Rotary.apply(grad_q, grad_k, positions, rotary, layout, not inverse)
+        elif grad_k is not None:
+            grad_k, _ = _Rotary.apply(grad_k, None, positions, rotary, layout, not inverse)
+        return grad_q, grad_k, None, None, None, None
+
+
+def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: RotaryAxes,
+                 tensor_layout: str = "HND") -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """q and k with every pair turned by its frequency times the token's position on the pair's axis.
+
+    q: ``[B,H,S,D]`` ("HND") or ``[B,S,H,D]`` ("NHD"), fp16 / bf16 / fp32; k likewise with its own number of heads, or
+    None (then only q is returned).  positions: int32 or int64 on the device, ``[S]`` or ``[B,S]`` for one axis, else
+    ``[S, axes]`` or ``[B, S, axes]``; any integers, negative ones too.  Returns new tensors; the arithmetic is fp32 with
+    one rounding at the end.  Differentiable in q and k."""
+    assert isinstance(rotary, RotaryAxes), "rotary must come from rotary_axes()."
+    assert q.dtype in (torch.float16, torch.bfloat16, torch.float32), "Input tensors must be fp16, bf16, or fp32."
+    assert tensor_layout in _LAYOUT_CODE, f"tensor_layout must be 'HND' or 'NHD', got {tensor_layout!r}."
+    assert q.dim() == 4 and q.size(3) == rotary.head_dim, f"q must be 4-D with head_dim {rotary.head_dim}, got {tuple(q.shape)}."
+    seq_dim = 2 if tensor_layout == "HND" else 1
+    B, S = q.size(0), q.size(seq_dim)
+    if k is not None:
+        assert k.device == q.device and k.dtype == q.dtype, "q and k must have the same device and dtype."
+        assert k.dim() == 4 and k.size(3) == q.size(3) and k.size(0) == B and k.size(seq_dim) == S, (
+            "q and k must have the same batch, length and head_dim (call twice for different lengths).")
+    assert rotary.freq.device == q.device, "the rotary table is on another device than q."
+    assert positions.device == q.device and positions.dtype in (torch.int32, torch.int64), (
+        "positions must be int32 or int64 on the device of q.")
+    n = rotary.n_axes
+    if n == 1 and tuple(positions.shape) in ((S,), (B, S)):
+        positions = positions.unsqueeze(-1)
+    assert tuple(positions.shape) in ((S, n), (B, S, n)), (
+        f"positions must be {'[S] or [B, S]' if n == 1 else '[S, axes] or [B, S, axes]'} with S = {S} and {n} axes, "
+        f"got {tuple(positions.shape)}.")
+    assert q.is_cuda, "Input tensors must be on a CUDA device."
+    if n > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    out = _Rotary.apply(q, k, positions, rotary, _LAYOUT_CODE[tensor_layout], False)
+    return out[0] if k is None else out
