@@ -80,6 +80,22 @@ typedef struct sage_rows {
 int sage_paged_append(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, const sage_rows_t* k, const sage_rows_t* v,
                       const sage_rows_t* q, const sage_rows_t* q_out, int Hq, const sage_rotary_t* rotary, int* status, void* stream);
 
+/* Attention of the new tokens over the cache: row t, head h of `o` = softmax(sm_scale q.k) v over the visible keys of the
+ * token's sequence - all of them, or with is_causal those up to the token's own position - and of kv head h / (Hq / Hkv).
+ * A row that sees no key is 0, its log-sum-exp -inf.
+ * o: 16-bit rows like q, in any strides.  lse (optional): [T, Hq] fp32, contiguous, natural log.
+ * Hq: a multiple of Hkv, at most 128 times it.  max_q: an upper bound of the new tokens of a sequence, 0 if not known (it
+ * chooses the kernel; a wrong one costs time only).
+ * shared_pages (optional): n_shared page indices on the device.  The first n_shared * page_size keys of EVERY sequence are
+ * in these pages; the first n_shared columns of page_table are not looked at.  The result is the same as with them in
+ * the table, but these keys and values are read once for all sequences.
+ * zero_rest: rows of o (lse) that belong to no sequence are set to 0 (-inf); 0: they are left as they are.
+ * workspace: sage_paged_workspace_bytes() bytes, 16-byte aligned; it belongs to the call until that has completed. */
+int64_t sage_paged_workspace_bytes(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, int Hq, int max_q, int n_shared);
+int sage_paged_attn(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, const sage_rows_t* q, const sage_rows_t* o, int Hq,
+                    int max_q, int is_causal, float sm_scale, float* lse, const int32_t* shared_pages, int n_shared, int zero_rest,
+                    int* status, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

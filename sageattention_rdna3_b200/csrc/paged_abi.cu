@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "host_common.h"
+#include "paged_rows_kernel.cuh"
 #include "rotary_kernels.cuh"
 
 using namespace sage_host;
@@ -101,7 +102,7 @@ int check_cache(const sage_paged_kv_t* c) {
 int check_batch(const sage_paged_batch_t* b) {
   SAGE_REQUIRE(b->B >= 0 && b->T >= 0, "negative sizes");
   SAGE_REQUIRE(b->cu_q != nullptr || b->T == b->B, "without cu_q every sequence has one token: T must be B");
-  SAGE_REQUIRE(b->B == 0 || (b->kv_lens != nullptr && b->page_table != nullptr), "null kv_lens or page_table");
+  SAGE_REQUIRE(b->B == 0 || (b->kv_lens != nullptr && (b->page_table != nullptr || b->table_width == 0)), "null kv_lens or page_table");
   SAGE_REQUIRE(b->table_width >= 0 && b->table_stride >= 0, "negative extent of the page table");
   return SAGE_OK;
 }
@@ -121,9 +122,154 @@ Batch batch_of(const sage_paged_batch_t* b, const sage_paged_kv_t* c) {
   return x;
 }
 
+// One pass of attention over the cache: which kernel, how many CTAs, and what it needs of the workspace.
+struct PagedPlan {
+  int tile_rows = 0;
+  int grid = 0;
+  bool merge = false;           // an item may be cut
+  int64_t header_bytes = 0, e_bytes = 0, o_bytes = 0;
+  int64_t bytes() const { return header_bytes + e_bytes + o_bytes; }
+};
+int64_t round16(int64_t n) { return (n + 15) & ~int64_t{15}; }
+
+// seqs: sequences of the pass, max_q: new tokens of one of them, tokens: of all; max_keys: keys of one.
+int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t tokens, int64_t max_q, int64_t max_keys, int group) {
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc) return rc;
+  *plan = PagedPlan();
+  const int64_t rows = std::min(max_q, tokens) * group;
+  plan->tile_rows = rows <= 16 ? 16 : 32;
+  const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
+  const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
+  plan->grid = static_cast<int>(std::min<int64_t>(sms, std::min<int64_t>(row_tiles * c->Hkv, sms) * tiles));
+  plan->merge = tiles > 1;
+  plan->header_bytes = round16(static_cast<int64_t>(plan->grid) * sizeof(PartHeader));
+  plan->e_bytes = round16(static_cast<int64_t>(plan->grid) * 2 * plan->tile_rows * sizeof(float));
+  plan->o_bytes = plan->merge ? static_cast<int64_t>(plan->grid) * 2 * plan->tile_rows * c->D * static_cast<int64_t>(sizeof(float)) : 0;
+  return SAGE_OK;
+}
+
+struct CallPlan {
+  PagedPlan own, shared;
+  int64_t joined_o_bytes = 0, joined_e_bytes = 0;     // what the sequences' own keys give, before the shared ones join
+  int64_t bytes() const { return std::max(own.bytes(), shared.bytes()) + joined_o_bytes + joined_e_bytes; }
+};
+int plan_call(CallPlan* plan, const sage_paged_kv_t* c, const sage_paged_batch_t* b, int Hq, int max_q, int n_shared) {
+  const int group = Hq / c->Hkv;
+  int longest = b->cu_q == nullptr ? 1 : b->T;
+  if (max_q > 0) longest = std::min(longest, max_q);
+  const int64_t own_keys = static_cast<int64_t>(std::max(0, b->table_width - n_shared)) * c->page_size;
+  int rc = plan_pass(&plan->own, c, b->B, b->T, longest, own_keys, group);
+  if (rc || n_shared == 0) return rc;
+  rc = plan_pass(&plan->shared, c, 1, b->T, b->T, static_cast<int64_t>(n_shared) * c->page_size, group);
+  plan->joined_o_bytes = static_cast<int64_t>(b->T) * Hq * c->D * static_cast<int64_t>(sizeof(float));
+  plan->joined_e_bytes = round16(static_cast<int64_t>(b->T) * Hq * sizeof(float));
+  return rc;
+}
+
+template <typename T, int D, int MT>
+int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& p, const PagedPlan& plan, cudaStream_t stream) {
+  constexpr int kSmem = RowsSmem<D, MT>::kTotal;
+  static std::atomic<bool> configured[64];
+  const int rc = configure_smem(sage_paged_rows_kernel<T, D, MT>, kSmem, configured);
+  if (rc) return rc;
+  return launch(sage_paged_rows_kernel<T, D, MT>, static_cast<unsigned>(plan.grid), kRowsThreads, kSmem, stream, tk, tv, p);
+}
+
+template <typename T, int D>
+int launch_pass(const sage_paged_kv_t* c, AttnParams p, const PagedPlan& plan, char* workspace, cudaStream_t stream) {
+  p.tile_rows = plan.tile_rows;
+  p.headers = reinterpret_cast<PartHeader*>(workspace);
+  p.part_e = reinterpret_cast<float*>(workspace + plan.header_bytes);
+  p.part_o = reinterpret_cast<float*>(workspace + plan.header_bytes + plan.e_bytes);
+  const CUtensorMapDataType dt = c->dtype == SAGE_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const int box_rows = std::min(c->page_size, kUnitKeys);
+  CUtensorMap tk, tv;
+  int rc = encode_strided_16bit(&tk, dt, c->k, D, c->page_size, c->Hkv, c->num_pages, c->k_stride_slot, c->k_stride_head, c->k_stride_page, box_rows, "k_pages");
+  if (rc) return rc;
+  rc = encode_strided_16bit(&tv, dt, c->v, D, c->page_size, c->Hkv, c->num_pages, c->v_stride_slot, c->v_stride_head, c->v_stride_page, box_rows, "v_pages");
+  if (rc) return rc;
+  rc = plan.tile_rows == 16 ? launch_rows<T, D, 1>(tk, tv, p, plan, stream) : launch_rows<T, D, 2>(tk, tv, p, plan, stream);
+  if (rc || !plan.merge) return rc;
+  return launch(sage_paged_merge_kernel<T, D, 2>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>(plan.tile_rows / 2)), kMergeThreads, 0, stream, p);
+}
+
+int dispatch_pass(const sage_paged_kv_t* c, const AttnParams& p, const PagedPlan& plan, char* workspace, cudaStream_t stream) {
+  if (c->dtype == SAGE_DTYPE_F16) return c->D == 64 ? launch_pass<__half, 64>(c, p, plan, workspace, stream) : launch_pass<__half, 128>(c, p, plan, workspace, stream);
+  return c->D == 64 ? launch_pass<__nv_bfloat16, 64>(c, p, plan, workspace, stream) : launch_pass<__nv_bfloat16, 128>(c, p, plan, workspace, stream);
+}
+
+int check_attn(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, int Hq, int max_q, int n_shared) {
+  SAGE_REQUIRE(cache != nullptr && batch != nullptr, "paged attention: null argument");
+  int rc = check_cache(cache);
+  if (rc) return rc;
+  rc = check_batch(batch);
+  if (rc) return rc;
+  SAGE_REQUIRE(Hq >= 1 && Hq % cache->Hkv == 0 && Hq / cache->Hkv <= 128, "num_qo_heads must be a multiple of num_kv_heads, at most 128 times it; got %d and %d", Hq, cache->Hkv);
+  SAGE_REQUIRE(max_q >= 0 && n_shared >= 0, "negative sizes");
+  SAGE_REQUIRE(static_cast<int64_t>(n_shared) * cache->page_size <= 0x3fffffff && static_cast<int64_t>(batch->table_width) * cache->page_size <= 0x3fffffff,
+               "a sequence may have at most 2^30 keys");
+  SAGE_REQUIRE(n_shared <= batch->table_width || batch->B == 0, "the page table has fewer columns than there are shared pages");
+  return SAGE_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int64_t sage_paged_workspace_bytes(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, int Hq, int max_q, int n_shared) {
+  if (check_attn(cache, batch, Hq, max_q, n_shared) != SAGE_OK) return -1;
+  if (batch->T == 0 || batch->B == 0) return 0;
+  CallPlan plan;
+  return plan_call(&plan, cache, batch, Hq, max_q, n_shared) == SAGE_OK ? plan.bytes() : -1;
+}
+
+int sage_paged_attn(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, const sage_rows_t* q, const sage_rows_t* o, int Hq,
+                    int max_q, int is_causal, float sm_scale, float* lse, const int32_t* shared_pages, int n_shared, int zero_rest,
+                    int* status, void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_attn(cache, batch, Hq, max_q, n_shared);
+  if (rc) return rc;
+  SAGE_REQUIRE(q != nullptr && o != nullptr, "paged attention: null argument");
+  if (batch->T == 0 || batch->B == 0) return SAGE_OK;
+  SAGE_REQUIRE(rows_ok(q) && rows_ok(o), "paged attention: rows need a 16-byte aligned base and strides that are multiples of 8 elements");
+  SAGE_REQUIRE(n_shared == 0 || shared_pages != nullptr, "paged attention: null shared_pages");
+  CallPlan plan;
+  rc = plan_call(&plan, cache, batch, Hq, max_q, n_shared);
+  if (rc) return rc;
+  SAGE_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes(),
+               "paged attention: the workspace must be 16-byte aligned and have %lld bytes", static_cast<long long>(plan.bytes()));
+  AttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = q->ptr; p.q_stride_t = q->stride_t; p.q_stride_h = q->stride_h;
+  p.o = const_cast<void*>(o->ptr); p.o_stride_t = o->stride_t; p.o_stride_h = o->stride_h;
+  p.lse = lse;
+  p.batch = batch_of(batch, cache);
+  p.status = status_of(status);
+  p.shared_len = n_shared * cache->page_size;
+  p.shared_pages = shared_pages;
+  p.Hq = Hq; p.Hkv = cache->Hkv; p.group = Hq / cache->Hkv;
+  p.causal = is_causal != 0;
+  p.zero_rest = zero_rest != 0;
+  p.score_scale = sm_scale * 1.4426950408889634f;
+  p.wait_limit_cycles = g_wait_limit_cycles.load(std::memory_order_relaxed);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  if (n_shared == 0) return dispatch_pass(cache, p, plan.own, ws, st);
+  // The sequences' own keys first, into fp32; the pass over the shared keys joins them on writing the output.
+  AttnParams own = p;
+  own.o = nullptr;
+  own.lse = nullptr;
+  own.zero_rest = 0;
+  own.o32 = reinterpret_cast<float*>(ws + std::max(plan.own.bytes(), plan.shared.bytes()));
+  own.e32 = own.o32 + static_cast<int64_t>(batch->T) * Hq * cache->D;
+  rc = dispatch_pass(cache, own, plan.own, ws, st);
+  if (rc) return rc;
+  p.shared_pass = 1;
+  p.prior_o = own.o32;
+  p.prior_e = own.e32;
+  return dispatch_pass(cache, p, plan.shared, ws, st);
+}
 
 int sage_apply_rotary(const sage_strided_t* q, const sage_strided_t* q_out, const sage_strided_t* k, const sage_strided_t* k_out,
                       const sage_rotary_t* rotary, int dtype, int B, int Hq, int Hkv, int S, int D, int inverse, void* stream) {

@@ -15,6 +15,8 @@ namespace paged {
 
 constexpr int kStatusBadPage = SAGE_STATUS_BAD_PAGE;
 constexpr int kStatusBadLength = SAGE_STATUS_BAD_LENGTH;
+constexpr int kStatusMisaligned = 1;                  // as attn_kernel.cuh
+constexpr int kStatusWait = 2 + 16 * 20;              // ... and its numbering of waits: 20, a load of keys and values
 
 struct Status {
   int* word;                    // optional device word, stays 0 on success

@@ -1,0 +1,401 @@
+// How attention over a paged cache is cut into work for a fixed grid, without the host knowing a length.
+//
+// An item is one row tile of one kv head of one sequence: up to `tile_rows` rows (new token, query head of the group) that
+// read the same keys.  Its steps are tiles of 128 keys, at least one (an item without keys writes zeros).  The steps of all items,
+// sequence after sequence, kv head after kv head, row tile after row tile, form one line that is cut into equal spans, one per CTA:
+// lengths may differ as they like and all CTAs get the same number of tiles.  A span that covers part of an item leaves
+// its result in a slot of the workspace (slot 1 the head of an item, slot 0 anything else: at most one of each per
+// CTA) and a header that tells sage_paged_merge_kernel which parts follow.  Every CTA works this out for itself from kv_lens and
+// cu_q, by a block-wide prefix sum; nothing is communicated and the order of all sums is fixed.
+#pragma once
+
+#include "paged_common.cuh"
+
+namespace sage {
+namespace paged {
+
+constexpr int kTileKeys = 128;
+
+struct AttnParams {
+  const void* q;
+  long long q_stride_t, q_stride_h;
+  void* o;                      // 16-bit output, or null: `o32` is written
+  long long o_stride_t, o_stride_h;
+  float* o32;                   // [T, Hq, D] fp32 and [T, Hq] base-2 log-sum-exp: the result as one part of a larger one
+  float* e32;
+  const float* prior_o;         // ... and such a part to be merged with on writing `o`, or null
+  const float* prior_e;
+  float* lse;                   // optional [T, Hq], natural log
+  Batch batch;                  // of the sequences; cu_q and kv_lens also give the visible keys of every row
+  Status status;
+  const int32_t* shared_pages;  // keys [0, shared_len) of every sequence, or null
+  int shared_len;
+  int shared_pass;              // 1: one sequence of all T tokens against the shared keys; 0: every sequence against its keys behind them
+  int Hq, Hkv, group;           // group = Hq / Hkv
+  int tile_rows;                // rows of a row tile
+  int causal;
+  int zero_rest;                // write zeros to rows that belong to no sequence
+  float score_scale;            // sm_scale * log2(e)
+  float* part_o;                // [grid][2][tile rows][D] fp32
+  float* part_e;                // [grid][2][tile rows]
+  struct PartHeader* headers;   // [grid]
+  long long wait_limit_cycles;
+};
+
+struct PartHeader {             // of the part in slot 1 of a CTA, if it is the head of an item that others finish
+  int n_parts;                  // 0: none
+  int token0, tokens;           // new tokens of the sequence: rows [token0, token0 + tokens)
+  int head0;                    // first query head of the group
+  int row0;                     // first row of the tile, counted (token, head of the group) from the sequence's first token
+  int rows;                     // rows in the tile
+  int pad[2];
+};
+
+// One sequence as the schedule sees it.
+struct Seq {
+  int q0, n_q;                  // new tokens
+  int key0, len;                // keys [key0, len)
+  int row_tiles, key_tiles;
+};
+
+__device__ __forceinline__ int n_seqs(const AttnParams& p) { return p.shared_pass ? 1 : p.batch.B; }
+
+__device__ __forceinline__ int clipped_len(const AttnParams& p, int b) {
+  const long long most = static_cast<long long>(p.batch.table_width) << p.batch.page_log2;
+  return static_cast<int>(min(static_cast<long long>(max(p.batch.kv_lens[b], 0)), most));
+}
+
+__device__ __forceinline__ Seq seq_at(const AttnParams& p, int b) {
+  Seq s;
+  if (p.shared_pass) {
+    s.q0 = 0;
+    s.n_q = p.batch.T;
+    s.key0 = 0;
+    s.len = p.shared_len;
+  } else {
+    int q1;
+    p.batch.tokens(b, &s.q0, &q1);
+    s.n_q = q1 - s.q0;
+    s.key0 = p.shared_len;
+    s.len = clipped_len(p, b);
+  }
+  s.row_tiles = static_cast<int>((static_cast<long long>(s.n_q) * p.group + p.tile_rows - 1) / p.tile_rows);
+  s.key_tiles = max(1, (s.len - s.key0 + kTileKeys - 1) / kTileKeys);
+  return s;
+}
+
+__device__ __forceinline__ long long steps_of(const AttnParams& p, const Seq& s) {
+  return static_cast<long long>(s.row_tiles) * s.key_tiles * p.Hkv;
+}
+
+// Keys that a new token sees: [0, limit).
+__device__ __forceinline__ int visible_keys(const AttnParams& p, int b, int q1, int token) {
+  const int len = clipped_len(p, b);
+  return p.causal ? max(0, len - (q1 - 1 - token)) : len;
+}
+// The sequence of a token, by search (the shared pass, where a row tile spans sequences); B if it belongs to none.
+__device__ __forceinline__ int seq_of_token(const AttnParams& p, int token, int* q1) {
+  if (p.batch.cu_q == nullptr) {
+    *q1 = token + 1;
+    return token;
+  }
+  int lo = 0, hi = p.batch.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (p.batch.cu_q[mid] <= token) lo = mid;
+    else hi = mid;
+  }
+  int q0;
+  p.batch.tokens(lo, &q0, q1);
+  return token >= q0 && token < *q1 ? lo : p.batch.B;
+}
+
+// The span of a CTA and where it starts; found once by all threads together.
+struct Span {
+  long long t, t_end;           // steps
+  long long total;
+  int ctas;                     // CTAs that have steps at all
+  int b;                        // sequence of step t ...
+  long long before;             // ... and the steps before that sequence
+};
+
+// `scratch`: shared memory for kThreads / 32 + 4 long longs.  Ends with a barrier.
+template <int kThreads>
+__device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratch) {
+  const int n = n_seqs(p);
+  const int per = (n + kThreads - 1) / kThreads;
+  const int first = threadIdx.x * per, last = min(first + per, n);
+  long long mine = 0;
+  for (int b = first; b < last; ++b) {
+    mine += steps_of(p, seq_at(p, b));
+    if (blockIdx.x == 0 && !p.shared_pass && p.batch.kv_lens[b] > clipped_len(p, b)) p.status.report(kStatusBadLength);
+  }
+  long long upto = mine;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += other;
+  }
+  if (lane == 31) scratch[warp] = upto;
+  __syncthreads();
+  long long total = 0, base = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) base += scratch[w];
+    total += scratch[w];
+  }
+  upto += base;
+  Span s;
+  s.total = total;
+  s.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  const bool idle = static_cast<int>(blockIdx.x) >= s.ctas;
+  s.t = idle ? 0 : total * blockIdx.x / s.ctas;
+  s.t_end = idle ? 0 : total * (blockIdx.x + 1) / s.ctas;
+  // The thread whose sequences hold step t walks through them.
+  if (!idle && s.t >= upto - mine && s.t < upto) {
+    long long before = upto - mine;
+    int b = first;
+    while (true) {
+      const long long steps = steps_of(p, seq_at(p, b));
+      if (s.t < before + steps) break;
+      before += steps;
+      ++b;
+    }
+    scratch[kThreads / 32] = b;
+    scratch[kThreads / 32 + 1] = before;
+  }
+  __syncthreads();
+  s.b = idle ? 0 : static_cast<int>(scratch[kThreads / 32]);
+  s.before = idle ? 0 : scratch[kThreads / 32 + 1];
+  return s;
+}
+
+// A part of a span that belongs to one item.
+struct Segment {
+  Seq seq;
+  int b, head, row_tile;        // kv head
+  int tile, n_tiles;            // key tiles [tile, tile + n_tiles)
+  int slot;                     // -1: the whole item; 1: its head, 0: another part
+  int n_parts;                  // slot 1: parts of the item
+};
+
+// Walks through a span.  Every thread that uses one gets the same segments.
+struct SegmentIter {
+  const AttnParams& p;
+  Span s;
+  Seq seq;
+  long long steps;              // of seq
+  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span) {
+    if (s.t < s.t_end) {
+      seq = seq_at(p, s.b);
+      steps = steps_of(p, seq);
+    }
+  }
+  __device__ __forceinline__ bool next(Segment* g) {
+    if (s.t >= s.t_end) return false;
+    while (s.t >= s.before + steps) {                 // (sequences without new tokens have no steps)
+      s.before += steps;
+      seq = seq_at(p, ++s.b);
+      steps = steps_of(p, seq);
+    }
+    const long long r = s.t - s.before;
+    const long long item = r / seq.key_tiles;
+    g->seq = seq;
+    g->b = s.b;
+    g->head = static_cast<int>(item / seq.row_tiles);
+    g->row_tile = static_cast<int>(item - static_cast<long long>(g->head) * seq.row_tiles);
+    g->tile = static_cast<int>(r - item * seq.key_tiles);
+    const long long left = s.t_end - s.t;
+    g->n_tiles = static_cast<int>(min(static_cast<long long>(seq.key_tiles - g->tile), left));
+    g->n_parts = 1;
+    if (g->tile > 0) {
+      g->slot = 0;
+    } else if (g->n_tiles == seq.key_tiles) {
+      g->slot = -1;
+    } else {
+      g->slot = 1;
+      // the CTA that owns the last step e of the item: the largest c with total * c / ctas <= e
+      const long long e = s.t + seq.key_tiles - 1;
+      const long long c = ((e + 1) * s.ctas - 1) / s.total;
+      g->n_parts = static_cast<int>(c) - static_cast<int>(blockIdx.x) + 1;
+    }
+    s.t += g->n_tiles;
+    return true;
+  }
+};
+
+// Row r of a tile -> new token (counted in the batch) and query head; false if the row is empty.
+__device__ __forceinline__ bool row_at(int token0, int tokens, int head0, int group, int row0, int rows, int r, int* token, int* head) {
+  if (r >= rows) return false;
+  const int flat = row0 + r;
+  const int i = flat / group;
+  *token = token0 + i;
+  *head = head0 + flat - i * group;
+  return i < tokens;
+}
+
+// Base-2 log-sum-exp of a part with maximum m and sum l.  A part that is not a number gets +inf, which fmaxf keeps where it
+// would drop a NaN: the weights of all parts of the row become NaN then.
+__device__ __forceinline__ float part_lse(float m, float l) {
+  const float e = m + log2f(l);
+  return l == 0.0f ? -INFINITY : e != e ? INFINITY : e;
+}
+
+// Joins a finished row with what is already known of it: both normalised, with their base-2 log-sum-exp.
+__device__ __forceinline__ void join_weights(float e, float prior, float* w, float* w_prior, float* joined) {
+  const float top = fmaxf(e, prior);
+  if (e == -INFINITY && prior == -INFINITY) {
+    *w = *w_prior = 0.0f;
+    *joined = -INFINITY;
+    return;
+  }
+  const float a = exp2f(e - top), b = exp2f(prior - top), sum = a + b;
+  *w = a / sum;
+  *w_prior = b / sum;
+  *joined = top + log2f(sum);
+}
+
+// Writes N neighbouring values of a finished row: normalised `x`, log-sum-exp e (base 2).
+template <typename T, int N>
+__device__ __forceinline__ void write_row(const AttnParams& p, int token, int head, int D, int col, float (&x)[N], float e, bool with_lse) {
+  const long long row = static_cast<long long>(token) * p.Hq + head;
+  if (p.o == nullptr) {
+    float* dst = p.o32 + row * D + col;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(x[i], x[i + 1]);
+    if (with_lse) p.e32[row] = e;
+    return;
+  }
+  if (p.prior_o != nullptr) {
+    float w, wp, joined;
+    join_weights(e, p.prior_e[row], &w, &wp, &joined);
+    const float* src = p.prior_o + row * D + col;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 y = *reinterpret_cast<const float2*>(src + i);
+      x[i] = w * x[i] + wp * y.x;
+      x[i + 1] = w * x[i + 1] + wp * y.y;
+    }
+    e = joined;
+  }
+  T* dst = static_cast<T*>(p.o) + token * p.o_stride_t + head * p.o_stride_h + col;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = from_float2(x[i], x[i + 1], static_cast<const T*>(nullptr));
+  if (with_lse && p.lse != nullptr) p.lse[row] = e * 0.6931471805599453f;      // (-inf stays -inf)
+}
+
+// Rows that belong to no sequence, as the calling CTA's share of them.  `threads` threads take part, this one is `thread`.
+template <typename T>
+__device__ __forceinline__ void zero_rest(const AttnParams& p, int D, int thread, int threads) {
+  if (!p.zero_rest || p.batch.cu_q == nullptr) return;
+  const int first = min(max(p.batch.cu_q[0], 0), p.batch.T), last = min(max(p.batch.cu_q[p.batch.B], 0), p.batch.T);
+  const int rest = first + p.batch.T - last;
+  const int vecs = p.Hq * (D / 8);
+  for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+    const int token = i < first ? i : last + i - first;
+    for (int v = thread; v < vecs; v += threads) {
+      const int head = v / (D / 8);
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + token * p.o_stride_t + head * p.o_stride_h + (v - head * (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+      if (p.lse != nullptr && v % (D / 8) == 0) p.lse[static_cast<long long>(token) * p.Hq + head] = -INFINITY;
+    }
+  }
+}
+
+// One CTA: part `blockIdx.y` of the rows of header `blockIdx.x`.  A warp per row and group of parts; the kRowWarps warps of a row
+// take every kRowWarps-th part, four in flight, and are joined in shared memory in a fixed order.
+constexpr int kMergeThreads = 256;
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_kernel(const AttnParams p) {
+  constexpr int kWarps = kMergeThreads / 32, kRowWarps = kWarps / ROWS, kPer = D / 32;   // values per lane: 4 or 2
+  __shared__ float s_o[kWarps][D];
+  __shared__ float s_e[kWarps];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const PartHeader h = p.headers[blockIdx.x];
+  if (h.n_parts < 2) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * ROWS + warp / kRowWarps, w = warp % kRowWarps;
+  int token = 0, head = 0;
+  bool live = row_at(h.token0, h.tokens, h.head0, p.group, h.row0, h.rows, r, &token, &head);
+  if (live && p.shared_pass) {
+    int q1;
+    live = seq_of_token(p, token, &q1) < p.batch.B;
+  }
+  float e = -INFINITY, sum = 0.0f, x[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
+  if (live) {
+    for (int k0 = w; k0 < h.n_parts; k0 += 4 * kRowWarps) {
+      float pe[4], px[4][kPer];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int k = k0 + c * kRowWarps;
+        pe[c] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) px[c][i] = 0.0f;
+        if (k < h.n_parts) {
+          const long long at = ((static_cast<long long>(blockIdx.x) + k) * 2 + (k == 0 ? 1 : 0)) * p.tile_rows + r;
+          pe[c] = p.part_e[at];
+          const float* src = p.part_o + at * D + lane * kPer;
+          if constexpr (kPer == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            px[c][0] = v.x; px[c][1] = v.y; px[c][2] = v.z; px[c][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            px[c][0] = v.x; px[c][1] = v.y;
+          }
+        }
+      }
+      float top = e;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) top = fmaxf(top, pe[c]);
+      if (top == -INFINITY) continue;                 // no visible keys so far
+      const float back = exp2f(e - top);
+      sum *= back;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] *= back;
+      e = top;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float f = exp2f(pe[c] - top);
+        sum += f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] += f * px[c][i];
+      }
+    }
+  }
+  // e: the maximum; the row is x / sum, its log-sum-exp e + log2(sum)
+  if constexpr (kRowWarps > 1) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s_o[warp][lane * kPer + i] = x[i] * inv;
+    if (lane == 0) s_e[warp] = part_lse(e, sum);
+    __syncthreads();
+    if (w != 0 || !live) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kRowWarps; ++c) top = fmaxf(top, s_e[warp + c]);
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
+    e = top;
+    if (top > -INFINITY) {
+#pragma unroll
+      for (int c = 0; c < kRowWarps; ++c) {
+        const float f = exp2f(s_e[warp + c] - top);
+        sum += f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] += f * s_o[warp + c][lane * kPer + i];
+      }
+    }
+  }
+  if (!live) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) x[i] *= inv;
+  write_row<T, kPer>(p, token, head, D, lane * kPer, x, sum == 0.0f ? -INFINITY : e + log2f(sum), lane == 0);
+}
+
+}  // namespace paged
+}  // namespace sage

@@ -206,6 +206,41 @@ std::vector<at::Tensor> paged_append(at::Tensor& k_pages, at::Tensor& v_pages, i
   return out;
 }
 
+// paged_attn(Tensor query, Tensor(a!) output, Tensor k_pages, Tensor v_pages, int tensor_layout, Tensor page_table, Tensor kv_lens,
+//            Tensor? cu_q, int max_q, int is_causal, float sm_scale, Tensor? lse, Tensor? shared_pages, int zero_rest, Tensor status) -> ()
+void paged_attn(const at::Tensor& q, at::Tensor& o, const at::Tensor& k_pages, const at::Tensor& v_pages, int64_t layout,
+                const at::Tensor& page_table, const at::Tensor& kv_lens, const c10::optional<at::Tensor>& cu_q, int64_t max_q,
+                int64_t is_causal, double sm_scale, const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& shared_pages,
+                int64_t zero_rest, const at::Tensor& status) {
+  const sage_paged_kv_t cache = cache_of(k_pages, v_pages, layout);
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  check_rows(q, k_pages, -1, "query");
+  check_rows(o, k_pages, q.size(1), "output");
+  TORCH_CHECK(o.size(0) == q.size(0), "query and output differ in length");
+  const sage_paged_batch_t batch = batch_of(page_table, kv_lens, cu_q, q.size(0), k_pages);
+  const int Hq = size_of(q.size(1), "heads"), longest = size_of(max_q, "max_q");
+  int n_shared = 0;
+  if (shared_pages.has_value()) {
+    TORCH_CHECK(shared_pages->dim() == 1, "shared_pages must be 1-D");
+    check_int32(*shared_pages, k_pages, "shared_pages");
+    n_shared = size_of(shared_pages->size(0), "shared pages");
+  }
+  float* lse_ptr = nullptr;
+  if (lse.has_value()) {
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->numel() == q.size(0) * q.size(1) && lse->device() == q.device(),
+                "lse must be a contiguous fp32 [T, heads] tensor");
+    lse_ptr = lse->data_ptr<float>();
+  }
+  const int64_t bytes = sage_paged_workspace_bytes(&cache, &batch, Hq, longest, n_shared);
+  TORCH_CHECK(bytes >= 0, "paged_attn failed: ", sage_last_error());
+  at::Tensor workspace = at::empty({bytes}, k_pages.options().dtype(at::kByte));
+  const sage_rows_t qs = rows_of(q), os = rows_of(o);
+  check_rc(sage_paged_attn(&cache, &batch, &qs, &os, Hq, longest, is_causal != 0, static_cast<float>(sm_scale), lse_ptr,
+                           n_shared > 0 ? shared_pages->data_ptr<int32_t>() : nullptr, n_shared, zero_rest != 0,
+                           status_of(status, k_pages), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, current_stream(k_pages)),
+           "paged_attn");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(sageattention, m) {
@@ -214,9 +249,13 @@ TORCH_LIBRARY_FRAGMENT(sageattention, m) {
   m.def("paged_append(Tensor(a!) k_pages, Tensor(b!) v_pages, int tensor_layout, Tensor key, Tensor value, Tensor page_table, "
         "Tensor kv_lens, Tensor? cu_q, Tensor? query, Tensor? freq, Tensor? axis, int n_axes, int interleaved, Tensor? positions, "
         "Tensor status) -> Tensor[]");
+  m.def("paged_attn(Tensor query, Tensor(a!) output, Tensor k_pages, Tensor v_pages, int tensor_layout, Tensor page_table, "
+        "Tensor kv_lens, Tensor? cu_q, int max_q, int is_causal, float sm_scale, Tensor? lse, Tensor? shared_pages, int zero_rest, "
+        "Tensor status) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(sageattention, CUDA, m) {
   m.impl("rotary", &rotary);
   m.impl("paged_append", &paged_append);
+  m.impl("paged_attn", &paged_attn);
 }

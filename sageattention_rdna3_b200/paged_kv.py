@@ -15,7 +15,7 @@ device: no call synchronises, and every call can be captured in a CUDA graph.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Union
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -152,3 +152,61 @@ def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table
                            None if rotary is None else rotary.axis, 0 if rotary is None else rotary.n_axes,
                            0 if rotary is None else int(rotary.interleaved), positions, _status_word(dev))
     return out[0] if q is not None else None
+
+
+def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                   cu_q: Optional[torch.Tensor] = None, max_q: Optional[int] = None, is_causal: bool = True,
+                   sm_scale: Optional[float] = None, return_lse: bool = False, shared_pages: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention of the newest tokens of every sequence over its keys and values in the cache.
+
+    q: ``[T, Hq, D]`` in the dtype of the cache, the tokens that ``paged_kv_append`` stored last (Hq a multiple of the cache's
+    heads, at most 128 times them).  kv_lens: ``[B]`` int32, keys of every sequence with its new tokens.  ``cu_q`` as in
+    ``paged_kv_append``; ``max_q``, if the program knows it, is an upper bound of the new tokens of one sequence and helps to choose
+    the kernel.  ``is_causal`` aligns the last new token with the last key (a token sees the keys up to its own
+    position); without it every token sees all keys of its sequence.  A row without keys is zero, its log-sum-exp -inf.
+
+    shared_pages: ``[n]`` int32.  The first ``n * page_size`` keys of every sequence stand in these pages (a system
+    prompt, one question with many answers); they are read once for the whole batch, and the first n columns of ``page_table``
+    are not looked at.  Positions and ``kv_lens`` count them as ever, and the result is the same as without the argument, up to
+    rounding.
+
+    Returns ``[T, Hq, D]``, with ``return_lse`` also the natural log-sum-exp ``[T, Hq]`` (fp32).  Rows that belong to no sequence are
+    zero (-inf); given ``out``, which receives the result, they are left as they were there.  Keys and values behind a
+    sequence's last one may be anything, NaN too.  Lengths beyond the page table are cut to it, page indices
+    outside the cache are read as page 0, and both are reported like the errors of ``sageattn``, by the next call or
+    ``check_status()``.  No gradient."""
+    _check_batch(cache, q, page_table, kv_lens, cu_q)
+    _check_rows(cache, "q", q)
+    T, heads, B = q.size(0), q.size(1), kv_lens.size(0)
+    assert heads > 0 and heads % cache.num_kv_heads == 0 and heads // cache.num_kv_heads <= 128, (
+        f"num_qo_heads must be a multiple of num_kv_heads, at most 128 times it; got {heads} and {cache.num_kv_heads}.")
+    assert max_q is None or max_q >= 0, f"max_q must not be negative, got {max_q}."
+    dev = cache.k_pages.device
+    if shared_pages is not None:
+        assert shared_pages.dtype == torch.int32 and shared_pages.device == dev and shared_pages.dim() == 1, (
+            "shared_pages must be a 1-D int32 tensor on the device of the cache.")
+        assert shared_pages.size(0) <= 1 or shared_pages.stride(0) == 1, "shared_pages must be contiguous."
+        assert shared_pages.size(0) <= page_table.size(1), "page_table has fewer columns than there are shared pages."
+    if out is not None:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, (
+            "out must have the shape, dtype and device of q.")
+        assert out.stride(2) == 1 and out.data_ptr() % 16 == 0 and all(
+            n <= 1 or s % 8 == 0 for n, s in zip(out.shape[:2], out.stride()[:2])), (
+            f"out needs a contiguous last dim and 16-byte aligned rows; got strides {out.stride()}.")
+    assert dev.type == "cuda", "the cache must be on a CUDA device."
+    ops = _native.load_ops()
+    _raise_pending(dev)
+    zero_rest = out is None and cu_q is not None
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev) if B > 0 else torch.zeros(q.shape, dtype=q.dtype, device=dev)
+    lse = None
+    if return_lse:
+        lse = torch.empty(T, heads, dtype=torch.float32, device=dev)
+        if B == 0 or (cu_q is not None and not zero_rest):
+            lse.fill_(float("-inf"))
+    ops.paged_attn(_vector_aligned(q), out, cache.k_pages, cache.v_pages, _LAYOUT_CODE[cache.tensor_layout], page_table, kv_lens,
+                   cu_q, 0 if max_q is None else int(max_q), int(is_causal),
+                   cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale), lse, shared_pages, int(zero_rest),
+                   _status_word(dev))
+    return (out, lse) if return_lse else out
