@@ -84,7 +84,7 @@ def build_abi(force: bool = False, verbose: bool = False) -> Path:
     attn = [*common, CSRC / "attn_kernel.cuh", CSRC / "prep_kernels.cuh", CSRC / "merge_kernels.cuh", CSRC / "pair_kernel.cuh",
             CSRC / "internal.h"]
     paged = [*common, CSRC / "paged_common.cuh", CSRC / "rotary_kernels.cuh", CSRC / "paged_schedule.cuh",
-             CSRC / "paged_rows_kernel.cuh", REPO_DIR / "include" / "sage_paged_b200.h"]
+             CSRC / "paged_rows_kernel.cuh", CSRC / "paged_tile_kernel.cuh", REPO_DIR / "include" / "sage_paged_b200.h"]
     units = [(CSRC / "sage_abi.cu", attn), (CSRC / "paged_abi.cu", paged)]
     sources = sorted({f for unit, headers in units for f in (unit, *headers)})
     if force or not _up_to_date(LIB_ABI, sources):

@@ -5,7 +5,7 @@
 #include <algorithm>
 
 #include "host_common.h"
-#include "paged_rows_kernel.cuh"
+#include "paged_tile_kernel.cuh"
 #include "rotary_kernels.cuh"
 
 using namespace sage_host;
@@ -124,6 +124,7 @@ Batch batch_of(const sage_paged_batch_t* b, const sage_paged_kv_t* c) {
 
 // One pass of attention over the cache: which kernel, how many CTAs, and what it needs of the workspace.
 struct PagedPlan {
+  bool tensor = false;          // sage_paged_tile_kernel
   int tile_rows = 0;
   int grid = 0;
   bool merge = false;           // an item may be cut
@@ -139,10 +140,12 @@ int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t t
   if (rc) return rc;
   *plan = PagedPlan();
   const int64_t rows = std::min(max_q, tokens) * group;
-  plan->tile_rows = rows <= 16 ? 16 : 32;
+  plan->tensor = rows > 32;
+  plan->tile_rows = plan->tensor ? kTileM / group * group : rows <= 16 ? 16 : 32;
+  const int64_t slots = plan->tensor ? 2 * sms : sms;
   const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
   const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
-  plan->grid = static_cast<int>(std::min<int64_t>(sms, std::min<int64_t>(row_tiles * c->Hkv, sms) * tiles));
+  plan->grid = static_cast<int>(std::min<int64_t>(slots, std::min<int64_t>(row_tiles * c->Hkv, slots) * tiles));
   plan->merge = tiles > 1;
   plan->header_bytes = round16(static_cast<int64_t>(plan->grid) * sizeof(PartHeader));
   plan->e_bytes = round16(static_cast<int64_t>(plan->grid) * 2 * plan->tile_rows * sizeof(float));
@@ -178,18 +181,44 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& 
 }
 
 template <typename T, int D>
+int launch_tile(const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& p, const PagedPlan& plan, CUtensorMapDataType dt, cudaStream_t stream) {
+  constexpr int kSmem = TileSmem<D>::kTotal;
+  static std::atomic<bool> configured[64];
+  int rc = configure_smem(sage_paged_tile_kernel<T, D>, kSmem, configured);
+  if (rc) return rc;
+  // Q as (D, heads, tokens), a box: 64 values, the heads of a group, as many tokens as fill a tile.  A dimension of extent 1
+  // may carry any stride in the caller's tensor; it gets the span of the others.
+  const cuuint64_t row = static_cast<cuuint64_t>(D) * 2;
+  cuuint64_t sh = static_cast<cuuint64_t>(p.q_stride_h) * 2, st = static_cast<cuuint64_t>(p.q_stride_t) * 2;
+  if (p.Hq == 1) sh = p.batch.T > 1 ? st * p.batch.T : row;
+  if (p.batch.T == 1) st = p.Hq > 1 ? sh * p.Hq : row;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(p.Hq), static_cast<cuuint64_t>(p.batch.T)};
+  const cuuint64_t strides[2] = {sh, st};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(plan.tile_rows / p.group)};
+  CUtensorMap tq;
+  rc = encode_map(&tq, dt, 3, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "q");
+  if (rc) return rc;
+  return launch(sage_paged_tile_kernel<T, D>, static_cast<unsigned>(plan.grid), kTileThreads, kSmem, stream, tq, tk, tv, p);
+}
+
+template <typename T, int D>
 int launch_pass(const sage_paged_kv_t* c, AttnParams p, const PagedPlan& plan, char* workspace, cudaStream_t stream) {
   p.tile_rows = plan.tile_rows;
   p.headers = reinterpret_cast<PartHeader*>(workspace);
   p.part_e = reinterpret_cast<float*>(workspace + plan.header_bytes);
   p.part_o = reinterpret_cast<float*>(workspace + plan.header_bytes + plan.e_bytes);
   const CUtensorMapDataType dt = c->dtype == SAGE_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int box_rows = std::min(c->page_size, kUnitKeys);
+  const int box_rows = std::min(c->page_size, plan.tensor ? kTileKeys : kUnitKeys);
   CUtensorMap tk, tv;
   int rc = encode_strided_16bit(&tk, dt, c->k, D, c->page_size, c->Hkv, c->num_pages, c->k_stride_slot, c->k_stride_head, c->k_stride_page, box_rows, "k_pages");
   if (rc) return rc;
   rc = encode_strided_16bit(&tv, dt, c->v, D, c->page_size, c->Hkv, c->num_pages, c->v_stride_slot, c->v_stride_head, c->v_stride_page, box_rows, "v_pages");
   if (rc) return rc;
+  if (plan.tensor) {
+    rc = launch_tile<T, D>(tk, tv, p, plan, dt, stream);
+    if (rc || !plan.merge) return rc;
+    return launch(sage_paged_merge_kernel<T, D, 8>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>((plan.tile_rows + 7) / 8)), kMergeThreads, 0, stream, p);
+  }
   rc = plan.tile_rows == 16 ? launch_rows<T, D, 1>(tk, tv, p, plan, stream) : launch_rows<T, D, 2>(tk, tv, p, plan, stream);
   if (rc || !plan.merge) return rc;
   return launch(sage_paged_merge_kernel<T, D, 2>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>(plan.tile_rows / 2)), kMergeThreads, 0, stream, p);
@@ -233,6 +262,7 @@ int sage_paged_attn(const sage_paged_kv_t* cache, const sage_paged_batch_t* batc
   SAGE_REQUIRE(q != nullptr && o != nullptr, "paged attention: null argument");
   if (batch->T == 0 || batch->B == 0) return SAGE_OK;
   SAGE_REQUIRE(rows_ok(q) && rows_ok(o), "paged attention: rows need a 16-byte aligned base and strides that are multiples of 8 elements");
+  SAGE_REQUIRE((batch->T <= 1 || q->stride_t > 0) && (Hq == 1 || q->stride_h > 0), "paged attention: the strides of q must be positive");
   SAGE_REQUIRE(n_shared == 0 || shared_pages != nullptr, "paged attention: null shared_pages");
   CallPlan plan;
   rc = plan_call(&plan, cache, batch, Hq, max_q, n_shared);

@@ -18,6 +18,12 @@ constexpr int kStatusBadLength = SAGE_STATUS_BAD_LENGTH;
 constexpr int kStatusMisaligned = 1;                  // as attn_kernel.cuh
 constexpr int kStatusWait = 2 + 16 * 20;              // ... and its numbering of waits: 20, a load of keys and values
 
+// A bounded wait by a whole warp: its lanes go on or give up together.
+template <bool kHinted>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, long long limit_cycles) {
+  return __all_sync(0xffffffffu, mbar_wait<kHinted>(bar, parity, abort_flag, limit_cycles));
+}
+
 struct Status {
   int* word;                    // optional device word, stays 0 on success
   int* host;                    // optional word in mapped pinned host memory that receives the same code

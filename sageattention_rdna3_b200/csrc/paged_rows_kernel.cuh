@@ -237,7 +237,7 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       const int keys = min(kUnitKeys, g.seq.len - first);
       if (keys <= 0) continue;
       const int stage = used % kStages;
-      if (ok && !mbar_wait<false>(bars + stage, (used / kStages) & 1, abort_flag, p.wait_limit_cycles)) {
+      if (ok && !warp_wait<false>(bars + stage, (used / kStages) & 1, abort_flag, p.wait_limit_cycles)) {
         ok = false;
         if (lane == 0) p.status.report(kStatusWait);
       }

@@ -256,32 +256,59 @@ __device__ __forceinline__ void join_weights(float e, float prior, float* w, flo
   *joined = top + log2f(sum);
 }
 
-// Writes N neighbouring values of a finished row: normalised `x`, log-sum-exp e (base 2).
+template <int N>
+__device__ __forceinline__ void store_floats(float* dst, const float (&x)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) reinterpret_cast<float4*>(dst)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  } else {
+    *reinterpret_cast<float2*>(dst) = make_float2(x[0], x[1]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_floats(const float* src, float (&x)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(src)[i];
+      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    }
+  } else {
+    const float2 v = *reinterpret_cast<const float2*>(src);
+    x[0] = v.x; x[1] = v.y;
+  }
+}
+
+// Writes N (2, 4 or a multiple of 8) neighbouring values of a finished row: normalised `x`, log-sum-exp e (base 2).
 template <typename T, int N>
 __device__ __forceinline__ void write_row(const AttnParams& p, int token, int head, int D, int col, float (&x)[N], float e, bool with_lse) {
   const long long row = static_cast<long long>(token) * p.Hq + head;
   if (p.o == nullptr) {
-    float* dst = p.o32 + row * D + col;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(x[i], x[i + 1]);
+    store_floats(p.o32 + row * D + col, x);
     if (with_lse) p.e32[row] = e;
     return;
   }
   if (p.prior_o != nullptr) {
     float w, wp, joined;
     join_weights(e, p.prior_e[row], &w, &wp, &joined);
-    const float* src = p.prior_o + row * D + col;
+    float y[N];
+    load_floats(p.prior_o + row * D + col, y);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 y = *reinterpret_cast<const float2*>(src + i);
-      x[i] = w * x[i] + wp * y.x;
-      x[i + 1] = w * x[i + 1] + wp * y.y;
-    }
+    for (int i = 0; i < N; ++i) x[i] = w * x[i] + wp * y[i];
     e = joined;
   }
   T* dst = static_cast<T*>(p.o) + token * p.o_stride_t + head * p.o_stride_h + col;
+  uint32_t packed[N / 2];
 #pragma unroll
-  for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = from_float2(x[i], x[i + 1], static_cast<const T*>(nullptr));
+  for (int i = 0; i < N / 2; ++i) packed[i] = from_float2(x[2 * i], x[2 * i + 1], static_cast<const T*>(nullptr));
+  if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = packed[0];
+  }
   if (with_lse && p.lse != nullptr) p.lse[row] = e * 0.6931471805599453f;      // (-inf stays -inf)
 }
 
@@ -338,13 +365,7 @@ __global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_kernel(const A
           const long long at = ((static_cast<long long>(blockIdx.x) + k) * 2 + (k == 0 ? 1 : 0)) * p.tile_rows + r;
           pe[c] = p.part_e[at];
           const float* src = p.part_o + at * D + lane * kPer;
-          if constexpr (kPer == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src);
-            px[c][0] = v.x; px[c][1] = v.y; px[c][2] = v.z; px[c][3] = v.w;
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(src);
-            px[c][0] = v.x; px[c][1] = v.y;
-          }
+          load_floats(src, px[c]);
         }
       }
       float top = e;

@@ -1,0 +1,440 @@
+// Attention of many rows over a paged cache: chunks of prompts, and a whole batch against the prefix that it shares.
+//
+// The mathematics is that of paged_rows_kernel.cuh; with 128 rows per key tile the products are the work (4 D flops per
+// row and key against 4 D bytes per key), so they go to the tensor cores through tcgen05.  A CTA owns a tile of 128 rows, the
+// query heads of a GQA group for 128 / group new tokens (one TMA box), and streams 128-key tiles:
+//   warp 4    TMA producer  Q; K and V tiles page by page (a box per page, or per 128 keys of a larger page)
+//   warp 5    MMA issuer    S = Q.K^T in halves of 64 keys, O += P.V, fp32 accumulators in TMEM
+//   warps 0-3 softmax       thread t owns row t: running maximum and sum in fp32, P back into TMEM over S
+// Two CTAs fit on an SM (112 KB of shared memory and 256 TMEM columns each), so that the tensor cores of one work under the
+// exponentials of the other.  The grid is 2 * SMs persistent CTAs over equal spans of key tiles (paged_schedule.cuh); loads and the first
+// Q.K^T of the next item run under the end of this one.  TMEM columns: [0,128) S, in place P (16-bit pairs); [128,128+D) O.
+//
+// Masks: a row sees the keys below its limit.  Behind the last key of a sequence pages hold anything; the softmax warps
+// write zeros over those rows of V before the product reads them (0 * NaN is NaN), and pages behind it are not
+// loaded at all.  Weights are 2^(s - m + 7): an optimistic pass takes them against the maximum so far, which moves only when
+// 64 of them add up to more than 2^15, and for fp16 the smallest numbers (2^-24) are 2^-31 of the largest weight.
+// P is rounded to the type of V; the sum is taken before that.
+#pragma once
+
+#include "paged_rows_kernel.cuh"
+
+namespace sage {
+namespace paged {
+
+constexpr int kTileThreads = 192;
+constexpr int kTileM = 128;
+constexpr int kHalfKeys = 64;
+constexpr int kTileTmemCols = 256;
+constexpr int kColO = 128;
+constexpr float kTileBias = 7.0f;                     // log2 of the largest weight while the maximum stands still
+constexpr float kTileLazy = 8.0f;                     // growth of the maximum that is let pass: weights up to 2^15
+constexpr float kTileSumMax = 32768.0f;
+constexpr float kTileRefusedLazy = 2.0f;              // 64 weights add up to more than 2^15: one is above 2^9
+
+template <int D>
+struct TileSmem {
+  static constexpr int kStages = D == 128 ? 1 : 2;
+  static constexpr int kQBytes = kTileM * D * 2;
+  static constexpr int kKVBytes = kTileKeys * D * 2;
+  static constexpr int kSlab = 128 * 128;             // 128 rows x 64 values, 128-byte swizzle
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = kQBytes;
+  static constexpr int kOffV = kOffK + kStages * kKVBytes;
+  static constexpr int kOffBar = kOffV + kStages * kKVBytes;
+  static constexpr int kNumBars = 10 + 4 * kStages;
+  static constexpr int kOffScratch = kOffBar + 8 * kNumBars;
+  static constexpr int kOffMisc = kOffScratch + 8 * (kTileThreads / 32 + 4);
+  static constexpr int kTotal = kOffMisc + 16;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTileThreads, 2)
+sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
+  using L = TileSmem<D>;
+  constexpr int kStages = L::kStages, kSlabs = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* s_q = smem + L::kOffQ;
+  uint8_t* s_k = smem + L::kOffK;
+  uint8_t* s_v = smem + L::kOffV;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* q_empty = bars + 1;     // every Q.K^T of the item is complete
+  uint64_t* o_final = bars + 2;     // every P.V of the item is complete
+  uint64_t* o_free = bars + 3;      // all 128 softmax threads hold the item's O in registers
+  uint64_t* s_full = bars + 4;      // [2] S_h holds Q.K_h^T
+  uint64_t* p_full = bars + 6;      // [2] P_h is written (and O scaled) by all 128 softmax threads
+  uint64_t* pv_done = bars + 8;     // [2] O += P_h.V_h is complete
+  uint64_t* k_full = bars + 10;
+  uint64_t* v_full = bars + 10 + kStages;
+  uint64_t* k_empty = bars + 10 + 2 * kStages;
+  uint64_t* v_empty = bars + 10 + 3 * kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
+  int* fail_code = reinterpret_cast<int*>(smem + L::kOffMisc + 8);
+  const bool misaligned = (smem_u32(smem) & 1023u) != 0u;
+
+  if (warp == 4 && elect_one()) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(o_final, 1);
+    mbar_init(o_free, 128);
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(s_full + h, 1);
+      mbar_init(p_full + h, 128);
+      mbar_init(pv_done + h, 1);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(k_full + s, 1);
+      mbar_init(v_full + s, 1);
+      mbar_init(k_empty + s, 1);
+      mbar_init(v_empty + s, 1);
+    }
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  grid_dependency_wait();
+  if (warp == 5) {                                    // (after the wait: attn_kernel.cuh)
+    tmem_alloc(tmem_slot, kTileTmemCols);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    const int before = p.status.word != nullptr ? *reinterpret_cast<volatile int*>(p.status.word) : 0;
+    *abort_flag = misaligned || (before & 15) == 2;
+    *fail_code = 0;
+    if (misaligned) p.status.report(kStatusMisaligned);
+    p.headers[blockIdx.x].n_parts = 0;
+  }
+  tc_fence_before();
+  const Span span = find_span<kTileThreads>(p, reinterpret_cast<long long*>(smem + L::kOffScratch));
+  tc_fence_after();
+  grid_launch_dependents();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool dead_on_arrival = *abort_flag != 0;
+
+// SAGE_PAGED_WAIT_OR: by one thread.  SAGE_PAGED_WARP_WAIT_OR: by a whole warp, whose lanes go on or give up together.
+#define SAGE_PAGED_WAIT_OR(hinted, bar_ptr, parity, bar_id, action)                 \
+  if (!mbar_wait<hinted>((bar_ptr), (parity), abort_flag, p.wait_limit_cycles)) {   \
+    atomicCAS(fail_code, 0, 2 + 16 * (bar_id));                                     \
+    action;                                                                         \
+  }
+#define SAGE_PAGED_WARP_WAIT_OR(hinted, bar_ptr, parity, bar_id, action)            \
+  if (!warp_wait<hinted>((bar_ptr), (parity), abort_flag, p.wait_limit_cycles)) {   \
+    atomicCAS(fail_code, 0, 2 + 16 * (bar_id));                                     \
+    action;                                                                         \
+  }
+
+  if (dead_on_arrival) {
+    // nothing to do
+  } else if (warp == 4) {
+    // ------------------------------------------------------------------ TMA producer
+    const bool leader = elect_one();
+    const int box_rows = min(1 << p.batch.page_log2, kTileKeys);
+    const int slot_mask = (1 << p.batch.page_log2) - 1;
+    SegmentIter it(p, span);
+    Segment g;
+    int kt = 0, items = 0;
+    bool ok = true;
+    // lane i holds the page of box i of a tile
+    int first = 0, boxes = 0, pages = 0;
+    auto find_pages = [&](int tile) {
+      first = g.seq.key0 + tile * kTileKeys;
+      const int keys = min(max(g.seq.len - first, 0), kTileKeys);
+      boxes = (keys + box_rows - 1) / box_rows;
+      pages = lane < boxes ? page_of_key(p, g.b, first + lane * box_rows) : 0;
+    };
+    auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int head) {
+      if (leader) mbar_arrive_expect_tx(bar, boxes * box_rows * D * 2);
+      for (int i = 0; i < boxes; ++i) {
+        const int id = __shfl_sync(0xffffffffu, pages, i);
+        if (leader) {
+#pragma unroll
+          for (int c = 0; c < kSlabs; ++c) tma_load_4d(dst + c * L::kSlab + i * box_rows * 128, map, bar, c * 64, first & slot_mask, head, id);
+        }
+      }
+    };
+    bool more = it.next(&g);
+    if (more) find_pages(g.tile);
+#pragma unroll 1
+    while (ok && more) {
+      if (items > 0) SAGE_PAGED_WARP_WAIT_OR(true, q_empty, (items - 1) & 1, 22, { ok = false; break; });
+      if (leader) {
+        mbar_arrive_expect_tx(q_full, p.tile_rows * D * 2);
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c)
+          tma_load_3d(s_q + c * L::kSlab, &tm_q, q_full, c * 64, g.head * p.group, g.seq.q0 + g.row_tile * (p.tile_rows / p.group));
+      }
+      __syncwarp();
+      const int n_tiles = g.n_tiles, tile0 = g.tile, head = g.head;
+#pragma unroll 1
+      for (int j = 0; j < n_tiles; ++j, ++kt) {
+        const int s = kt % kStages;
+        SAGE_PAGED_WARP_WAIT_OR(true, k_empty + s, ((kt / kStages) & 1) ^ 1u, 23, { ok = false; break; });
+        pages = checked_page(p, pages);
+        load(&tm_k, s_k + s * L::kKVBytes, k_full + s, head);
+        SAGE_PAGED_WARP_WAIT_OR(true, v_empty + s, ((kt / kStages) & 1) ^ 1u, 21, { ok = false; break; });
+        load(&tm_v, s_v + s * L::kKVBytes, v_full + s, head);
+        // the pages of the next tile arrive while its stage is waited for
+        if (j + 1 < n_tiles) {
+          find_pages(tile0 + j + 1);
+        } else {
+          more = it.next(&g);
+          if (more) find_pages(g.tile);
+        }
+      }
+      ++items;
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------ MMA issuer
+    // Order of the tensor cores: QK(0,0) QK(0,1) | PV(0,0) QK(1,0) PV(0,1) QK(1,1) | ...
+    if (elect_one()) {
+      constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+      constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kHalfKeys);
+      constexpr uint32_t kIdescPV = umma_idesc(1, kFmt, kFmt, 0, 1, kTileM, D);              // V MN-major
+      const uint32_t t_o = tmem_base + kColO;
+      SegmentIter it(p, span);
+      Segment g;
+      int kt = 0, items = 0;
+      bool ok = true;
+      auto issue_qk = [&](int stage, int h) {
+        // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes, half h of K starts
+        // 64 rows into each slab
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t slab = (k / 4) * L::kSlab;
+          const uint64_t dq = umma_smem_desc(smem_u32(s_q + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+          const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab + h * (kHalfKeys * 128)), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+          mma_f16_ss(tmem_base + h * kHalfKeys, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
+        }
+        tc_commit(s_full + h);
+      };
+#pragma unroll 1
+      while (ok && it.next(&g)) {
+        const int n_tiles = g.n_tiles;
+        SAGE_PAGED_WAIT_OR(false, q_full, items & 1, 24, { ok = false; break; });
+        SAGE_PAGED_WAIT_OR(false, k_full + kt % kStages, (kt / kStages) & 1, 25, { ok = false; break; });
+        tc_fence_after();
+        issue_qk(kt % kStages, 0);
+        issue_qk(kt % kStages, 1);
+        tc_commit(k_empty + kt % kStages);
+        if (n_tiles == 1) tc_commit(q_empty);
+#pragma unroll 1
+        for (int j = 0; ok && j < n_tiles; ++j) {
+          const int t = kt + j, s = t % kStages, s1 = (t + 1) % kStages;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            SAGE_PAGED_WAIT_OR(false, p_full + h, t & 1, 26, { ok = false; break; });
+            if (h == 0) SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
+            // the first P.V of an item overwrites O: the O of the item before must have been read
+            if (h == 0 && j == 0 && items > 0) SAGE_PAGED_WAIT_OR(false, o_free, (items - 1) & 1, 28, { ok = false; break; });
+            tc_fence_after();
+            // V: [128 keys][64 values] slabs; half h starts 64 rows = 8192 bytes in, an instruction takes 16 rows = 2048 bytes
+            const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes + h * (kHalfKeys * 128)), L::kSlab, 1024, kSwizzle128B);
+#pragma unroll
+            for (int k = 0; k < kHalfKeys / 16; ++k) {
+              mma_f16_ts(t_o, tmem_base + h * kHalfKeys + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || h > 0 || k > 0) ? 1u : 0u);
+            }
+            tc_commit(pv_done + h);
+            if (h == 1) tc_commit(v_empty + s);
+            if (j + 1 < n_tiles) {
+              if (h == 0) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
+              tc_fence_after();
+              issue_qk(s1, h);
+              if (h == 1) {
+                tc_commit(k_empty + s1);
+                if (j + 2 == n_tiles) tc_commit(q_empty);
+              }
+            }
+          }
+        }
+        tc_commit(o_final);
+        kt += n_tiles;
+        ++items;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax and output
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t t_o = tmem_base + lane_base + kColO;
+    SegmentIter it(p, span);
+    Segment g;
+    int kt = 0, items = 0;
+    bool ok = true;
+#pragma unroll 1
+    while (ok && it.next(&g)) {
+      const int head0 = g.head * p.group, row0 = g.row_tile * p.tile_rows;
+      int token = 0, head = 0, limit = 0;
+      bool live = row_at(g.seq.q0, g.seq.n_q, head0, p.group, row0, p.tile_rows, threadIdx.x, &token, &head);
+      if (live) {
+        if (p.shared_pass) {
+          int q1;
+          const int b = seq_of_token(p, token, &q1);
+          live = b < p.batch.B;
+          if (live) limit = min(g.seq.len, visible_keys(p, b, q1, token));
+        } else {
+          limit = visible_keys(p, g.b, g.seq.q0 + g.seq.n_q, token);
+        }
+      }
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      float m = -INFINITY, l = 0.0f;
+      int distrust = 0;                               // > 1: the optimistic pass is skipped
+#pragma unroll 1
+      for (int hh = 0; hh < 2 * g.n_tiles; ++hh) {
+        const int t = kt + (hh >> 1), h = hh & 1;
+        const int first = g.seq.key0 + g.tile * kTileKeys + hh * kHalfKeys;
+        SAGE_PAGED_WARP_WAIT_OR(false, s_full + h, t & 1, 31, { ok = false; break; });
+        tc_fence_after();
+        if (h == 0 && first + kTileKeys > g.seq.len) {
+          // The last tile: zeros over what is no value of the sequence.  (Behind the wait for S, which says that the stage's
+          // load before this one has long been used: a parity cannot tell phases apart that are two turns away.)
+          const int stage = t % kStages;
+          SAGE_PAGED_WARP_WAIT_OR(false, v_full + stage, (t / kStages) & 1, 30, { ok = false; break; });
+          const int keys = max(g.seq.len - first, 0);
+          for (int i = threadIdx.x; i < (kTileKeys - keys) * kSlabs * 8; i += 128) {
+            const int row = keys + i / (kSlabs * 8), x = i % (kSlabs * 8);
+            *reinterpret_cast<uint4*>(s_v + stage * L::kKVBytes + (x >> 3) * L::kSlab + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();                   // the tensor cores read it through the async proxy
+        }
+        if (warp_live) {
+          uint32_t sr[2][32];
+          tmem_ld32(tmem_base + lane_base + h * kHalfKeys, sr[0]);
+          tmem_ld32(tmem_base + lane_base + h * kHalfKeys + 32, sr[1]);
+          tc_wait_ld();
+          const int col_end = live ? limit - first : kHalfKeys;      // columns below it are visible
+          const bool masked = __any_sync(0xffffffffu, col_end < kHalfKeys);
+          uint32_t pk[32];
+          const f32x2_t scale2 = pack2(p.score_scale, p.score_scale);
+          auto exp_pass = [&](auto masked_tag, float base) -> float {
+            constexpr bool kMasked = decltype(masked_tag)::value;
+            const f32x2_t neg = pack2(kTileBias - base, kTileBias - base);
+            f32x2_t acc = pack2(0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 x = unpack2(ffma2(pack2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, neg));
+                float2 w = make_float2(ex2(x.x), ex2(x.y));
+                if constexpr (kMasked) {
+                  if (32 * c + 2 * i >= col_end) w.x = 0.0f;
+                  if (32 * c + 2 * i + 1 >= col_end) w.y = 0.0f;
+                }
+                acc = fadd2(acc, pack2(w.x, w.y));
+                pk[16 * c + i] = from_float2(w.x, w.y, static_cast<const T*>(nullptr));
+              }
+            }
+            const float2 a = unpack2(acc);
+            return a.x + a.y;
+          };
+          bool done = false;
+          const bool attempt = hh > 0 && !masked && distrust < 2 && !__any_sync(0xffffffffu, m == -INFINITY);
+          if (attempt) {
+            const float sum = exp_pass(std::false_type{}, m);
+            done = !__any_sync(0xffffffffu, !(sum <= kTileSumMax));
+            if (done) l += sum;
+            distrust = done ? max(distrust - 1, 0) : min(distrust + 2, 4);
+          }
+          if (!done) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float x = __uint_as_float(sr[c][i]) * p.score_scale;
+                if (32 * c + i < col_end) top = fmaxf(top, x);
+              }
+            const bool need = top > m + (attempt ? kTileRefusedLazy : kTileLazy) || (m == -INFINITY && top > m);
+            const bool moved = __any_sync(0xffffffffu, need);
+            if (!attempt && hh > 0) distrust = moved ? min(distrust + 1, 4) : max(distrust - 1, 0);
+            if (moved) {
+              if (hh > 0) {
+                const int hp = h ^ 1;
+                SAGE_PAGED_WARP_WAIT_OR(false, pv_done + hp, (h ? t : t - 1) & 1, 32, { ok = false; break; });
+                tc_fence_after();
+                const float back = need ? ex2(m - top) : 1.0f;
+                l *= back;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                  uint32_t orr[32];
+                  tmem_ld32(t_o + 32 * c, orr);
+                  tc_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * back);
+                  tmem_st32(t_o + 32 * c, orr);
+                }
+              }
+              if (need) m = top;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;            // (a row that has seen nothing yet)
+            if (masked) l += exp_pass(std::true_type{}, base);
+            else l += exp_pass(std::false_type{}, base);
+          }
+          tmem_st32(tmem_base + lane_base + h * kHalfKeys, pk);
+          tc_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(p_full + h);
+      }
+      if (!ok) break;
+      SAGE_PAGED_WARP_WAIT_OR(false, o_final, items & 1, 33, { ok = false; break; });
+      tc_fence_after();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      if (g.slot == 1 && threadIdx.x == 0) {
+        p.headers[blockIdx.x] = PartHeader{g.n_parts, g.seq.q0, g.seq.n_q, head0, row0, p.tile_rows, {0, 0}};
+      }
+      const long long at = (static_cast<long long>(blockIdx.x) * 2 + g.slot) * p.tile_rows + threadIdx.x;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t orr[32];
+        if (warp_live) {
+          tmem_ld32(t_o + 32 * c, orr);
+          tc_wait_ld();
+        }
+        if (c == D / 32 - 1) {                        // O is in registers: the next item may overwrite it
+          tc_fence_before();
+          mbar_arrive(o_free);
+        }
+        if (!live) continue;
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(orr[i]) * inv;
+        if (g.slot >= 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) reinterpret_cast<float4*>(p.part_o + at * D + 32 * c)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          if (c == 0) p.part_e[at] = part_lse(m - kTileBias, l);
+        } else {
+          write_row<T, 32>(p, token, head, D, 32 * c, x, l == 0.0f ? -INFINITY : m - kTileBias + log2f(l), c == 0);
+        }
+      }
+      kt += g.n_tiles;
+      ++items;
+    }
+    if (ok) zero_rest<T>(p, D, threadIdx.x, 128);
+  }
+#undef SAGE_PAGED_WAIT_OR
+#undef SAGE_PAGED_WARP_WAIT_OR
+
+  // ---------------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && !dead_on_arrival) {
+    // A wait gave up: copies and products that are still in flight land before shared memory and TMEM are handed back.
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    if (threadIdx.x == 0) p.status.report(*fail_code ? *fail_code : kStatusWait);
+    __syncthreads();
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTileTmemCols);
+  }
+}
+
+}  // namespace paged
+}  // namespace sage

@@ -63,8 +63,10 @@ def test_single_tokens(case):
     batch = PagedBatch([1] * len(kv_lens), kv_lens, Hq, Hkv, D, page, layout, dtype, torch.device("cuda"), seed=len(kv_lens) + Hq)
     o, lse = run(batch)
     compare(batch, o, lse)
-    o2, lse2 = run(batch, cu_q=batch.cu_q())
+    o2, lse2 = run(batch, cu_q=batch.cu_q(), max_q=1)              # the same batch said in another way
     assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    o2, lse2 = run(batch, cu_q=batch.cu_q())                       # ... and so that it may take the other kernel
+    compare(batch, o2, lse2)
     assert torch.equal(run(batch, lse=False), o)                   # and the same again
 
 
