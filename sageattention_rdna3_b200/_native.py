@@ -18,6 +18,7 @@ OPS_PATH = PKG_DIR / "_C.so"
 
 _ops = None
 _abi = None
+_module = None
 _import_error: Optional[BaseException] = None
 
 SAGE_DTYPE_F16 = 0
@@ -126,10 +127,14 @@ def load_ops():
 
 
 def load_module():
-    """The extension as a Python module: the short way into ``sageattn_fwd`` (``csrc/torch_ops.cpp``)."""
-    load_ops()
-    from . import _C
-    return _C
+    """The extension as a Python module: the short ways into the operators (``csrc/torch_ops.cpp``,
+    ``csrc/torch_paged_ops.cpp``)."""
+    global _module
+    if _module is None:
+        load_ops()
+        from . import _C
+        _module = _C
+    return _module
 
 
 def native_available() -> bool:

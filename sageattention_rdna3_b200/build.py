@@ -99,8 +99,8 @@ def build_ops(force: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    units = [(CSRC / "torch_ops.cpp", [CSRC / "internal.h", REPO_DIR / "include" / "sage_b200.h"]),
-             (CSRC / "torch_paged_ops.cpp", [REPO_DIR / "include" / "sage_b200.h", REPO_DIR / "include" / "sage_paged_b200.h"])]
+    units = [(CSRC / "torch_ops.cpp", [CSRC / "internal.h", CSRC / "torch_paged.h", REPO_DIR / "include" / "sage_b200.h"]),
+             (CSRC / "torch_paged_ops.cpp", [CSRC / "torch_paged.h", REPO_DIR / "include" / "sage_b200.h", REPO_DIR / "include" / "sage_paged_b200.h"])]
     sources = sorted({f for unit, headers in units for f in (unit, *headers)})
     extra = torch.__version__
     if force or not _up_to_date(LIB_OPS, sources, extra):

@@ -126,6 +126,7 @@ Batch batch_of(const sage_paged_batch_t* b, const sage_paged_kv_t* c) {
 struct PagedPlan {
   bool tensor = false;          // sage_paged_tile_kernel
   int tile_rows = 0;
+  int item_cost = 0;
   int grid = 0;
   bool merge = false;           // an item may be cut
   int64_t header_bytes = 0, e_bytes = 0, o_bytes = 0;
@@ -142,6 +143,10 @@ int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t t
   const int64_t rows = std::min(max_q, tokens) * group;
   plan->tensor = rows > 32;
   plan->tile_rows = plan->tensor ? kTileM / group * group : rows <= 16 ? 16 : 32;
+  // What the start and end of an item cost, in key tiles.  us of the attention kernel with 0 / 1 / 2 / 3: 64 sequences of 60 to
+  // 16000 keys, a token each, 157 / 148 / 150 / 152; 32 of 500 to 6000, 3 to 5 tokens (32 rows) 94 / 88 / 81 / 78; chunks of
+  // prompts (128 rows) 244 / 235 / 223 / 222; 128 sequences of 1 to 1000 keys, a token each, 47 / 40 / 40 / 43.
+  plan->item_cost = plan->tensor ? 2 : plan->tile_rows == 16 ? 1 : 3;
   const int64_t slots = plan->tensor ? 2 * sms : sms;
   const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
   const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
@@ -204,11 +209,12 @@ int launch_tile(const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& 
 template <typename T, int D>
 int launch_pass(const sage_paged_kv_t* c, AttnParams p, const PagedPlan& plan, char* workspace, cudaStream_t stream) {
   p.tile_rows = plan.tile_rows;
+  p.item_cost = plan.item_cost;
   p.headers = reinterpret_cast<PartHeader*>(workspace);
   p.part_e = reinterpret_cast<float*>(workspace + plan.header_bytes);
   p.part_o = reinterpret_cast<float*>(workspace + plan.header_bytes + plan.e_bytes);
   const CUtensorMapDataType dt = c->dtype == SAGE_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const int box_rows = std::min(c->page_size, plan.tensor ? kTileKeys : kUnitKeys);
+  const int box_rows = std::min(c->page_size, kTileKeys);
   CUtensorMap tk, tv;
   int rc = encode_strided_16bit(&tk, dt, c->k, D, c->page_size, c->Hkv, c->num_pages, c->k_stride_slot, c->k_stride_head, c->k_stride_page, box_rows, "k_pages");
   if (rc) return rc;

@@ -3,10 +3,10 @@
 // o_r = sum_j 2^(s_rj - m) v_j / sum_j 2^(s_rj - m), s = q.k sm_scale log2 e, one pass over the keys with the running
 // maximum m.  With a handful of rows per key the cache is read once and everything else is small: the bound is HBM
 // (D=128: 512 bytes per key and kv head against 4 D flops per row).  So the split follows the loads: a CTA per SM takes an
-// equal span of key tiles (paged_schedule.cuh); of every 128-key tile each of its four warps takes 32 keys, with a ring
-// of TMA loads of its own (kStages x 16 KB at D=128, 192 KB in flight per SM) and its own running maximum and sum.  Warps meet
-// only at the end of an item, so none waits for another in between, and the loads of the next item are under way
-// while this one is finished.
+// equal span of 128-key tiles (paged_schedule.cuh).  A producer warp walks through it and keeps a ring of TMA loads full (192 KB in
+// flight per SM), across items, with the rows of Q of the next item: what it has to look up - lengths, pages -
+// it asks for ahead of its use.  Of every tile each of four warps takes 32 keys with a running maximum and sum of
+// its own; they meet only at the end of an item.
 //
 // The products are mma.sync (m16n8k16, fp32 accumulators): the 16 rows of one instruction hold the query heads of a GQA group
 // (and the drafted tokens).  tcgen05 has no shape below 64 rows, and its accumulator would go through TMEM to the
@@ -23,23 +23,30 @@
 namespace sage {
 namespace paged {
 
-constexpr int kRowsThreads = 128;
-constexpr int kUnitKeys = 32;                         // keys of one warp's load
+constexpr int kRowsThreads = 160;
+constexpr int kRowsWarps = 4;                         // that compute
+constexpr int kUnitKeys = 32;                         // keys of a tile that one of them takes
 
 template <int D, int MT>
 struct RowsSmem {
   static constexpr int kRows = 16 * MT;
   static constexpr int kStages = D == 128 ? 3 : 6;
-  static constexpr int kSlab = kUnitKeys * 128;       // 32 keys x 64 values, 128-byte swizzle
-  static constexpr int kUnit = 2 * (D / 64) * kSlab;  // K and V
-  static constexpr int kMergeCols = 64 / MT;          // columns joined at a time
-  static constexpr int kMergeStride = kMergeCols + 8;
-  static constexpr int kOffMerge = 4 * kStages * kUnit;
-  static constexpr int kOffStats = kOffMerge + 4 * kRows * kMergeStride * 4;     // m, l of every warp and row
-  static constexpr int kOffBar = kOffStats + 2 * 4 * kRows * 4;
-  static constexpr int kOffScratch = kOffBar + 4 * kStages * 8;
+  static constexpr int kSlab = kTileKeys * 128;       // 128 keys x 64 values, 128-byte swizzle
+  static constexpr int kStage = 2 * (D / 64) * kSlab; // K and V of a tile
+  static constexpr int kItems = 2;                    // items ahead: segment and rows of Q
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kJoinRows = 8;                 // rows that the warps join at a time
+  static constexpr int kJoinStride = D + 8;
+  static constexpr int kOffQ = kStages * kStage;
+  static constexpr int kOffJoin = kOffQ + kItems * kQBytes;
+  static constexpr int kOffStats = kOffJoin + kRowsWarps * kJoinRows * kJoinStride * 4;     // m, l of every warp and row
+  static constexpr int kOffSegments = kOffStats + 2 * kRowsWarps * kRows * 4;
+  static constexpr int kOffBar = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
+  static constexpr int kNumBars = 2 * kStages + 2 * kItems + 1;
+  static constexpr int kOffScratch = kOffBar + kNumBars * 8;
   static constexpr int kOffMisc = kOffScratch + (kRowsThreads / 32 + 4) * 8;
   static constexpr int kTotal = kOffMisc + 16;
+  static_assert(kTotal <= 232448, "shared memory of an SM");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -76,49 +83,44 @@ __device__ __forceinline__ int checked_page(const AttnParams& p, int page) {
   return 0;
 }
 
-// The units (32 keys) of one warp in the order in which they are used, across segments.
-struct UnitIter {
-  SegmentIter it;
-  Segment g;
-  int tile, left;
-  __device__ __forceinline__ UnitIter(const AttnParams& p, const Span& s) : it(p, s), left(0) {}
-  // The next unit that has keys: first key and their number (at most 32); false at the end of the span.
-  __device__ __forceinline__ bool next(int warp, int* first, int* keys) {
-    while (true) {
-      if (left == 0) {
-        if (!it.next(&g)) return false;
-        tile = g.tile;
-        left = g.n_tiles;
-      }
-      *first = g.seq.key0 + tile * kTileKeys + warp * kUnitKeys;
-      *keys = min(kUnitKeys, g.seq.len - *first);
-      ++tile;
-      --left;
-      if (*keys > 0) return true;
-    }
-  }
-};
+// 16 bytes from global to shared memory, zeros if !ok; counted on an mbarrier by cp_async_arrive.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
   using L = RowsSmem<D, MT>;
-  constexpr int kRows = L::kRows, kStages = L::kStages, kSlabs = D / 64;
+  constexpr int kRows = L::kRows, kStages = L::kStages, kItems = L::kItems, kSlabs = D / 64;
   constexpr float kBias = std::is_same<T, __half>::value ? 15.0f : 0.0f;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * kStages;
-  uint8_t* ring = smem + warp * kStages * L::kUnit;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* empty = full + kStages;
+  uint64_t* item_full = empty + kStages;
+  uint64_t* item_empty = item_full + kItems;
+  uint64_t* joined = item_empty + kItems;
+  Segment* segments = reinterpret_cast<Segment*>(smem + L::kOffSegments);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc);
   const bool misaligned = (smem_u32(smem) & 1023u) != 0u;    // (the swizzled slabs need it)
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(bars + s, 1);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, kRowsWarps);
+    }
+    for (int s = 0; s < kItems; ++s) {
+      mbar_init(item_full + s, 33);                   // every lane's part of Q, and the segment
+      mbar_init(item_empty + s, kRowsWarps);
+    }
+    mbar_init(joined, kRowsWarps);
     fence_mbar_init();
     fence_proxy_async_smem();
-    if (warp == 0) {
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
-    }
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
   }
   grid_dependency_wait();
   if (threadIdx.x == 0) {
@@ -132,93 +134,142 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   grid_launch_dependents();
   if (*abort_flag) return;
 
-  // ---- loads
-  const int box_rows = min(1 << p.batch.page_log2, kUnitKeys);
-  UnitIter producer(p, span);
-  int issued = 0;
-  int next_first = 0, next_keys = 0, next_pages[2] = {0, 0}, next_head = 0;
-  bool more = true;
-  // Finds the next unit and asks for its pages, which are looked at when it is issued, a unit later.
-  auto fetch = [&]() {
-    more = producer.next(warp, &next_first, &next_keys);
-    if (more) {
-      next_head = producer.g.head;
-      next_pages[0] = page_of_key(p, producer.g.b, next_first);
-      next_pages[1] = 0;
-      if (box_rows < kUnitKeys && next_keys > box_rows) next_pages[1] = page_of_key(p, producer.g.b, next_first + box_rows);
-    }
-  };
-  auto issue = [&]() {
-    if (lane == 0) {
-      uint64_t* bar = bars + issued % kStages;
-      uint8_t* dst = ring + (issued % kStages) * L::kUnit;
-      const int boxes = box_rows < kUnitKeys && next_keys > box_rows ? 2 : 1;
-      const int slot = next_first & ((1 << p.batch.page_log2) - 1);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) next_pages[x] = checked_page(p, next_pages[x]);
-      mbar_arrive_expect_tx(bar, boxes * box_rows * D * 2 * 2);
-      for (int x = 0; x < boxes; ++x) {
-#pragma unroll
-        for (int c = 0; c < kSlabs; ++c) tma_load_4d(dst + c * L::kSlab + x * box_rows * 128, &tm_k, bar, c * 64, slot, next_head, next_pages[x]);
-      }
-      for (int x = 0; x < boxes; ++x) {
-#pragma unroll
-        for (int c = 0; c < kSlabs; ++c) tma_load_4d(dst + (kSlabs + c) * L::kSlab + x * box_rows * 128, &tm_v, bar, c * 64, slot, next_head, next_pages[x]);
-      }
-    }
-    ++issued;
-  };
-  fetch();
+  if (warp == kRowsWarps) {
+    // ------------------------------------------------------------------ producer
+    const bool leader = elect_one();
+    const int box_rows = min(1 << p.batch.page_log2, kTileKeys);
+    const int slot_mask = (1 << p.batch.page_log2) - 1;
+    SegmentIter it(p, span);
+    bool ok = true;
+    int tiles = 0;                                    // so far
+    int first = 0, boxes = 0, pages = 0;              // of the next tile: first key, boxes; lane i holds the page of box i
+    auto find_pages = [&](const Segment& g, int j) {
+      first = g.key0 + j * kTileKeys;
+      const int keys = min(max(g.len - first, 0), kTileKeys);
+      boxes = (keys + box_rows - 1) / box_rows;
+      pages = lane < boxes ? page_of_key(p, g.b, first + lane * box_rows) : 0;
+    };
+    Segment g = it.next();
+    if (g.n_tiles > 0) find_pages(g, 0);
 #pragma unroll 1
-  for (int s = 0; s < kStages && more; ++s) {
-    issue();
-    fetch();
+    for (int item = 0; ok; ++item) {
+      const int slot = item % kItems;
+      ok = warp_wait<true>(item_empty + slot, ((item / kItems) & 1) ^ 1u, abort_flag, p.wait_limit_cycles);
+      if (!ok) break;
+      if (g.n_tiles > 0) {
+        const uint32_t s_q = smem_u32(smem + L::kOffQ + slot * L::kQBytes);
+        constexpr int kChunks = D / 8;
+#pragma unroll
+        for (int i = 0; i < kRows * kChunks / 32; ++i) {
+          const int r = (i * 32 + lane) / kChunks, c = lane % kChunks;
+          int token = 0, head = 0;
+          const bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, kRows, r, &token, &head);
+          const T* src = static_cast<const T*>(p.q) + (live ? token * p.q_stride_t + head * p.q_stride_h + c * 8 : 0);
+          cp_async16(s_q + r * (D * 2) + ((c & ~7) << 4) + (((c ^ r) & 7) << 4), src, live);
+        }
+      }
+      if (lane == 0) segments[slot] = g;
+      cp_async_arrive(item_full + slot);
+      if (lane == 0) mbar_arrive(item_full + slot);
+      if (g.n_tiles == 0) break;
+      const Segment now = g;
+#pragma unroll 1
+      for (int j = 0; j < now.n_tiles; ++j, ++tiles) {
+        const int stage = tiles % kStages;
+        ok = warp_wait<true>(empty + stage, ((tiles / kStages) & 1) ^ 1u, abort_flag, p.wait_limit_cycles);
+        if (!ok) break;
+        uint8_t* dst = smem + stage * L::kStage;
+        const int checked = checked_page(p, pages);
+        if (leader) mbar_arrive_expect_tx(full + stage, boxes * box_rows * D * 2 * 2);
+        for (int x = 0; x < boxes; ++x) {
+          const int page = __shfl_sync(0xffffffffu, checked, x);
+          if (leader) {
+#pragma unroll
+            for (int c = 0; c < kSlabs; ++c) {
+              tma_load_4d(dst + c * L::kSlab + x * box_rows * 128, &tm_k, full + stage, c * 64, first & slot_mask, now.kv_head, page);
+              tma_load_4d(dst + (kSlabs + c) * L::kSlab + x * box_rows * 128, &tm_v, full + stage, c * 64, first & slot_mask, now.kv_head, page);
+            }
+          }
+        }
+        // the pages of the next tile arrive while its stage is waited for
+        if (j + 1 < now.n_tiles) {
+          find_pages(now, j + 1);
+        } else {
+          g = it.next();
+          if (g.n_tiles > 0) find_pages(g, 0);
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) p.status.report(kStatusWait);
+      // A launch that gave up waits (for a bounded time again) for its own copies in flight.
+      volatile int* again = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
+      *again = 0;
+      for (int n = max(tiles - kStages, 0); n < tiles; ++n) warp_wait<true>(full + n % kStages, (n / kStages) & 1, again, p.wait_limit_cycles);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
   }
 
-  // ---- work
-  float* s_merge = reinterpret_cast<float*>(smem + L::kOffMerge);
+  // -------------------------------------------------------------------- work
+  float* s_join = reinterpret_cast<float*>(smem + L::kOffJoin);
   float* s_m = reinterpret_cast<float*>(smem + L::kOffStats);
-  float* s_l = s_m + 4 * kRows;
-  int used = 0;
+  float* s_l = s_m + kRowsWarps * kRows;
   bool ok = true;
-  SegmentIter it(p, span);
-  Segment g;
+  int tiles = 0;
+  // A barrier of the four warps whose wait is bounded: one of them may have given up.
+  uint32_t joins = 0;
+  auto warps_sync = [&]() -> bool {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(joined);
+    ok = ok && warp_wait<false>(joined, joins++ & 1, abort_flag, p.wait_limit_cycles);
+    return ok;
+  };
 #pragma unroll 1
-  while (it.next(&g)) {
-    const int row0 = g.row_tile * kRows, head0 = g.head * p.group;
+  for (int item = 0;; ++item) {
+    const int q_slot = item % kItems;
+    ok = ok && warp_wait<false>(item_full + q_slot, (item / kItems) & 1, abort_flag, p.wait_limit_cycles);
+    if (!ok) break;
+    const Segment g = segments[q_slot];
+    if (g.n_tiles == 0) break;
+    const uint32_t s_q = smem_u32(smem + L::kOffQ + q_slot * L::kQBytes);
+    const int live_rows = min(kRows, g.n_q * p.group - g.row0);
     // this thread's rows of the accumulators: lane / 4 and 8 below, of every 16
-    uint32_t qf[MT][D / 16][4];
     int limit[MT][2];
-    int least = g.seq.len;
+    int least = g.len;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        int token, head;
-        bool live = row_at(g.seq.q0, g.seq.n_q, head0, p.group, row0, kRows, mt * 16 + half * 8 + lane / 4, &token, &head);
-        int lim = 0;
+        int token, head, lim = 0;
+        bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, kRows, mt * 16 + half * 8 + lane / 4, &token, &head);
         if (live) {
           if (p.shared_pass) {
             int q1;
             const int b = seq_of_token(p, token, &q1);
             live = b < p.batch.B;
-            if (live) lim = min(g.seq.len, visible_keys(p, b, q1, token));
+            if (live) lim = min(g.len, visible_keys(p, b, q1, token));
           } else {
-            lim = visible_keys(p, g.b, g.seq.q0 + g.seq.n_q, token);
+            lim = p.causal ? max(0, g.len - (g.q0 + g.n_q - 1 - token)) : g.len;
           }
         }
         limit[mt][half] = lim;
         if (live) least = min(least, lim);
-        const T* src = live ? static_cast<const T*>(p.q) + token * p.q_stride_t + head * p.q_stride_h + (lane % 4) * 2 : nullptr;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          qf[mt][k][half] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
-          qf[mt][k][2 + half] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
-        }
       }
-    }
+    least = __reduce_min_sync(0xffffffffu, least);
+
+    // (rows 0-7 and 8-15, values 0-7 and 8-15 of every 16: the A operand).  With 32 rows there are no registers to keep it in.
+    auto load_q = [&](int mt, int k, uint32_t (&a)[4]) {
+      const int r = mt * 16 + (lane & 15), c = 2 * k + (lane >> 4);
+      ldmatrix_x4(s_q + r * (D * 2) + ((c & ~7) << 4) + (((c ^ r) & 7) << 4), a);
+    };
+    uint32_t qf[MT == 1 ? D / 16 : 1][4];
+    if constexpr (MT == 1) {
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
+      for (int k = 0; k < D / 16; ++k) load_q(0, k, qf[k]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty + q_slot);
+    }
 
     float o[MT][D / 8][4], m[MT][2], l[MT][2];
 #pragma unroll
@@ -232,130 +283,136 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     }
 
 #pragma unroll 1
-    for (int tile = g.tile; tile < g.tile + g.n_tiles; ++tile) {
-      const int first = g.seq.key0 + tile * kTileKeys + warp * kUnitKeys;
-      const int keys = min(kUnitKeys, g.seq.len - first);
-      if (keys <= 0) continue;
-      const int stage = used % kStages;
-      if (ok && !warp_wait<false>(bars + stage, (used / kStages) & 1, abort_flag, p.wait_limit_cycles)) {
-        ok = false;
-        if (lane == 0) p.status.report(kStatusWait);
-      }
-      if (!ok) continue;
-      ++used;
-      const uint32_t s_k = smem_u32(ring + stage * L::kUnit), s_v = s_k + kSlabs * L::kSlab;
+    for (int j = 0; j < g.n_tiles; ++j, ++tiles) {
+      const int stage = tiles % kStages;
+      ok = ok && warp_wait<false>(full + stage, (tiles / kStages) & 1, abort_flag, p.wait_limit_cycles);
+      if (!ok) break;
+      const int first = g.key0 + j * kTileKeys + warp * kUnitKeys;
+      const int keys = min(kUnitKeys, g.len - first);
+      if (keys > 0) {
+        const uint32_t s_k = smem_u32(smem + stage * L::kStage) + warp * (kUnitKeys * 128), s_v = s_k + kSlabs * L::kSlab;
 
-      // S = Q.K^T: 4 groups of 8 keys
-      float s[MT][4][4];
+        // S = Q.K^T: 4 groups of 8 keys
+        float s[MT][4][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[mt][n][i] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-#pragma unroll
-        for (int n2 = 0; n2 < 2; ++n2) {
-          // matrices: (keys 0-7, values 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15) of a 16 x 16 block
-          const int key = n2 * 16 + (lane >> 4) * 8 + (lane & 7);
-          const int chunk = (k % 4) * 2 + ((lane >> 3) & 1);
-          uint32_t b[4];
-          ldmatrix_x4(s_k + (k / 4) * L::kSlab + key * 128 + ((chunk ^ (key & 7)) << 4), b);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma_16816(s[mt][2 * n2], qf[mt][k], b[0], b[1], static_cast<const T*>(nullptr));
-            mma_16816(s[mt][2 * n2 + 1], qf[mt][k], b[2], b[3], static_cast<const T*>(nullptr));
-          }
-        }
-      }
-
-      uint32_t pf[MT][2][4];                          // P as the A operand, 16 keys each
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[mt][n][i] *= p.score_scale;
-        if (first + kUnitKeys > least) {              // (some row does not see all keys)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int key = first + n * 8 + (lane % 4) * 2 + (i & 1);
-              if (key >= limit[mt][i >> 1]) s[mt][n][i] = -INFINITY;
-            }
-        }
-        float top[2] = {m[mt][0], m[mt][1]};
+            for (int i = 0; i < 4; ++i) s[mt][n][i] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], s[mt][n][i]);
-        float neg[2], back[2];
-        bool moved = false;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-          top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-          moved |= top[half] > m[mt][half];
-          const float base = top[half] == -INFINITY ? 0.0f : top[half];      // (a row that has seen nothing yet)
-          back[half] = ex2(m[mt][half] - base);
-          neg[half] = kBias - base;
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            l[mt][half] *= back[half];
-            m[mt][half] = top[half];
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              o[mt][n][2 * half] *= back[half];
-              o[mt][n][2 * half + 1] *= back[half];
-            }
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[mt][n][i] = ex2(s[mt][n][i] + neg[i >> 1]);
-            l[mt][i >> 1] += s[mt][n][i];
-          }
-          pf[mt][n / 2][(n & 1) * 2] = from_float2(s[mt][n][0], s[mt][n][1], static_cast<const T*>(nullptr));
-          pf[mt][n / 2][(n & 1) * 2 + 1] = from_float2(s[mt][n][2], s[mt][n][3], static_cast<const T*>(nullptr));
-        }
-      }
-
-      // O += P.V.  Behind the last key a page holds whatever it held: those values of V are taken as zero (0 * NaN is NaN).
-      const bool partial = keys < kUnitKeys;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t mask0 = 0xffffffffu, mask1 = 0xffffffffu;
-        if (partial) {
-          const int key = k * 16 + (lane % 4) * 2;
-          mask0 = (key < keys ? 0xffffu : 0u) | (key + 1 < keys ? 0xffff0000u : 0u);
-          mask1 = (key + 8 < keys ? 0xffffu : 0u) | (key + 9 < keys ? 0xffff0000u : 0u);
-        }
-#pragma unroll
-        for (int n2 = 0; n2 < D / 16; ++n2) {
-          // matrices: (keys 0-7, values 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15) of a 16 x 16 block, transposed
-          const int key = k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-          const int chunk = (n2 % 4) * 2 + (lane >> 4);
-          uint32_t b[4];
-          ldmatrix_x4_trans(s_v + (n2 / 4) * L::kSlab + key * 128 + ((chunk ^ (key & 7)) << 4), b);
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t a[MT][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            mma_16816(o[mt][2 * n2], pf[mt][k], b[0] & mask0, b[1] & mask1, static_cast<const T*>(nullptr));
-            mma_16816(o[mt][2 * n2 + 1], pf[mt][k], b[2] & mask0, b[3] & mask1, static_cast<const T*>(nullptr));
+            if constexpr (MT == 1) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) a[mt][i] = qf[k][i];
+            } else {
+              load_q(mt, k, a[mt]);
+            }
+          }
+#pragma unroll
+          for (int n2 = 0; n2 < 2; ++n2) {
+            // matrices: (keys 0-7, values 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15) of a 16 x 16 block
+            const int key = n2 * 16 + (lane >> 4) * 8 + (lane & 7);
+            const int chunk = (k % 4) * 2 + ((lane >> 3) & 1);
+            uint32_t b[4];
+            ldmatrix_x4(s_k + (k / 4) * L::kSlab + key * 128 + ((chunk ^ (key & 7)) << 4), b);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma_16816(s[mt][2 * n2], a[mt], b[0], b[1], static_cast<const T*>(nullptr));
+              mma_16816(s[mt][2 * n2 + 1], a[mt], b[2], b[3], static_cast<const T*>(nullptr));
+            }
           }
         }
+
+        uint32_t pf[MT][2][4];                        // P as the A operand, 16 keys each
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[mt][n][i] *= p.score_scale;
+          if (first + kUnitKeys > least) {            // (some row does not see all keys)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int key = first + n * 8 + (lane % 4) * 2 + (i & 1);
+                if (key >= limit[mt][i >> 1]) s[mt][n][i] = -INFINITY;
+              }
+          }
+          float top[2] = {m[mt][0], m[mt][1]};
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], s[mt][n][i]);
+          float neg[2], back[2];
+          bool moved = false;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
+            moved |= top[half] > m[mt][half];
+            const float base = top[half] == -INFINITY ? 0.0f : top[half];    // (a row that has seen nothing yet)
+            back[half] = ex2(m[mt][half] - base);
+            neg[half] = kBias - base;
+          }
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              l[mt][half] *= back[half];
+              m[mt][half] = top[half];
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) {
+                o[mt][n][2 * half] *= back[half];
+                o[mt][n][2 * half + 1] *= back[half];
+              }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[mt][n][i] = ex2(s[mt][n][i] + neg[i >> 1]);
+              l[mt][i >> 1] += s[mt][n][i];
+            }
+            pf[mt][n / 2][(n & 1) * 2] = from_float2(s[mt][n][0], s[mt][n][1], static_cast<const T*>(nullptr));
+            pf[mt][n / 2][(n & 1) * 2 + 1] = from_float2(s[mt][n][2], s[mt][n][3], static_cast<const T*>(nullptr));
+          }
+        }
+
+        // O += P.V.  Behind the last key a page holds whatever it held: those values of V are taken as zero (0 * NaN is NaN).
+        const bool partial = keys < kUnitKeys;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t mask0 = 0xffffffffu, mask1 = 0xffffffffu;
+          if (partial) {
+            const int key = k * 16 + (lane % 4) * 2;
+            mask0 = (key < keys ? 0xffffu : 0u) | (key + 1 < keys ? 0xffff0000u : 0u);
+            mask1 = (key + 8 < keys ? 0xffffu : 0u) | (key + 9 < keys ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int n2 = 0; n2 < D / 16; ++n2) {
+            // matrices: (keys 0-7, values 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15) of a 16 x 16 block, transposed
+            const int key = k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+            const int chunk = (n2 % 4) * 2 + (lane >> 4);
+            uint32_t b[4];
+            ldmatrix_x4_trans(s_v + (n2 / 4) * L::kSlab + key * 128 + ((chunk ^ (key & 7)) << 4), b);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma_16816(o[mt][2 * n2], pf[mt][k], b[0] & mask0, b[1] & mask1, static_cast<const T*>(nullptr));
+              mma_16816(o[mt][2 * n2 + 1], pf[mt][k], b[2] & mask0, b[3] & mask1, static_cast<const T*>(nullptr));
+            }
+          }
+        }
+        __syncwarp();                                 // all lanes have read the stage
       }
-      __syncwarp();                                   // all lanes have read the stage
-      if (more) {
-        issue();
-        fetch();
-      }
+      if (lane == 0) mbar_arrive(empty + stage);
     }
+    if (!ok) break;
+    if (MT > 1 && lane == 0) mbar_arrive(item_empty + q_slot);
 
     // ---- the four warps' parts become one
 #pragma unroll
@@ -369,74 +426,57 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           s_l[warp * kRows + mt * 16 + half * 8 + lane / 4] = l[mt][half];
         }
       }
-    __syncthreads();
     if (g.slot == 1 && threadIdx.x == 0) {
-      p.headers[blockIdx.x] = PartHeader{g.n_parts, g.seq.q0, g.seq.n_q, head0, row0, kRows, {0, 0}};
+      p.headers[blockIdx.x] = PartHeader{g.n_parts, g.q0, g.n_q, g.head0, g.row0, kRows, {0, 0}};
     }
-    const bool dead = *abort_flag != 0;               // (uniform: set before the barrier, or by a later wait that ends all the same)
-    float mine[MT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int pass = 0; pass < 2 * MT; ++pass) {       // rows 8 * pass to 8 * pass + 7
+      if (pass * 8 >= live_rows) break;
+      if (pass > 0 && !warps_sync()) break;           // the buffer has been read
+      float* dst = s_join + (warp * 8 + lane / 4) * L::kJoinStride + (lane % 4) * 2;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = mt * 16 + half * 8 + lane / 4;
-        const float top = fmaxf(fmaxf(s_m[r], s_m[kRows + r]), fmaxf(s_m[2 * kRows + r], s_m[3 * kRows + r]));
-        mine[mt][half] = top == -INFINITY ? 1.0f : ex2(m[mt][half] - top);
+      for (int n = 0; n < D / 8; ++n) {
+        const float* x = &o[pass / 2][n][2 * (pass % 2)];
+        *reinterpret_cast<float2*>(dst + n * 8) = make_float2(x[0], x[1]);
       }
+      if (!warps_sync()) break;
 #pragma unroll
-    for (int pass = 0; pass < D / L::kMergeCols; ++pass) {
+      for (int i = threadIdx.x; i < 8 * D / 4; i += 128) {
+        const int r8 = i / (D / 4), r = pass * 8 + r8, col = (i - r8 * (D / 4)) * 4;
+        if (r >= live_rows) break;
+        float top = -INFINITY;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+        for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, s_m[w * kRows + r]);
+        float out[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < L::kMergeCols / 8; ++n)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float* x = &o[mt][pass * (L::kMergeCols / 8) + n][2 * half];
-            float* dst = s_merge + (warp * kRows + mt * 16 + half * 8 + lane / 4) * L::kMergeStride + n * 8 + (lane % 4) * 2;
-            *reinterpret_cast<float2*>(dst) = make_float2(x[0] * mine[mt][half], x[1] * mine[mt][half]);
-          }
-      __syncthreads();
-      constexpr int kGroups = kRows * L::kMergeCols / 4;
-#pragma unroll
-      for (int i = threadIdx.x; i < kGroups; i += kRowsThreads) {
-        const int r = i / (L::kMergeCols / 4), c = (i - r * (L::kMergeCols / 4)) * 4;
-        int token, head;
-        bool live = !dead && row_at(g.seq.q0, g.seq.n_q, head0, p.group, row0, kRows, r, &token, &head);
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, s_m[w * kRows + r]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(s_merge + (w * kRows + r) * L::kMergeStride + c);
-          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-          sum += s_l[w * kRows + r] * (top == -INFINITY ? 1.0f : ex2(s_m[w * kRows + r] - top));
+        for (int w = 0; w < kRowsWarps; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(s_join + (w * 8 + r8) * L::kJoinStride + col);
+          const float f = top == -INFINITY ? 1.0f : ex2(s_m[w * kRows + r] - top);
+          out[0] += f * y.x; out[1] += f * y.y; out[2] += f * y.z; out[3] += f * y.w;
+          sum += f * s_l[w * kRows + r];
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        float out[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-        const int col = pass * L::kMergeCols + c;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) out[c] *= inv;
         if (g.slot >= 0) {
           const long long at = (static_cast<long long>(blockIdx.x) * 2 + g.slot) * kRows + r;
-          *reinterpret_cast<float4*>(p.part_o + at * D + col) = make_float4(out[0], out[1], out[2], out[3]);
+          store_floats(p.part_o + at * D + col, out);
           if (col == 0) p.part_e[at] = part_lse(top - kBias, sum);
-        } else if (live) {
-          if (p.shared_pass) {
+        } else {
+          int token, head;
+          bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, kRows, r, &token, &head);
+          if (live && p.shared_pass) {
             int q1;
             live = seq_of_token(p, token, &q1) < p.batch.B;
           }
           if (live) write_row<T, 4>(p, token, head, D, col, out, sum == 0.0f ? -INFINITY : top - kBias + log2f(sum), col == 0);
         }
       }
-      __syncthreads();
     }
+    if (!warps_sync()) break;                         // statistics and buffer are free again
   }
-  zero_rest<T>(p, D, threadIdx.x, kRowsThreads);
-  // a launch that gave up waits (for a bounded time again) for its own copies in flight
-  if (!ok) {
-    volatile int* again = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
-    *again = 0;
-    for (int u = used; u < issued; ++u) mbar_wait<false>(bars + u % kStages, (u / kStages) & 1, again, p.wait_limit_cycles);
-  }
+  if (ok) zero_rest<T>(p, D, threadIdx.x, 128);
+  else if (lane == 0) p.status.report(kStatusWait);
 }
 
 }  // namespace paged

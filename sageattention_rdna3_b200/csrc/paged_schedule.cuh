@@ -1,9 +1,9 @@
 // How attention over a paged cache is cut into work for a fixed grid, without the host knowing a length.
 //
 // An item is one row tile of one kv head of one sequence: up to `tile_rows` rows (new token, query head of the group) that
-// read the same keys.  Its steps are tiles of 128 keys, at least one (an item without keys writes zeros).  The steps of all items,
-// sequence after sequence, kv head after kv head, row tile after row tile, form one line that is cut into equal spans, one per CTA:
-// lengths may differ as they like and all CTAs get the same number of tiles.  A span that covers part of an item leaves
+// read the same keys.  Its steps are tiles of 128 keys, at least one (an item without keys writes zeros), behind `item_cost` more that
+// stand for its start and end.  The steps of all items, after sequence, kv head after kv head, row tile after row tile, form one line that is cut into equal spans, one per CTA:
+// lengths may differ as they like and all CTAs get the same amount of work.  A span that covers part of an item leaves
 // its result in a slot of the workspace (slot 1 the head of an item, slot 0 anything else: at most one of each per
 // CTA) and a header that tells sage_paged_merge_kernel which parts follow.  Every CTA works this out for itself from kv_lens and
 // cu_q, by a block-wide prefix sum; nothing is communicated and the order of all sums is fixed.
@@ -33,6 +33,7 @@ struct AttnParams {
   int shared_pass;              // 1: one sequence of all T tokens against the shared keys; 0: every sequence against its keys behind them
   int Hq, Hkv, group;           // group = Hq / Hkv
   int tile_rows;                // rows of a row tile
+  int item_cost;                // steps that stand for the start and end of an item
   int causal;
   int zero_rest;                // write zeros to rows that belong to no sequence
   float score_scale;            // sm_scale * log2(e)
@@ -85,7 +86,7 @@ __device__ __forceinline__ Seq seq_at(const AttnParams& p, int b) {
 }
 
 __device__ __forceinline__ long long steps_of(const AttnParams& p, const Seq& s) {
-  return static_cast<long long>(s.row_tiles) * s.key_tiles * p.Hkv;
+  return static_cast<long long>(s.row_tiles) * (s.key_tiles + p.item_cost) * p.Hkv;
 }
 
 // Keys that a new token sees: [0, limit).
@@ -171,57 +172,84 @@ __device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratc
   return s;
 }
 
-// A part of a span that belongs to one item.
+// A part of a span that belongs to one item, as the producer warp of a CTA tells it to the others.
 struct Segment {
-  Seq seq;
-  int b, head, row_tile;        // kv head
-  int tile, n_tiles;            // key tiles [tile, tile + n_tiles)
+  int q0, n_q, len;             // of the sequence
+  int key0;                     // first key of the segment's first tile
+  int n_tiles;                  // 0: no more segments
+  int head0, row0;              // first query head of the group, first row of the tile
   int slot;                     // -1: the whole item; 1: its head, 0: another part
   int n_parts;                  // slot 1: parts of the item
+  int b, kv_head;
+  int pad;
 };
 
-// Walks through a span.  Every thread that uses one gets the same segments.
+// Walks through a span; by a whole warp, whose lanes look ahead at 32 sequences at a time, so that an item costs no
+// round trip to memory.
 struct SegmentIter {
   const AttnParams& p;
   Span s;
-  Seq seq;
-  long long steps;              // of seq
-  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span) {
-    if (s.t < s.t_end) {
-      seq = seq_at(p, s.b);
-      steps = steps_of(p, seq);
+  int base;                     // lane i holds sequence base + i
+  Seq mine;
+  Seq seq;                      // of s.b
+  long long steps;
+  __device__ __forceinline__ void find(int b) {
+    const int lane = threadIdx.x & 31;
+    if (b >= base + 32) {
+      base = b;
+      if (b + lane < n_seqs(p)) mine = seq_at(p, b + lane);
     }
+    const int from = b - base;
+    seq.q0 = __shfl_sync(0xffffffffu, mine.q0, from);
+    seq.n_q = __shfl_sync(0xffffffffu, mine.n_q, from);
+    seq.key0 = p.shared_pass ? 0 : p.shared_len;
+    seq.len = __shfl_sync(0xffffffffu, mine.len, from);
+    seq.row_tiles = __shfl_sync(0xffffffffu, mine.row_tiles, from);
+    seq.key_tiles = __shfl_sync(0xffffffffu, mine.key_tiles, from);
+    steps = steps_of(p, seq);
   }
-  __device__ __forceinline__ bool next(Segment* g) {
-    if (s.t >= s.t_end) return false;
-    while (s.t >= s.before + steps) {                 // (sequences without new tokens have no steps)
-      s.before += steps;
-      seq = seq_at(p, ++s.b);
-      steps = steps_of(p, seq);
+  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span), base(-32) {
+    if (s.t < s.t_end) find(s.b);
+  }
+  __device__ __forceinline__ Segment next() {
+    Segment g;
+    g.n_tiles = 0;
+    while (s.t < s.t_end && g.n_tiles == 0) {
+      while (s.t >= s.before + steps) {               // (sequences without new tokens have no steps)
+        s.before += steps;
+        find(++s.b);
+      }
+      const int item_steps = seq.key_tiles + p.item_cost;
+      const long long r = s.t - s.before;
+      const int item = static_cast<int>(r / item_steps);
+      const int at = static_cast<int>(r - static_cast<long long>(item) * item_steps);
+      const int count = static_cast<int>(min(static_cast<long long>(item_steps - at), s.t_end - s.t));
+      const int tile = max(at - p.item_cost, 0);
+      g.n_tiles = at + count - p.item_cost - tile;    // 0: nothing but the set-up of the item, which the CTA with its first tile does
+      if (g.n_tiles < 0) g.n_tiles = 0;
+      g.q0 = seq.q0;
+      g.n_q = seq.n_q;
+      g.len = seq.len;
+      g.key0 = seq.key0 + tile * kTileKeys;
+      g.kv_head = item / seq.row_tiles;
+      g.head0 = g.kv_head * p.group;
+      g.row0 = (item - g.kv_head * seq.row_tiles) * p.tile_rows;
+      g.b = s.b;
+      g.n_parts = 1;
+      if (tile > 0) {
+        g.slot = 0;
+      } else if (g.n_tiles == seq.key_tiles) {
+        g.slot = -1;
+      } else {
+        g.slot = 1;
+        // the CTA that owns the last step e of the item: the largest c with total * c / ctas <= e
+        const long long e = s.t + item_steps - at - 1;
+        const long long c = ((e + 1) * s.ctas - 1) / s.total;
+        g.n_parts = static_cast<int>(c) - static_cast<int>(blockIdx.x) + 1;
+      }
+      s.t += count;
     }
-    const long long r = s.t - s.before;
-    const long long item = r / seq.key_tiles;
-    g->seq = seq;
-    g->b = s.b;
-    g->head = static_cast<int>(item / seq.row_tiles);
-    g->row_tile = static_cast<int>(item - static_cast<long long>(g->head) * seq.row_tiles);
-    g->tile = static_cast<int>(r - item * seq.key_tiles);
-    const long long left = s.t_end - s.t;
-    g->n_tiles = static_cast<int>(min(static_cast<long long>(seq.key_tiles - g->tile), left));
-    g->n_parts = 1;
-    if (g->tile > 0) {
-      g->slot = 0;
-    } else if (g->n_tiles == seq.key_tiles) {
-      g->slot = -1;
-    } else {
-      g->slot = 1;
-      // the CTA that owns the last step e of the item: the largest c with total * c / ctas <= e
-      const long long e = s.t + seq.key_tiles - 1;
-      const long long c = ((e + 1) * s.ctas - 1) / s.total;
-      g->n_parts = static_cast<int>(c) - static_cast<int>(blockIdx.x) + 1;
-    }
-    s.t += g->n_tiles;
-    return true;
+    return g;
   }
 };
 

@@ -42,8 +42,10 @@ struct TileSmem {
   static constexpr int kOffK = kQBytes;
   static constexpr int kOffV = kOffK + kStages * kKVBytes;
   static constexpr int kOffBar = kOffV + kStages * kKVBytes;
-  static constexpr int kNumBars = 10 + 4 * kStages;
-  static constexpr int kOffScratch = kOffBar + 8 * kNumBars;
+  static constexpr int kItems = 2;                    // items ahead
+  static constexpr int kNumBars = 10 + 4 * kStages + 2 * kItems;
+  static constexpr int kOffSegments = kOffBar + 8 * kNumBars;
+  static constexpr int kOffScratch = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
   static constexpr int kOffMisc = kOffScratch + 8 * (kTileThreads / 32 + 4);
   static constexpr int kTotal = kOffMisc + 16;
 };
@@ -71,6 +73,9 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   uint64_t* v_full = bars + 10 + kStages;
   uint64_t* k_empty = bars + 10 + 2 * kStages;
   uint64_t* v_empty = bars + 10 + 3 * kStages;
+  uint64_t* item_full = bars + 10 + 4 * kStages;               // [kItems] the segment is written
+  uint64_t* item_empty = bars + 10 + 4 * kStages + L::kItems;  // ... and read by the MMA warp and the four softmax warps
+  Segment* segments = reinterpret_cast<Segment*>(smem + L::kOffSegments);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
   int* fail_code = reinterpret_cast<int*>(smem + L::kOffMisc + 8);
@@ -91,6 +96,10 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       mbar_init(v_full + s, 1);
       mbar_init(k_empty + s, 1);
       mbar_init(v_empty + s, 1);
+    }
+    for (int s = 0; s < L::kItems; ++s) {
+      mbar_init(item_full + s, 1);
+      mbar_init(item_empty + s, 5);
     }
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -137,14 +146,12 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int box_rows = min(1 << p.batch.page_log2, kTileKeys);
     const int slot_mask = (1 << p.batch.page_log2) - 1;
     SegmentIter it(p, span);
-    Segment g;
-    int kt = 0, items = 0;
+    int kt = 0;
     bool ok = true;
-    // lane i holds the page of box i of a tile
-    int first = 0, boxes = 0, pages = 0;
-    auto find_pages = [&](int tile) {
-      first = g.seq.key0 + tile * kTileKeys;
-      const int keys = min(max(g.seq.len - first, 0), kTileKeys);
+    int first = 0, boxes = 0, pages = 0;              // of the next tile: first key, boxes; lane i holds the page of box i
+    auto find_pages = [&](const Segment& g, int j) {
+      first = g.key0 + j * kTileKeys;
+      const int keys = min(max(g.len - first, 0), kTileKeys);
       boxes = (keys + box_rows - 1) / box_rows;
       pages = lane < boxes ? page_of_key(p, g.b, first + lane * box_rows) : 0;
     };
@@ -158,36 +165,42 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
     };
-    bool more = it.next(&g);
-    if (more) find_pages(g.tile);
+    Segment g = it.next();
+    if (g.n_tiles > 0) find_pages(g, 0);
 #pragma unroll 1
-    while (ok && more) {
+    for (int items = 0; ok; ++items) {
+      const int slot = items % L::kItems;
+      SAGE_PAGED_WARP_WAIT_OR(true, item_empty + slot, ((items / L::kItems) & 1) ^ 1u, 20, { ok = false; break; });
+      if (lane == 0) {
+        segments[slot] = g;
+        mbar_arrive(item_full + slot);
+      }
+      __syncwarp();
+      if (g.n_tiles == 0) break;
       if (items > 0) SAGE_PAGED_WARP_WAIT_OR(true, q_empty, (items - 1) & 1, 22, { ok = false; break; });
       if (leader) {
         mbar_arrive_expect_tx(q_full, p.tile_rows * D * 2);
 #pragma unroll
-        for (int c = 0; c < kSlabs; ++c)
-          tma_load_3d(s_q + c * L::kSlab, &tm_q, q_full, c * 64, g.head * p.group, g.seq.q0 + g.row_tile * (p.tile_rows / p.group));
+        for (int c = 0; c < kSlabs; ++c) tma_load_3d(s_q + c * L::kSlab, &tm_q, q_full, c * 64, g.head0, g.q0 + g.row0 / p.group);
       }
       __syncwarp();
-      const int n_tiles = g.n_tiles, tile0 = g.tile, head = g.head;
+      const Segment now = g;
 #pragma unroll 1
-      for (int j = 0; j < n_tiles; ++j, ++kt) {
+      for (int j = 0; j < now.n_tiles; ++j, ++kt) {
         const int s = kt % kStages;
         SAGE_PAGED_WARP_WAIT_OR(true, k_empty + s, ((kt / kStages) & 1) ^ 1u, 23, { ok = false; break; });
         pages = checked_page(p, pages);
-        load(&tm_k, s_k + s * L::kKVBytes, k_full + s, head);
+        load(&tm_k, s_k + s * L::kKVBytes, k_full + s, now.kv_head);
         SAGE_PAGED_WARP_WAIT_OR(true, v_empty + s, ((kt / kStages) & 1) ^ 1u, 21, { ok = false; break; });
-        load(&tm_v, s_v + s * L::kKVBytes, v_full + s, head);
+        load(&tm_v, s_v + s * L::kKVBytes, v_full + s, now.kv_head);
         // the pages of the next tile arrive while its stage is waited for
-        if (j + 1 < n_tiles) {
-          find_pages(tile0 + j + 1);
+        if (j + 1 < now.n_tiles) {
+          find_pages(now, j + 1);
         } else {
-          more = it.next(&g);
-          if (more) find_pages(g.tile);
+          g = it.next();
+          if (g.n_tiles > 0) find_pages(g, 0);
         }
       }
-      ++items;
     }
     __syncwarp();
   } else if (warp == 5) {
@@ -198,9 +211,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kHalfKeys);
       constexpr uint32_t kIdescPV = umma_idesc(1, kFmt, kFmt, 0, 1, kTileM, D);              // V MN-major
       const uint32_t t_o = tmem_base + kColO;
-      SegmentIter it(p, span);
-      Segment g;
-      int kt = 0, items = 0;
+      int kt = 0;
       bool ok = true;
       auto issue_qk = [&](int stage, int h) {
         // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes, half h of K starts
@@ -215,8 +226,11 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         tc_commit(s_full + h);
       };
 #pragma unroll 1
-      while (ok && it.next(&g)) {
-        const int n_tiles = g.n_tiles;
+      for (int items = 0; ok; ++items) {
+        SAGE_PAGED_WAIT_OR(false, item_full + items % L::kItems, (items / L::kItems) & 1, 34, { ok = false; break; });
+        const int n_tiles = segments[items % L::kItems].n_tiles;
+        mbar_arrive(item_empty + items % L::kItems);
+        if (n_tiles == 0) break;
         SAGE_PAGED_WAIT_OR(false, q_full, items & 1, 24, { ok = false; break; });
         SAGE_PAGED_WAIT_OR(false, k_full + kt % kStages, (kt / kStages) & 1, 25, { ok = false; break; });
         tc_fence_after();
@@ -255,7 +269,6 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         tc_commit(o_final);
         kt += n_tiles;
-        ++items;
       }
     }
     __syncwarp();
@@ -263,23 +276,25 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     // ------------------------------------------------------------------ softmax and output
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t t_o = tmem_base + lane_base + kColO;
-    SegmentIter it(p, span);
-    Segment g;
-    int kt = 0, items = 0;
+    int kt = 0;
     bool ok = true;
 #pragma unroll 1
-    while (ok && it.next(&g)) {
-      const int head0 = g.head * p.group, row0 = g.row_tile * p.tile_rows;
+    for (int items = 0; ok; ++items) {
+      SAGE_PAGED_WARP_WAIT_OR(false, item_full + items % L::kItems, (items / L::kItems) & 1, 34, { ok = false; break; });
+      const Segment g = segments[items % L::kItems];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty + items % L::kItems);
+      if (g.n_tiles == 0) break;
       int token = 0, head = 0, limit = 0;
-      bool live = row_at(g.seq.q0, g.seq.n_q, head0, p.group, row0, p.tile_rows, threadIdx.x, &token, &head);
+      bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, p.tile_rows, threadIdx.x, &token, &head);
       if (live) {
         if (p.shared_pass) {
           int q1;
           const int b = seq_of_token(p, token, &q1);
           live = b < p.batch.B;
-          if (live) limit = min(g.seq.len, visible_keys(p, b, q1, token));
+          if (live) limit = min(g.len, visible_keys(p, b, q1, token));
         } else {
-          limit = visible_keys(p, g.b, g.seq.q0 + g.seq.n_q, token);
+          limit = p.causal ? max(0, g.len - (g.q0 + g.n_q - 1 - token)) : g.len;
         }
       }
       const bool warp_live = __any_sync(0xffffffffu, live);
@@ -288,15 +303,15 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll 1
       for (int hh = 0; hh < 2 * g.n_tiles; ++hh) {
         const int t = kt + (hh >> 1), h = hh & 1;
-        const int first = g.seq.key0 + g.tile * kTileKeys + hh * kHalfKeys;
+        const int first = g.key0 + hh * kHalfKeys;
         SAGE_PAGED_WARP_WAIT_OR(false, s_full + h, t & 1, 31, { ok = false; break; });
         tc_fence_after();
-        if (h == 0 && first + kTileKeys > g.seq.len) {
+        if (h == 0 && first + kTileKeys > g.len) {
           // The last tile: zeros over what is no value of the sequence.  (Behind the wait for S, which says that the stage's
           // load before this one has long been used: a parity cannot tell phases apart that are two turns away.)
           const int stage = t % kStages;
           SAGE_PAGED_WARP_WAIT_OR(false, v_full + stage, (t / kStages) & 1, 30, { ok = false; break; });
-          const int keys = max(g.seq.len - first, 0);
+          const int keys = max(g.len - first, 0);
           for (int i = threadIdx.x; i < (kTileKeys - keys) * kSlabs * 8; i += 128) {
             const int row = keys + i / (kSlabs * 8), x = i % (kSlabs * 8);
             *reinterpret_cast<uint4*>(s_v + stage * L::kKVBytes + (x >> 3) * L::kSlab + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -387,7 +402,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (g.slot == 1 && threadIdx.x == 0) {
-        p.headers[blockIdx.x] = PartHeader{g.n_parts, g.seq.q0, g.seq.n_q, head0, row0, p.tile_rows, {0, 0}};
+        p.headers[blockIdx.x] = PartHeader{g.n_parts, g.q0, g.n_q, g.head0, g.row0, p.tile_rows, {0, 0}};
       }
       const long long at = (static_cast<long long>(blockIdx.x) * 2 + g.slot) * p.tile_rows + threadIdx.x;
 #pragma unroll
@@ -414,7 +429,6 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
       kt += g.n_tiles;
-      ++items;
     }
     if (ok) zero_rest<T>(p, D, threadIdx.x, 128);
   }

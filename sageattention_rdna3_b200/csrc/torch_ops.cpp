@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "internal.h"
+#include "torch_paged.h"
 
 namespace {
 
@@ -681,12 +682,26 @@ PyObject* sageattn_plain(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+using FastCall = PyObject* (*)(PyObject*, PyObject* const*, Py_ssize_t);
+PyCFunction fastcall(FastCall f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)); }
+
 PyMethodDef sage_methods[] = {
     {"register_device", register_device, METH_VARARGS, nullptr},
     {"sageattn_plain", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sageattn_plain)), METH_FASTCALL, nullptr},
+    {"rotary_plain", fastcall(sage_rotary_plain), METH_FASTCALL, nullptr},
+    {"paged_append_plain", fastcall(sage_paged_append_plain), METH_FASTCALL, nullptr},
+    {"paged_attn_plain", fastcall(sage_paged_attn_plain), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
+
+bool sage_device_status(int index, int** status, const volatile int32_t** mirror) {
+  if (index < 0 || index >= kMaxDevices || g_devices[index] == nullptr) return false;
+  const DeviceState& d = *g_devices[index];
+  *status = d.status.data_ptr<int>();
+  *mirror = d.mirror.defined() ? static_cast<const volatile int32_t*>(d.mirror.data_ptr()) : nullptr;
+  return true;
+}
 
 static struct PyModuleDef sage_module_def = {PyModuleDef_HEAD_INIT, "_C", nullptr, -1, sage_methods};
 PyMODINIT_FUNC PyInit__C(void) { return PyModule_Create(&sage_module_def); }

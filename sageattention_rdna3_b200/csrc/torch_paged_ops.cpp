@@ -1,14 +1,24 @@
 // torch.ops.sageattention.* of the operators around a growing cache: a thin wrapper that turns tensors into the pointers,
 // sizes and strides of include/sage_paged_b200.h.
+#include <Python.h>
+#include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 #include <torch/types.h>
 
 #include <climits>
+#include <cmath>
+#include <cstdlib>
 #include <vector>
 
 #include "../../include/sage_paged_b200.h"
+#include "torch_paged.h"
 
 namespace {
 
@@ -258,4 +268,250 @@ TORCH_LIBRARY_IMPL(sageattention, CUDA, m) {
   m.impl("rotary", &rotary);
   m.impl("paged_append", &paged_append);
   m.impl("paged_attn", &paged_attn);
+}
+
+// ---------------------------------------------------------------- short ways
+// A call of a few microseconds on the GPU is bound by the host: of 19 us per call, the checks in Python and the conversion of
+// fifteen arguments by torch.ops took 13.  These functions make the same checks on the tensors themselves; whatever is not a plain
+// call - a check that fails, an argument of another type, a tensor that needs a gradient or a copy, a subclass, an active mode -
+// returns None and takes the way through Python, which raises the errors.
+namespace {
+
+// A strided CUDA tensor that is just that; *out is left alone for None where that is allowed.
+bool plain(PyObject* o, const at::Tensor** out, bool none = false) {
+  if (none && o == Py_None) return true;
+  if (!THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (at::isTensorSubclassLike(t) || t.layout() != at::kStrided || !t.is_cuda() || t.unsafeGetTensorImpl()->has_symbolic_sizes_strides() ||
+      t.is_neg() || t.is_conj()) {
+    return false;
+  }
+  *out = &t;
+  return true;
+}
+
+bool modes_active() { return at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+
+// Every call is to be looked at when it is done (core.py).
+bool checks_status() {
+  const char* e = std::getenv("SAGEATTN_B200_CHECK_STATUS");
+  return e != nullptr && *e != '\0';
+}
+
+bool vectors(const at::Tensor& t) {
+  const int64_t unit = 16 / t.element_size();
+  if (t.stride(-1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) {
+    if (t.stride(i) % unit != 0 || (t.size(i) > 1 && t.stride(i) == 0)) return false;
+  }
+  return true;
+}
+
+bool needs_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
+int64_t layout_of(PyObject* o) {
+  if (!PyUnicode_CheckExact(o)) return -1;
+  return PyUnicode_CompareWithASCIIString(o, "HND") == 0 ? 1 : PyUnicode_CompareWithASCIIString(o, "NHD") == 0 ? 0 : -1;
+}
+
+bool small_int(PyObject* o, int* out) {
+  if (!PyLong_CheckExact(o)) return false;
+  const long v = PyLong_AsLong(o);
+  if (v < 0 || v > INT_MAX) {
+    PyErr_Clear();
+    return false;
+  }
+  *out = static_cast<int>(v);
+  return true;
+}
+
+bool plain_int32(const at::Tensor& t, const at::Tensor& like, int64_t dim) {
+  return t.scalar_type() == at::kInt && t.device() == like.device() && t.dim() == dim && (t.size(-1) <= 1 || t.stride(-1) == 1) && t.numel() > 0;
+}
+
+bool plain_cache(const at::Tensor& k, const at::Tensor& v, int64_t layout) {
+  if (layout < 0 || k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || k.device() != v.device()) return false;
+  if (k.scalar_type() != at::kHalf && k.scalar_type() != at::kBFloat16) return false;
+  return vectors(k) && vectors(v) && k.numel() > 0;
+}
+
+bool plain_batch(const at::Tensor& table, const at::Tensor& lens, const at::Tensor* cu, const at::Tensor& rows, const at::Tensor& like) {
+  if (!plain_int32(table, like, 2) || !plain_int32(lens, like, 1) || table.size(0) != lens.size(0)) return false;
+  if (cu == nullptr) return rows.size(0) == lens.size(0);
+  return plain_int32(*cu, like, 1) && cu->size(0) == lens.size(0) + 1;
+}
+
+bool plain_rows(const at::Tensor& t, const at::Tensor& pages, int64_t heads) {
+  return t.dim() == 3 && t.numel() > 0 && t.size(2) == pages.size(3) && (heads < 0 || t.size(1) == heads) && t.scalar_type() == pages.scalar_type() &&
+         t.device() == pages.device() && vectors(t) && !needs_grad(t);
+}
+
+bool plain_table(const at::Tensor& freq, const at::Tensor& axis, int n_axes, const at::Tensor& like) {
+  return freq.device() == like.device() && axis.device() == like.device() && n_axes >= 1 && n_axes <= SAGE_MAX_ROTARY_AXES &&
+         freq.is_contiguous() && axis.is_contiguous() && freq.scalar_type() == at::kLong && axis.scalar_type() == at::kInt;
+}
+
+// positions [n] or [n, axes] (`batch` < 0), or with a batch dimension in front; false if they do not fit.
+bool plain_positions(sage_rotary_t* r, const at::Tensor& p, const at::Tensor& like, int64_t batch, int64_t n) {
+  if ((p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) || p.device() != like.device()) return false;
+  int64_t dim = p.dim();
+  const bool bare = r->n_axes == 1 && (dim == 1 ? p.size(0) == n : batch >= 0 && dim == 2 && p.size(0) == batch && p.size(1) == n);
+  if (!bare) {
+    if (dim < 2 || p.size(-1) != r->n_axes || (r->n_axes > 1 && p.stride(-1) != 1)) return false;
+    --dim;
+  }
+  if (p.size(dim - 1) != n || dim > (batch >= 0 ? 2 : 1) || (dim == 2 && p.size(0) != batch)) return false;
+  r->positions = p.data_ptr();
+  r->positions_64 = p.scalar_type() == at::kLong;
+  r->stride_s = p.stride(dim - 1);
+  r->stride_b = dim == 2 ? p.stride(0) : 0;
+  return true;
+}
+
+}  // namespace
+
+// rotary_plain(q, k or None, positions, freq, axis, n_axes, interleaved, head_dim, tensor_layout) -> (q, k) or q, or None
+PyObject* sage_rotary_plain(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q = nullptr, *k = nullptr, *positions = nullptr, *freq = nullptr, *axis = nullptr;
+  int n_axes = 0, head_dim = 0;
+  if (nargs != 9 || !plain(args[0], &q) || !plain(args[1], &k, true) || !plain(args[2], &positions) || !plain(args[3], &freq) ||
+      !plain(args[4], &axis) || !small_int(args[5], &n_axes) || !PyBool_Check(args[6]) || !small_int(args[7], &head_dim) || modes_active()) {
+    Py_RETURN_NONE;
+  }
+  const int64_t layout = layout_of(args[8]);
+  const at::ScalarType dt = q->scalar_type();
+  if (layout < 0 || (dt != at::kHalf && dt != at::kBFloat16 && dt != at::kFloat) || q->dim() != 4 || q->numel() == 0 || q->size(3) != head_dim ||
+      !vectors(*q) || needs_grad(*q) || !plain_table(*freq, *axis, n_axes, *q)) {
+    Py_RETURN_NONE;
+  }
+  const int h_dim = layout == 1 ? 1 : 2, s_dim = layout == 1 ? 2 : 1;
+  const int64_t B = q->size(0), S = q->size(s_dim);
+  if (k != nullptr && (k->dim() != 4 || k->numel() == 0 || k->scalar_type() != dt || k->device() != q->device() || k->size(0) != B ||
+                       k->size(s_dim) != S || k->size(3) != head_dim || !vectors(*k) || needs_grad(*k))) {
+    Py_RETURN_NONE;
+  }
+  sage_rotary_t r = rotary_of(*freq, *axis, n_axes, args[6] == Py_True, *q);
+  if (!plain_positions(&r, *positions, *q, B, S)) Py_RETURN_NONE;
+  at::Tensor qo, ko;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::CUDAGuard guard(q->device());
+    qo = at::empty(q->sizes(), q->options());
+    if (k != nullptr) ko = at::empty(k->sizes(), k->options());
+    const sage_strided_t qs = strided_of(*q, layout), qos = strided_of(qo, layout);
+    sage_strided_t ks{}, kos{};
+    if (k != nullptr) {
+      ks = strided_of(*k, layout);
+      kos = strided_of(ko, layout);
+    }
+    check_rc(sage_apply_rotary(&qs, &qos, k != nullptr ? &ks : nullptr, k != nullptr ? &kos : nullptr, &r, dtype_code(*q, true),
+                               size_of(B, "batch"), size_of(q->size(h_dim), "heads"), k != nullptr ? size_of(k->size(h_dim), "heads") : 0,
+                               size_of(S, "length"), head_dim, 0, current_stream(*q)),
+             "rotary");
+  }
+  if (k == nullptr) return THPVariable_Wrap(qo);
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(qo));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(ko));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append_plain(k_pages, v_pages, tensor_layout, k, v, page_table, kv_lens, cu_q or None, q or None, freq or None, axis or None, n_axes,
+//                    interleaved, positions or None) -> q, or True without one, or None
+PyObject* sage_paged_append_plain(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *kp = nullptr, *vp = nullptr, *k = nullptr, *v = nullptr, *table = nullptr, *lens = nullptr, *cu = nullptr, *q = nullptr,
+                   *freq = nullptr, *axis = nullptr, *positions = nullptr;
+  int n_axes = 0;
+  if (nargs != 14 || !plain(args[0], &kp) || !plain(args[1], &vp) || !plain(args[3], &k) || !plain(args[4], &v) || !plain(args[5], &table) ||
+      !plain(args[6], &lens) || !plain(args[7], &cu, true) || !plain(args[8], &q, true) || !plain(args[9], &freq, true) ||
+      !plain(args[10], &axis, true) || !small_int(args[11], &n_axes) || !PyBool_Check(args[12]) || !plain(args[13], &positions, true) || modes_active() || checks_status()) {
+    Py_RETURN_NONE;
+  }
+  const int64_t layout = layout_of(args[2]);
+  if (!plain_cache(*kp, *vp, layout) || !plain_batch(*table, *lens, cu, *k, *kp)) Py_RETURN_NONE;
+  const int64_t Hkv = kp->size(layout == 1 ? 1 : 2), T = k->size(0);
+  if (!plain_rows(*k, *kp, Hkv) || !plain_rows(*v, *kp, Hkv) || v->size(0) != T || (q != nullptr && (!plain_rows(*q, *kp, -1) || q->size(0) != T)) ||
+      (freq == nullptr) != (axis == nullptr) || (freq == nullptr && (q != nullptr || positions != nullptr)) ||
+      (freq != nullptr && !plain_table(*freq, *axis, n_axes, *kp))) {
+    Py_RETURN_NONE;
+  }
+  int* status = nullptr;
+  const volatile int32_t* mirror = nullptr;
+  if (!sage_device_status(kp->get_device(), &status, &mirror) || (mirror != nullptr && *mirror != 0)) Py_RETURN_NONE;
+  sage_rotary_t r{};
+  if (freq != nullptr) {
+    r = rotary_of(*freq, *axis, n_axes, args[12] == Py_True, *kp);
+    if (positions != nullptr && !plain_positions(&r, *positions, *kp, -1, T)) Py_RETURN_NONE;
+  }
+  at::Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::CUDAGuard guard(kp->device());
+    const sage_paged_kv_t cache = cache_of(*kp, *vp, layout);
+    const sage_paged_batch_t batch = batch_of(*table, *lens, cu != nullptr ? c10::optional<at::Tensor>(*cu) : c10::nullopt, T, *kp);
+    sage_rows_t qs{}, qo{};
+    if (q != nullptr) {
+      out = at::empty(q->sizes(), q->options());
+      qs = rows_of(*q);
+      qo = rows_of(out);
+    }
+    const sage_rows_t ks = rows_of(*k), vs = rows_of(*v);
+    check_rc(sage_paged_append(&cache, &batch, &ks, &vs, q != nullptr ? &qs : nullptr, q != nullptr ? &qo : nullptr,
+                               q != nullptr ? size_of(q->size(1), "heads") : 0, freq != nullptr ? &r : nullptr, status, current_stream(*kp)),
+             "paged_append");
+  }
+  if (q == nullptr) Py_RETURN_TRUE;
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attn_plain(q, k_pages, v_pages, tensor_layout, page_table, kv_lens, cu_q or None, max_q or None, is_causal, sm_scale or None,
+//                  return_lse, shared_pages or None) -> o or (o, lse), or None
+PyObject* sage_paged_attn_plain(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q = nullptr, *kp = nullptr, *vp = nullptr, *table = nullptr, *lens = nullptr, *cu = nullptr, *shared = nullptr;
+  int max_q = 0;
+  if (nargs != 12 || !plain(args[0], &q) || !plain(args[1], &kp) || !plain(args[2], &vp) || !plain(args[4], &table) || !plain(args[5], &lens) ||
+      !plain(args[6], &cu, true) || (args[7] != Py_None && !small_int(args[7], &max_q)) || !PyBool_Check(args[8]) ||
+      (args[9] != Py_None && !PyFloat_CheckExact(args[9])) || !PyBool_Check(args[10]) || !plain(args[11], &shared, true) || modes_active() || checks_status()) {
+    Py_RETURN_NONE;
+  }
+  const int64_t layout = layout_of(args[3]);
+  if (!plain_cache(*kp, *vp, layout) || !plain_rows(*q, *kp, -1) || !plain_batch(*table, *lens, cu, *q, *kp)) Py_RETURN_NONE;
+  const int64_t Hkv = kp->size(layout == 1 ? 1 : 2), Hq = q->size(1), T = q->size(0);
+  if (Hq % Hkv != 0 || Hq / Hkv > 128 || (shared != nullptr && (!plain_int32(*shared, *kp, 1) || shared->size(0) > table->size(1)))) Py_RETURN_NONE;
+  int* status = nullptr;
+  const volatile int32_t* mirror = nullptr;
+  if (!sage_device_status(kp->get_device(), &status, &mirror) || (mirror != nullptr && *mirror != 0)) Py_RETURN_NONE;
+  const double sm_scale = args[9] == Py_None ? std::pow(static_cast<double>(kp->size(3)), -0.5) : PyFloat_AS_DOUBLE(args[9]);
+  const bool causal = args[8] == Py_True, want_lse = args[10] == Py_True;
+  at::Tensor out, lse;
+  {
+    pybind11::gil_scoped_release no_gil;
+    c10::cuda::CUDAGuard guard(kp->device());
+    const sage_paged_kv_t cache = cache_of(*kp, *vp, layout);
+    const sage_paged_batch_t batch = batch_of(*table, *lens, cu != nullptr ? c10::optional<at::Tensor>(*cu) : c10::nullopt, T, *kp);
+    const int heads = size_of(Hq, "heads"), n_shared = shared != nullptr ? size_of(shared->size(0), "shared pages") : 0;
+    out = at::empty(q->sizes(), q->options());
+    if (want_lse) lse = at::empty({T, Hq}, q->options().dtype(at::kFloat));
+    const int64_t bytes = sage_paged_workspace_bytes(&cache, &batch, heads, max_q, n_shared);
+    TORCH_CHECK(bytes >= 0, "paged_attn failed: ", sage_last_error());
+    const c10::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes));
+    const sage_rows_t qs = rows_of(*q), os = rows_of(out);
+    check_rc(sage_paged_attn(&cache, &batch, &qs, &os, heads, max_q, causal, static_cast<float>(sm_scale), want_lse ? lse.data_ptr<float>() : nullptr,
+                             n_shared > 0 ? shared->data_ptr<int32_t>() : nullptr, n_shared, cu != nullptr, status, workspace.get(), bytes,
+                             current_stream(*kp)),
+             "paged_attn");
+  }
+  if (!want_lse) return THPVariable_Wrap(out);
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(out));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(lse));
+  return pair;
+  END_HANDLE_TH_ERRORS
 }

@@ -14,13 +14,14 @@ device: no call synchronises, and every call can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
+import os
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _native
-from .core import _LAYOUT_CODE, _prepare_status, _raise_pending, _status_word
+from .core import _LAYOUT_CODE, _prepare_status, _raise_pending, _register, _status_word, check_status
 from .rotary import RotaryAxes, _vector_aligned
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -78,7 +79,6 @@ class PagedKV:
 
 def _check_batch(cache: PagedKV, rows: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
                  cu_q: Optional[torch.Tensor]) -> None:
-    assert isinstance(cache, PagedKV), "cache must be a PagedKV."
     dev = cache.k_pages.device
     for name, t, dim in (("page_table", page_table, 2), ("kv_lens", kv_lens, 1), ("cu_q", cu_q, 1)):
         if t is None:
@@ -92,6 +92,16 @@ def _check_batch(cache: PagedKV, rows: torch.Tensor, page_table: torch.Tensor, k
         assert rows.size(0) == B, f"without cu_q there is one token per sequence: {rows.size(0)} rows for {B} sequences."
     else:
         assert cu_q.size(0) == B + 1, f"cu_q must have {B + 1} entries, got {cu_q.size(0)}."
+
+
+def _check_if_asked(device: torch.device) -> None:
+    if os.environ.get("SAGEATTN_B200_CHECK_STATUS", "0") == "1":
+        check_status(device)
+
+
+def _table_of(rotary: Optional[RotaryAxes]) -> tuple:
+    """(frequencies, axes, number of axes, interleaved) as the operators take them."""
+    return (None, None, 0, False) if rotary is None else (rotary.freq, rotary.axis, len(rotary.axes), rotary.interleaved)
 
 
 def _check_rows(cache: PagedKV, name: str, t: torch.Tensor, heads: Optional[int] = None) -> None:
@@ -120,6 +130,14 @@ def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table
     outside the cache, a position outside the page table or more new tokens than ``kv_lens`` says are not stored either; they
     are reported like the errors of ``sageattn``, by the next call or ``check_status()``.  Two sequences that share a page
     must not append to it at once."""
+    assert isinstance(cache, PagedKV), "cache must be a PagedKV."
+    assert rotary is None or (isinstance(rotary, RotaryAxes) and rotary.head_dim == cache.head_dim), (
+        "rotary must come from rotary_axes() with the head_dim of the cache.")
+    if not torch.compiler.is_compiling():
+        got = _native.load_module().paged_append_plain(
+            cache.k_pages, cache.v_pages, cache.tensor_layout, k, v, page_table, kv_lens, cu_q, q, *_table_of(rotary), positions)
+        if got is not None:                  # None: not a plain call, or one that the checks below refuse
+            return None if got is True else got
     _check_batch(cache, k, page_table, kv_lens, cu_q)
     _check_rows(cache, "k", k, cache.num_kv_heads)
     _check_rows(cache, "v", v, cache.num_kv_heads)
@@ -132,7 +150,6 @@ def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table
         q = _vector_aligned(q)
     assert positions is None or rotary is not None, "positions are those of rotary."
     if rotary is not None:
-        assert isinstance(rotary, RotaryAxes) and rotary.head_dim == cache.head_dim, "rotary must come from rotary_axes() with the head_dim of the cache."
         assert rotary.freq.device == cache.k_pages.device, "the rotary table is on another device than the cache."
     if positions is not None:
         assert positions.device == cache.k_pages.device and positions.dtype in (torch.int32, torch.int64), (
@@ -147,10 +164,10 @@ def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table
     assert dev.type == "cuda", "the cache must be on a CUDA device."
     ops = _native.load_ops()
     _raise_pending(dev)
+    _register(dev)
     out = ops.paged_append(cache.k_pages, cache.v_pages, _LAYOUT_CODE[cache.tensor_layout], _vector_aligned(k), _vector_aligned(v),
-                           page_table, kv_lens, cu_q, q, None if rotary is None else rotary.freq,
-                           None if rotary is None else rotary.axis, 0 if rotary is None else rotary.n_axes,
-                           0 if rotary is None else int(rotary.interleaved), positions, _status_word(dev))
+                           page_table, kv_lens, cu_q, q, *_table_of(rotary), positions, _status_word(dev))
+    _check_if_asked(dev)
     return out[0] if q is not None else None
 
 
@@ -176,6 +193,12 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
     sequence's last one may be anything, NaN too.  Lengths beyond the page table are cut to it, page indices
     outside the cache are read as page 0, and both are reported like the errors of ``sageattn``, by the next call or
     ``check_status()``.  No gradient."""
+    assert isinstance(cache, PagedKV), "cache must be a PagedKV."
+    if out is None and not torch.compiler.is_compiling():
+        got = _native.load_module().paged_attn_plain(q, cache.k_pages, cache.v_pages, cache.tensor_layout, page_table, kv_lens, cu_q,
+                                                     max_q, is_causal, sm_scale, return_lse, shared_pages)
+        if got is not None:                  # None: not a plain call, or one that the checks below refuse
+            return got
     _check_batch(cache, q, page_table, kv_lens, cu_q)
     _check_rows(cache, "q", q)
     T, heads, B = q.size(0), q.size(1), kv_lens.size(0)
@@ -197,6 +220,7 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
     assert dev.type == "cuda", "the cache must be on a CUDA device."
     ops = _native.load_ops()
     _raise_pending(dev)
+    _register(dev)
     zero_rest = out is None and cu_q is not None
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev) if B > 0 else torch.zeros(q.shape, dtype=q.dtype, device=dev)
@@ -211,4 +235,5 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
                    cu_q, 0 if max_q is None else int(max_q), int(is_causal),
                    cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale), lse, shared_pages, int(zero_rest),
                    _status_word(dev))
+    _check_if_asked(dev)
     return (out, lse) if return_lse else out

@@ -115,6 +115,11 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     ``[S, axes]`` or ``[B, S, axes]``; any integers, negative ones too.  Returns new tensors; the arithmetic is fp32 with
     one rounding at the end.  Differentiable in q and k."""
     assert isinstance(rotary, RotaryAxes), "rotary must come from rotary_axes()."
+    module = _native.load_module()
+    if not torch.compiler.is_compiling():
+        got = module.rotary_plain(q, k, positions, rotary.freq, rotary.axis, len(rotary.axes), rotary.interleaved, rotary.head_dim, tensor_layout)
+        if got is not None:                  # None: not a plain call, or one that the checks below refuse
+            return got
     assert q.dtype in (torch.float16, torch.bfloat16, torch.float32), "Input tensors must be fp16, bf16, or fp32."
     assert tensor_layout in _LAYOUT_CODE, f"tensor_layout must be 'HND' or 'NHD', got {tensor_layout!r}."
     assert q.dim() == 4 and q.size(3) == rotary.head_dim, f"q must be 4-D with head_dim {rotary.head_dim}, got {tuple(q.shape)}."
