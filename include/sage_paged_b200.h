@@ -29,8 +29,8 @@ extern "C" {
  * an integer position wraps at whole turns and is exact for positions of any size.  pairs is a multiple of 8;
  * what a head has behind its pairs is copied. */
 typedef struct sage_rotary {
-  const uint64_t* freq;              /* [pairs] */
-  const int32_t* axis;               /* [pairs], each below n_axes */
+  const uint64_t* freq;              /* [pairs], 16-byte aligned */
+  const int32_t* axis;               /* [pairs], each below n_axes; 16-byte aligned */
   int pairs, n_axes, interleaved;
   const void* positions;             /* n_axes neighbouring integers per token */
   int positions_64;                  /* 0: int32, 1: int64 */

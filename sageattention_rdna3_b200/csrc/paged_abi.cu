@@ -29,7 +29,7 @@ bool stride_ok(int64_t stride, int unit) { return stride % unit == 0; }
 bool rows_ok(const sage_rows_t* r) { return r->ptr != nullptr && aligned16(r->ptr) && r->stride_t % 8 == 0 && r->stride_h % 8 == 0; }
 
 int check_rotary(const sage_rotary_t* r, int D) {
-  SAGE_REQUIRE(r->freq != nullptr && r->axis != nullptr, "rotary: null table");
+  SAGE_REQUIRE(r->freq != nullptr && r->axis != nullptr && aligned16(r->freq) && aligned16(r->axis), "rotary: the table needs 16-byte aligned bases");
   SAGE_REQUIRE(r->pairs >= 8 && r->pairs % 8 == 0 && 2 * r->pairs <= D, "rotary: the number of pairs must be a multiple of 8 and at most head_dim / 2, got %d", r->pairs);
   SAGE_REQUIRE(r->n_axes >= 1 && r->n_axes <= SAGE_MAX_ROTARY_AXES, "rotary: 1 to %d axes, got %d", SAGE_MAX_ROTARY_AXES, r->n_axes);
   return SAGE_OK;
@@ -52,38 +52,31 @@ Rotary rotary_of(const sage_rotary_t* r, int inverse) {
   return x;
 }
 
-// Heads per block of the rotary and append kernels: as many as leave four blocks of 256 threads to every SM, at most 8; few
-// tokens get a thread per group and head.
-struct HeadSplit {
-  int per_block, unroll;
-};
-int split_heads(HeadSplit* out, long long token_blocks, int heads) {
+// Heads per block of the rotary and append kernels: 8, or as many as leave every SM its blocks; 2 for few tokens, whose
+// time is the latency of a call (117 tokens, 60 heads, us with 2 / 4 / 8: 3.8 / 5.0 / 6.6).
+int split_heads(int* per_block, long long token_blocks, int heads) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
-  out->unroll = 4;
-  for (int n : {8, 4}) {
-    out->per_block = n;
-    if (token_blocks * ((heads + n - 1) / n) >= 4LL * sms) return SAGE_OK;
+  for (int n : {8, 4, 2}) {
+    *per_block = n;
+    if (token_blocks * ((heads + n - 1) / n) >= static_cast<long long>(kRotaryBlocks) * sms) break;
   }
-  out->per_block = out->unroll = 1;
   return SAGE_OK;
 }
 
 template <typename T, int D>
-int launch_rotary(const RotaryParams& p, const HeadSplit& split, unsigned token_blocks, cudaStream_t stream) {
+int launch_rotary(const RotaryParams& p, unsigned token_blocks, cudaStream_t stream) {
   const int heads = p.Hq + p.Hkv;
-  const dim3 grid(token_blocks, static_cast<unsigned>((heads + split.per_block - 1) / split.per_block));
-  return split.unroll == 1 ? launch(sage_rotary_kernel<T, D, 1>, grid, kRotaryThreads, 0, stream, p)
-                           : launch(sage_rotary_kernel<T, D, 4>, grid, kRotaryThreads, 0, stream, p);
+  const dim3 grid(token_blocks, static_cast<unsigned>((heads + p.heads_per_block - 1) / p.heads_per_block));
+  return launch(sage_rotary_kernel<T, D>, grid, kRotaryThreads, 0, stream, p);
 }
 
 template <typename T, int D>
-int launch_append(const AppendParams& p, const HeadSplit& split, unsigned token_blocks, cudaStream_t stream) {
+int launch_append(const AppendParams& p, unsigned token_blocks, cudaStream_t stream) {
   const int heads = p.Hq + 2 * p.Hkv;
-  const dim3 grid(token_blocks, static_cast<unsigned>((heads + split.per_block - 1) / split.per_block));
-  return split.unroll == 1 ? launch(sage_paged_append_kernel<T, D, 1>, grid, kRotaryThreads, 0, stream, p)
-                           : launch(sage_paged_append_kernel<T, D, 4>, grid, kRotaryThreads, 0, stream, p);
+  const dim3 grid(token_blocks, static_cast<unsigned>((heads + p.heads_per_block - 1) / p.heads_per_block));
+  return launch(sage_paged_append_kernel<T, D>, grid, kRotaryThreads, 0, stream, p);
 }
 
 int check_cache(const sage_paged_kv_t* c) {
@@ -340,16 +333,14 @@ int sage_apply_rotary(const sage_strided_t* q, const sage_strided_t* q_out, cons
   const int per_block = kRotaryThreads / (D / 16);
   const long long blocks = (static_cast<long long>(B) * S + per_block - 1) / per_block;
   SAGE_REQUIRE(blocks <= 0x7fffffffLL, "rotary: too many tokens");
-  HeadSplit split;
-  rc = split_heads(&split, blocks, Hq + Hkv);
+  SAGE_REQUIRE((Hq + Hkv + 1) / 2 <= 65535, "rotary: too many heads");
+  rc = split_heads(&p.heads_per_block, blocks, Hq + Hkv);
   if (rc) return rc;
-  SAGE_REQUIRE((Hq + Hkv + split.per_block - 1) / split.per_block <= 65535, "rotary: too many heads");
-  p.heads_per_block = split.per_block;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const unsigned n = static_cast<unsigned>(blocks);
-  if (dtype == SAGE_DTYPE_F32) return D == 64 ? launch_rotary<float, 64>(p, split, n, st) : launch_rotary<float, 128>(p, split, n, st);
-  if (dtype == SAGE_DTYPE_F16) return D == 64 ? launch_rotary<__half, 64>(p, split, n, st) : launch_rotary<__half, 128>(p, split, n, st);
-  return D == 64 ? launch_rotary<__nv_bfloat16, 64>(p, split, n, st) : launch_rotary<__nv_bfloat16, 128>(p, split, n, st);
+  if (dtype == SAGE_DTYPE_F32) return D == 64 ? launch_rotary<float, 64>(p, n, st) : launch_rotary<float, 128>(p, n, st);
+  if (dtype == SAGE_DTYPE_F16) return D == 64 ? launch_rotary<__half, 64>(p, n, st) : launch_rotary<__half, 128>(p, n, st);
+  return D == 64 ? launch_rotary<__nv_bfloat16, 64>(p, n, st) : launch_rotary<__nv_bfloat16, 128>(p, n, st);
 }
 
 int sage_paged_append(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, const sage_rows_t* k, const sage_rows_t* v,
@@ -384,14 +375,12 @@ int sage_paged_append(const sage_paged_kv_t* cache, const sage_paged_batch_t* ba
   p.Hq = Hq; p.Hkv = cache->Hkv;
   const int per_block = kRotaryThreads / (cache->D / 16);
   const unsigned blocks = static_cast<unsigned>((static_cast<long long>(batch->T) + per_block - 1) / per_block);
-  HeadSplit split;
-  rc = split_heads(&split, blocks, Hq + 2 * cache->Hkv);
+  SAGE_REQUIRE((Hq + 2 * cache->Hkv + 1) / 2 <= 65535, "append: too many heads");
+  rc = split_heads(&p.heads_per_block, blocks, Hq + 2 * cache->Hkv);
   if (rc) return rc;
-  SAGE_REQUIRE((Hq + 2 * cache->Hkv + split.per_block - 1) / split.per_block <= 65535, "append: too many heads");
-  p.heads_per_block = split.per_block;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cache->dtype == SAGE_DTYPE_F16) return cache->D == 64 ? launch_append<__half, 64>(p, split, blocks, st) : launch_append<__half, 128>(p, split, blocks, st);
-  return cache->D == 64 ? launch_append<__nv_bfloat16, 64>(p, split, blocks, st) : launch_append<__nv_bfloat16, 128>(p, split, blocks, st);
+  if (cache->dtype == SAGE_DTYPE_F16) return cache->D == 64 ? launch_append<__half, 64>(p, blocks, st) : launch_append<__half, 128>(p, blocks, st);
+  return cache->D == 64 ? launch_append<__nv_bfloat16, 64>(p, blocks, st) : launch_append<__nv_bfloat16, 128>(p, blocks, st);
 }
 
 }  // extern "C"

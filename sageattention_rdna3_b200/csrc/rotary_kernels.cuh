@@ -6,12 +6,14 @@
 //
 // The angle.  A position of 10^6 times a frequency in fp32 is off by up to 0.06 radians.  Here the frequency is a
 // fraction of a turn in units of 2^-64; a 64-bit product with the integer position wraps at whole turns by itself, and
-// its upper 32 bits are the angle in [-1/2, 1/2) turns: exact to 2^-33 turns wherever the token stands, without a
-// range reduction.  As fp32 it is off by 2^-25 of itself, and cos and sin by about 2 ulp.
+// its upper 32 bits are the angle, exact to 2^-32 turns wherever the token stands, without a range reduction.
 //
 // The split.  A thread owns 8 pairs of a token (16-byte loads of both halves), computes their 8 angles once and walks over
-// a slice of the heads with them, kUnroll heads in flight: with one head per thread the sines would take longer
-// than the memory.
+// a slice of the heads with them, two heads in flight: with one head per thread the sines take longer than the memory.
+// us, 4213 tokens, 48 + 12 heads of 128 (floor 20.1) / 24576 tokens, 32 heads of 64 (31.2) / append of 8404 tokens, 48 + 24 heads (48):
+// slices of 2 heads 31.7 / 43.6 / 72.3, of 4 26.1 / 35.2 / 60.2, of 8 26.1 / 35.1 / 58.3, of 16 29.5 / 39.2 / 59.7; four heads in flight
+// (three blocks per SM instead of four) in slices of 8 26.9 / 39.0 / 60.1; one 30.0 / 39.2 / 63.7.  sincospif in place of the
+// polynomials below 26.6 / 35.6 / 62.4.
 #pragma once
 
 #include "paged_common.cuh"
@@ -20,6 +22,8 @@ namespace sage {
 namespace paged {
 
 constexpr int kRotaryThreads = 256;
+constexpr int kRotaryBlocks = 4;                      // per SM
+constexpr int kHeadsInFlight = 2;
 
 struct Rotary {
   const uint64_t* freq;         // null: nothing is turned
@@ -80,9 +84,13 @@ struct Group {
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 x = to_float2(wa[i], static_cast<const T*>(nullptr)), y = to_float2(wb[i], static_cast<const T*>(nullptr));
-        wa[i] = from_float2(x.x * c[2 * i] - y.x * s[2 * i], x.y * c[2 * i + 1] - y.y * s[2 * i + 1], static_cast<const T*>(nullptr));
-        wb[i] = from_float2(x.x * s[2 * i] + y.x * c[2 * i], x.y * s[2 * i + 1] + y.y * c[2 * i + 1], static_cast<const T*>(nullptr));
+        const float2 xf = to_float2(wa[i], static_cast<const T*>(nullptr)), yf = to_float2(wb[i], static_cast<const T*>(nullptr));
+        const f32x2_t x = pack2(xf.x, xf.y), y = pack2(yf.x, yf.y);
+        const f32x2_t cc = pack2(c[2 * i], c[2 * i + 1]), ss = pack2(s[2 * i], s[2 * i + 1]);
+        const float2 lo = unpack2(ffma2(y, pack2(-s[2 * i], -s[2 * i + 1]), fmul2(x, cc)));
+        const float2 hi = unpack2(ffma2(y, cc, fmul2(x, ss)));
+        wa[i] = from_float2(lo.x, lo.y, static_cast<const T*>(nullptr));
+        wb[i] = from_float2(hi.x, hi.y, static_cast<const T*>(nullptr));
       }
     }
   }
@@ -106,21 +114,63 @@ __device__ __forceinline__ long long position_at(const Rotary& r, long long offs
                         : static_cast<const int32_t*>(r.positions)[offset + axis];
 }
 
+// cos and sin of 2 pi t / 2^32 for two angles.  The nearest quarter turn is taken off in integers, which leaves r in
+// [-1/8, 1/8] turns, exact to fp32; there sin(2 pi r) = r S(r^2) and cos(2 pi r) = C(r^2) with polynomials of degree 3 and 4, fitted for
+// the smallest largest error (1.2e-9 and 5e-11; 1e-7 with fp32 arithmetic).  Two angles at a time in packed arithmetic this is
+// half the instructions of sincospif, and the sines are what the kernel computes most.
+__device__ __forceinline__ void sincos_turns(uint32_t t0, uint32_t t1, float* s0, float* s1, float* c0, float* c1) {
+  const uint32_t q0 = (t0 + 0x20000000u) >> 30, q1 = (t1 + 0x20000000u) >> 30;
+  const f32x2_t r = fmul2(pack2(static_cast<float>(static_cast<int32_t>(t0 - (q0 << 30))), static_cast<float>(static_cast<int32_t>(t1 - (q1 << 30)))),
+                          pack2(2.3283064365386963e-10f, 2.3283064365386963e-10f));
+  const f32x2_t u = fmul2(r, r);
+  auto both = [](float x) { return pack2(x, x); };
+  f32x2_t s = ffma2(u, both(-75.24006420070805f), both(81.58812464087775f));
+  s = ffma2(u, s, both(-41.34162804270634f));
+  s = fmul2(r, ffma2(u, s, both(6.28318522034183f)));
+  f32x2_t c = ffma2(u, both(59.22040756857688f), both(-85.44285212867844f));
+  c = ffma2(u, c, both(64.93931620850677f));
+  c = ffma2(u, c, both(-19.739208650358023f));
+  c = ffma2(u, c, both(1.0f));
+  const float2 ss = unpack2(s), cc = unpack2(c);
+  // quarter turns: (sin, cos) -> (cos, -sin) -> (-sin, -cos) -> (-cos, sin)
+  auto place = [](uint32_t q, float sn, float cs, float* s_out, float* c_out) {
+    const float a = q & 1u ? cs : sn, b = q & 1u ? sn : cs;
+    *s_out = __uint_as_float(__float_as_uint(a) ^ (q << 30 & 0x80000000u));
+    *c_out = __uint_as_float(__float_as_uint(b) ^ ((q + 1u) << 30 & 0x80000000u));
+  };
+  place(q0, ss.x, cc.x, s0, c0);
+  place(q1, ss.y, cc.y, s1, c1);
+}
+
 // cos and sin of the 8 pairs of a chunk; `pos` holds the token's position on every axis.
 __device__ __forceinline__ void chunk_angles(const Rotary& r, int chunk, const long long (&pos)[SAGE_MAX_ROTARY_AXES], float (&c)[8],
                                              float (&s)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int pair = 8 * chunk + i;
-    const int axis = __ldg(r.axis + pair);
+  const ulonglong2* freq = reinterpret_cast<const ulonglong2*>(r.freq + 8 * chunk);
+  const int4* axes = reinterpret_cast<const int4*>(r.axis + 8 * chunk);
+  uint32_t turns[8];
+  auto turn = [&](int axis, unsigned long long f) -> uint32_t {
     long long at = pos[0];
+    if (r.n_axes > 1) {
+      at = axis == 1 ? pos[1] : at;
+      at = axis == 2 ? pos[2] : at;
+      at = axis == 3 ? pos[3] : at;
+    }
+    return static_cast<uint32_t>(static_cast<unsigned long long>(at) * f >> 32);
+  };
 #pragma unroll
-    for (int a = 1; a < SAGE_MAX_ROTARY_AXES; ++a) at = axis == a ? pos[a] : at;
-    const unsigned long long turns = static_cast<unsigned long long>(at) * __ldg(reinterpret_cast<const unsigned long long*>(r.freq) + pair);
-    // half turns, for sincospi: 2 * 2^-32 of the upper word
-    const float half_turns = static_cast<float>(static_cast<int32_t>(turns >> 32)) * 4.656612873077393e-10f;
-    sincospif(half_turns, &s[i], &c[i]);
-    if (r.inverse) s[i] = -s[i];
+  for (int i = 0; i < 2; ++i) {
+    const int4 a = r.n_axes > 1 ? __ldg(axes + i) : make_int4(0, 0, 0, 0);
+    const ulonglong2 f = __ldg(freq + 2 * i), g = __ldg(freq + 2 * i + 1);
+    turns[4 * i] = turn(a.x, f.x);
+    turns[4 * i + 1] = turn(a.y, f.y);
+    turns[4 * i + 2] = turn(a.z, g.x);
+    turns[4 * i + 3] = turn(a.w, g.y);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) sincos_turns(turns[i], turns[i + 1], &s[i], &s[i + 1], &c[i], &c[i + 1]);
+  if (r.inverse) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = -s[i];
   }
 }
 
@@ -132,8 +182,8 @@ struct RotaryParams {
 };
 
 // grid: (token blocks, slices of the Hq + Hkv heads)
-template <typename T, int D, int UNROLL>
-__global__ void __launch_bounds__(kRotaryThreads) sage_rotary_kernel(const RotaryParams p) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) sage_rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int kChunks = D / 16;
   constexpr int kTokens = kRotaryThreads / kChunks;
   const int chunk = threadIdx.x % kChunks;
@@ -155,11 +205,11 @@ __global__ void __launch_bounds__(kRotaryThreads) sage_rotary_kernel(const Rotar
   };
   float c[8], s[8];
 #pragma unroll 1
-  for (int h = h0; h < h1; h += UNROLL) {
-    Group<T> g[UNROLL];
-    T* out[UNROLL];
+  for (int h = h0; h < h1; h += kHeadsInFlight) {
+    Group<T> g[kHeadsInFlight];
+    T* out[kHeadsInFlight];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
+    for (int u = 0; u < kHeadsInFlight; ++u) {
       const T* in;
       span_of(min(h + u, h1 - 1), &in, &out[u]);
       g[u].load(in + lo, in + hi);
@@ -172,7 +222,7 @@ __global__ void __launch_bounds__(kRotaryThreads) sage_rotary_kernel(const Rotar
       chunk_angles(p.rotary, chunk, pos, c, s);
     }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
+    for (int u = 0; u < kHeadsInFlight; ++u) {
       if (h + u >= h1) break;
       if (turned) g[u].turn(c, s, p.rotary.interleaved != 0);
       g[u].store(out[u] + lo, out[u] + hi);
@@ -192,8 +242,8 @@ struct AppendParams {
 constexpr int kAppendCuMax = 1024;                    // sequences whose cu_q is searched in shared memory
 
 // Heads in the order q, k, v.  grid: (token blocks, slices of the Hq + 2 Hkv heads)
-template <typename T, int D, int UNROLL>
-__global__ void __launch_bounds__(kRotaryThreads) sage_paged_append_kernel(const AppendParams p) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) sage_paged_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kChunks = D / 16;
   constexpr int kTokens = kRotaryThreads / kChunks;
   __shared__ int s_cu[kAppendCuMax + 1];
@@ -256,11 +306,11 @@ __global__ void __launch_bounds__(kRotaryThreads) sage_paged_append_kernel(const
   };
   float c[8], s[8];
 #pragma unroll 1
-  for (int h = h0; h < h1; h += UNROLL) {
-    Group<T> g[UNROLL];
-    T* out[UNROLL];
+  for (int h = h0; h < h1; h += kHeadsInFlight) {
+    Group<T> g[kHeadsInFlight];
+    T* out[kHeadsInFlight];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
+    for (int u = 0; u < kHeadsInFlight; ++u) {
       const T* in;
       span_of(min(h + u, h1 - 1), &in, &out[u]);
       g[u].load(in + lo, in + hi);
@@ -274,7 +324,7 @@ __global__ void __launch_bounds__(kRotaryThreads) sage_paged_append_kernel(const
       chunk_angles(p.rotary, chunk, pos, c, s);
     }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
+    for (int u = 0; u < kHeadsInFlight; ++u) {
       if (h + u >= h1 || out[u] == nullptr) continue;
       if (!belongs) {                                 // a row of q behind the last sequence
 #pragma unroll

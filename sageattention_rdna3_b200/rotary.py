@@ -85,27 +85,6 @@ def _vector_aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, rotary, layout, inverse):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions)
-        ctx.args = (rotary, layout, inverse)
-        out = _native.load_ops().rotary(_vector_aligned(q), None if k is None else _vector_aligned(k), positions, rotary.freq,
-                                        rotary.axis, int(rotary.interleaved), layout, int(inverse))
-        return (out[0], None) if k is None else (out[0], out[1])
-
-    @staticmethod
-    def backward(ctx, grad_q, grad_k):
-        (positions,) = ctx.saved_tensors
-        rotary, layout, inverse = ctx.args
-        if grad_q is not None:                   # a rotation: the gradient is turned the other way
-            grad_q, grad_k = _Rotary.apply(grad_q, grad_k, positions, rotary, layout, not inverse)
-        elif grad_k is not None:
-            grad_k, _ = _Rotary.apply(grad_k, None, positions, rotary, layout, not inverse)
-        return grad_q, grad_k, None, None, None, None
-
-
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: RotaryAxes,
                  tensor_layout: str = "HND") -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """q and k with every pair turned by its frequency times the token's position on the pair's axis.
@@ -141,5 +120,5 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     assert q.is_cuda, "Input tensors must be on a CUDA device."
     if n > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    out = _Rotary.apply(q, k, positions, rotary, _LAYOUT_CODE[tensor_layout], False)
-    return out[0] if k is None else out
+    out = _native.load_ops().rotary(q, k, positions, rotary.freq, rotary.axis, int(rotary.interleaved), _LAYOUT_CODE[tensor_layout], 0)
+    return out[0] if k is None else (out[0], out[1])
