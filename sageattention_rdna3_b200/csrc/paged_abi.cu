@@ -135,15 +135,14 @@ int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t t
   *plan = PagedPlan();
   const int64_t rows = std::min(max_q, tokens) * group;
   plan->tensor = rows > 32;
-  plan->tile_rows = plan->tensor ? kTileM / group * group : rows <= 16 ? 16 : 32;
+  plan->tile_rows = plan->tensor ? 2 * (kTileM / group) * group : rows <= 16 ? 16 : 32;
   // What the start and end of an item cost, in key tiles.  us of the attention kernel with 0 / 1 / 2 / 3: 64 sequences of 60 to
   // 16000 keys, a token each, 157 / 148 / 150 / 152; 32 of 500 to 6000, 3 to 5 tokens (32 rows) 94 / 88 / 81 / 78; chunks of
   // prompts (128 rows) 244 / 235 / 223 / 222; 128 sequences of 1 to 1000 keys, a token each, 47 / 40 / 40 / 43.
   plan->item_cost = plan->tensor ? 2 : plan->tile_rows == 16 ? 1 : 3;
-  const int64_t slots = plan->tensor ? 2 * sms : sms;
   const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
   const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
-  plan->grid = static_cast<int>(std::min<int64_t>(slots, std::min<int64_t>(row_tiles * c->Hkv, slots) * tiles));
+  plan->grid = static_cast<int>(std::min<int64_t>(sms, std::min<int64_t>(row_tiles * c->Hkv, sms) * tiles));
   plan->merge = tiles > 1;
   plan->header_bytes = round16(static_cast<int64_t>(plan->grid) * sizeof(PartHeader));
   plan->e_bytes = round16(static_cast<int64_t>(plan->grid) * 2 * plan->tile_rows * sizeof(float));
@@ -192,7 +191,7 @@ int launch_tile(const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& 
   if (p.batch.T == 1) st = p.Hq > 1 ? sh * p.Hq : row;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(p.Hq), static_cast<cuuint64_t>(p.batch.T)};
   const cuuint64_t strides[2] = {sh, st};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(plan.tile_rows / p.group)};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(plan.tile_rows / 2 / p.group)};
   CUtensorMap tq;
   rc = encode_map(&tq, dt, 3, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "q");
   if (rc) return rc;

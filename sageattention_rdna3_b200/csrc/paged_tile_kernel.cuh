@@ -1,14 +1,17 @@
 // Attention of many rows over a paged cache: chunks of prompts, and a whole batch against the prefix that it shares.
 //
-// The mathematics is that of paged_rows_kernel.cuh; with 128 rows per key tile the products are the work (4 D flops per
-// row and key against 4 D bytes per key), so they go to the tensor cores through tcgen05.  A CTA owns a tile of 128 rows, the
-// query heads of a GQA group for 128 / group new tokens (one TMA box), and streams 128-key tiles:
-//   warp 4    TMA producer  Q; K and V tiles page by page (a box per page, or per 128 keys of a larger page)
-//   warp 5    MMA issuer    S = Q.K^T in halves of 64 keys, O += P.V, fp32 accumulators in TMEM
-//   warps 0-3 softmax       thread t owns row t: running maximum and sum in fp32, P back into TMEM over S
-// Two CTAs fit on an SM (112 KB of shared memory and 256 TMEM columns each), so that the tensor cores of one work under the
-// exponentials of the other.  The grid is 2 * SMs persistent CTAs over equal spans of key tiles (paged_schedule.cuh); loads and the first
-// Q.K^T of the next item run under the end of this one.  TMEM columns: [0,128) S, in place P (16-bit pairs); [128,128+D) O.
+// The mathematics is that of paged_rows_kernel.cuh; with many rows per key tile the products are the work (4 D flops per
+// row and key against 4 D bytes per key), so they go to the tensor cores through tcgen05.  A CTA owns two tiles of up to 128 rows, the
+// query heads of a GQA group for 128 / group new tokens each (one TMA box), and streams 128-key tiles past both:
+//   warp 8     TMA producer  Q; K and V tiles page by page (a box per page, or per 128 keys of a larger page), two stages
+//   warp 9     MMA issuer    S_q = Q_q.K^T, O_q += P_q.V in halves of 64 keys, fp32 accumulators in TMEM
+//   warps 4q.. softmax of tile q: thread t owns row t, running maximum and sum in fp32, P back into TMEM over S
+// While one tile's rows are at their exponentials the tensor cores work for the other; both take as long (D=128: 1024
+// clocks of products and 1024 of the exponential units per tile).  Two row tiles to a key tile also halve what is fetched
+// through the L2: with one (two CTAs of 128 rows per SM, one stage of K and V each) 128 rows of 32 tiles took 66 us,
+// waiting for loads.  A second tile without rows (fewer than 128 rows in all) is left out.
+// The grid is a persistent CTA per SM over equal spans of key tiles (paged_schedule.cuh); loads and the first Q.K^T of the next item
+// run under the end of this one.  TMEM columns: [128 q, 128 q + 128) S_q, in place P_q (16-bit pairs); [256 + D q, ..) O_q.
 //
 // Masks: a row sees the keys below its limit.  Behind the last key of a sequence pages hold anything; the softmax warps
 // write zeros over those rows of V before the product reads them (0 * NaN is NaN), and pages behind it are not
@@ -22,11 +25,11 @@
 namespace sage {
 namespace paged {
 
-constexpr int kTileThreads = 192;
+constexpr int kTileThreads = 320;
 constexpr int kTileM = 128;
 constexpr int kHalfKeys = 64;
-constexpr int kTileTmemCols = 256;
-constexpr int kColO = 128;
+constexpr int kTileTmemCols = 512;
+constexpr int kColO = 256;
 constexpr float kTileBias = 7.0f;                     // log2 of the largest weight while the maximum stands still
 constexpr float kTileLazy = 8.0f;                     // growth of the maximum that is let pass: weights up to 2^15
 constexpr float kTileSumMax = 32768.0f;
@@ -34,24 +37,29 @@ constexpr float kTileRefusedLazy = 2.0f;              // 64 weights add up to mo
 
 template <int D>
 struct TileSmem {
-  static constexpr int kStages = D == 128 ? 1 : 2;
-  static constexpr int kQBytes = kTileM * D * 2;
+  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kQBytes = kTileM * D * 2;      // of one row tile
   static constexpr int kKVBytes = kTileKeys * D * 2;
   static constexpr int kSlab = 128 * 128;             // 128 rows x 64 values, 128-byte swizzle
   static constexpr int kOffQ = 0;
-  static constexpr int kOffK = kQBytes;
+  static constexpr int kOffK = 2 * kQBytes;
   static constexpr int kOffV = kOffK + kStages * kKVBytes;
   static constexpr int kOffBar = kOffV + kStages * kKVBytes;
   static constexpr int kItems = 2;                    // items ahead
-  static constexpr int kNumBars = 10 + 4 * kStages + 2 * kItems;
+  static constexpr int kNumBars = 16 + 4 * kStages + 2 * kItems;
   static constexpr int kOffSegments = kOffBar + 8 * kNumBars;
   static constexpr int kOffScratch = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
   static constexpr int kOffMisc = kOffScratch + 8 * (kTileThreads / 32 + 4);
   static constexpr int kTotal = kOffMisc + 16;
 };
 
+// Row tiles of a segment that have rows.
+__device__ __forceinline__ int n_row_tiles(const AttnParams& p, const Segment& g) {
+  return static_cast<long long>(g.n_q) * p.group - g.row0 > p.tile_rows / 2 ? 2 : 1;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kTileThreads, 2)
+__global__ void __launch_bounds__(kTileThreads, 1)
 sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
   using L = TileSmem<D>;
@@ -64,32 +72,34 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint64_t* q_full = bars + 0;
   uint64_t* q_empty = bars + 1;     // every Q.K^T of the item is complete
-  uint64_t* o_final = bars + 2;     // every P.V of the item is complete
-  uint64_t* o_free = bars + 3;      // all 128 softmax threads hold the item's O in registers
-  uint64_t* s_full = bars + 4;      // [2] S_h holds Q.K_h^T
-  uint64_t* p_full = bars + 6;      // [2] P_h is written (and O scaled) by all 128 softmax threads
-  uint64_t* pv_done = bars + 8;     // [2] O += P_h.V_h is complete
-  uint64_t* k_full = bars + 10;
-  uint64_t* v_full = bars + 10 + kStages;
-  uint64_t* k_empty = bars + 10 + 2 * kStages;
-  uint64_t* v_empty = bars + 10 + 3 * kStages;
-  uint64_t* item_full = bars + 10 + 4 * kStages;               // [kItems] the segment is written
-  uint64_t* item_empty = bars + 10 + 4 * kStages + L::kItems;  // ... and read by the MMA warp and the four softmax warps
+  uint64_t* o_final = bars + 2;     // [2] every P.V of the item's row tile is complete
+  uint64_t* o_free = bars + 4;      // [2] all 128 threads of the tile hold its O in registers
+  uint64_t* s_full = bars + 6;      // [2] S_q holds Q_q.K^T
+  uint64_t* p_full = bars + 8;      // [2][2] half h of P_q is written (and O_q scaled) by all 128 threads of the tile
+  uint64_t* pv_done = bars + 12;    // [2][2] O_q += P_q.V over half h is complete
+  uint64_t* k_full = bars + 16;
+  uint64_t* v_full = bars + 16 + kStages;
+  uint64_t* k_empty = bars + 16 + 2 * kStages;
+  uint64_t* v_empty = bars + 16 + 3 * kStages;
+  uint64_t* item_full = bars + 16 + 4 * kStages;               // [kItems] the segment is written
+  uint64_t* item_empty = bars + 16 + 4 * kStages + L::kItems;  // ... and read by the MMA warp and the eight softmax warps
   Segment* segments = reinterpret_cast<Segment*>(smem + L::kOffSegments);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
   int* fail_code = reinterpret_cast<int*>(smem + L::kOffMisc + 8);
   const bool misaligned = (smem_u32(smem) & 1023u) != 0u;
 
-  if (warp == 4 && elect_one()) {
+  if (warp == 8 && elect_one()) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    mbar_init(o_final, 1);
-    mbar_init(o_free, 128);
-    for (int h = 0; h < 2; ++h) {
-      mbar_init(s_full + h, 1);
-      mbar_init(p_full + h, 128);
-      mbar_init(pv_done + h, 1);
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(o_final + q, 1);
+      mbar_init(o_free + q, 128);
+      mbar_init(s_full + q, 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(p_full + 2 * q + h, 128);
+        mbar_init(pv_done + 2 * q + h, 1);
+      }
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(k_full + s, 1);
@@ -99,7 +109,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     }
     for (int s = 0; s < L::kItems; ++s) {
       mbar_init(item_full + s, 1);
-      mbar_init(item_empty + s, 5);
+      mbar_init(item_empty + s, 9);
     }
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -108,7 +118,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     tma_prefetch_desc(&tm_v);
   }
   grid_dependency_wait();
-  if (warp == 5) {                                    // (after the wait: attn_kernel.cuh)
+  if (warp == 9) {                                    // (after the wait: attn_kernel.cuh)
     tmem_alloc(tmem_slot, kTileTmemCols);
     tmem_relinquish();
   }
@@ -140,7 +150,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (dead_on_arrival) {
     // nothing to do
-  } else if (warp == 4) {
+  } else if (warp == 8) {
     // ------------------------------------------------------------------ TMA producer
     const bool leader = elect_one();
     const int box_rows = min(1 << p.batch.page_log2, kTileKeys);
@@ -179,9 +189,13 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (g.n_tiles == 0) break;
       if (items > 0) SAGE_PAGED_WARP_WAIT_OR(true, q_empty, (items - 1) & 1, 22, { ok = false; break; });
       if (leader) {
-        mbar_arrive_expect_tx(q_full, p.tile_rows * D * 2);
+        const int tiles = n_row_tiles(p, g), half_rows = p.tile_rows / 2;
+        mbar_arrive_expect_tx(q_full, tiles * half_rows * D * 2);
+        for (int q = 0; q < tiles; ++q) {
 #pragma unroll
-        for (int c = 0; c < kSlabs; ++c) tma_load_3d(s_q + c * L::kSlab, &tm_q, q_full, c * 64, g.head0, g.q0 + g.row0 / p.group);
+          for (int c = 0; c < kSlabs; ++c)
+            tma_load_3d(s_q + q * L::kQBytes + c * L::kSlab, &tm_q, q_full, c * 64, g.head0, g.q0 + (g.row0 + q * half_rows) / p.group);
+        }
       }
       __syncwarp();
       const Segment now = g;
@@ -203,80 +217,89 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA issuer
-    // Order of the tensor cores: QK(0,0) QK(0,1) | PV(0,0) QK(1,0) PV(0,1) QK(1,1) | ...
+    // Order of the tensor cores: QK0(0) QK1(0) | PV0(0) QK0(1) | PV1(0) QK1(1) | PV0(1) QK0(2) | ...
     if (elect_one()) {
       constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
-      constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kHalfKeys);
+      constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kTileKeys);
       constexpr uint32_t kIdescPV = umma_idesc(1, kFmt, kFmt, 0, 1, kTileM, D);              // V MN-major
-      const uint32_t t_o = tmem_base + kColO;
-      int kt = 0;
+      int kt = 0;                                     // key tiles so far
+      int qt[2] = {0, 0}, live_items[2] = {0, 0};     // ... and of each row tile; items in which it had rows
       bool ok = true;
-      auto issue_qk = [&](int stage, int h) {
-        // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes, half h of K starts
-        // 64 rows into each slab
+      auto issue_qk = [&](int stage, int q) {
+        // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t slab = (k / 4) * L::kSlab;
-          const uint64_t dq = umma_smem_desc(smem_u32(s_q + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-          const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab + h * (kHalfKeys * 128)), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-          mma_f16_ss(tmem_base + h * kHalfKeys, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
+          const uint64_t dq = umma_smem_desc(smem_u32(s_q + q * L::kQBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+          const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+          mma_f16_ss(tmem_base + q * kTileKeys, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
         }
-        tc_commit(s_full + h);
+        tc_commit(s_full + q);
       };
 #pragma unroll 1
       for (int items = 0; ok; ++items) {
         SAGE_PAGED_WAIT_OR(false, item_full + items % L::kItems, (items / L::kItems) & 1, 34, { ok = false; break; });
         const int n_tiles = segments[items % L::kItems].n_tiles;
+        const int tiles = n_row_tiles(p, segments[items % L::kItems]);
         mbar_arrive(item_empty + items % L::kItems);
         if (n_tiles == 0) break;
         SAGE_PAGED_WAIT_OR(false, q_full, items & 1, 24, { ok = false; break; });
         SAGE_PAGED_WAIT_OR(false, k_full + kt % kStages, (kt / kStages) & 1, 25, { ok = false; break; });
         tc_fence_after();
-        issue_qk(kt % kStages, 0);
-        issue_qk(kt % kStages, 1);
+        for (int q = 0; q < tiles; ++q) issue_qk(kt % kStages, q);
         tc_commit(k_empty + kt % kStages);
         if (n_tiles == 1) tc_commit(q_empty);
 #pragma unroll 1
         for (int j = 0; ok && j < n_tiles; ++j) {
           const int t = kt + j, s = t % kStages, s1 = (t + 1) % kStages;
+#pragma unroll 1
+          for (int q = 0; ok && q < tiles; ++q) {
+            const uint32_t t_o = tmem_base + kColO + q * D;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            SAGE_PAGED_WAIT_OR(false, p_full + h, t & 1, 26, { ok = false; break; });
-            if (h == 0) SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
-            // the first P.V of an item overwrites O: the O of the item before must have been read
-            if (h == 0 && j == 0 && items > 0) SAGE_PAGED_WAIT_OR(false, o_free, (items - 1) & 1, 28, { ok = false; break; });
-            tc_fence_after();
-            // V: [128 keys][64 values] slabs; half h starts 64 rows = 8192 bytes in, an instruction takes 16 rows = 2048 bytes
-            const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes + h * (kHalfKeys * 128)), L::kSlab, 1024, kSwizzle128B);
-#pragma unroll
-            for (int k = 0; k < kHalfKeys / 16; ++k) {
-              mma_f16_ts(t_o, tmem_base + h * kHalfKeys + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || h > 0 || k > 0) ? 1u : 0u);
-            }
-            tc_commit(pv_done + h);
-            if (h == 1) tc_commit(v_empty + s);
-            if (j + 1 < n_tiles) {
-              if (h == 0) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
+            for (int h = 0; h < 2; ++h) {
+              SAGE_PAGED_WAIT_OR(false, p_full + 2 * q + h, qt[q] & 1, 26, { ok = false; break; });
+              if (q == 0 && h == 0) SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
+              // the first P.V of an item overwrites O: the O of the item before must have been read
+              if (j == 0 && h == 0 && live_items[q] > 0) SAGE_PAGED_WAIT_OR(false, o_free + q, (live_items[q] - 1) & 1, 28, { ok = false; break; });
               tc_fence_after();
-              issue_qk(s1, h);
-              if (h == 1) {
+              // V: [128 keys][64 values] slabs; half h starts 64 rows = 8192 bytes in, an instruction takes 16 rows = 2048 bytes
+              const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes + h * (kHalfKeys * 128)), L::kSlab, 1024, kSwizzle128B);
+#pragma unroll
+              for (int k = 0; k < kHalfKeys / 16; ++k) {
+                mma_f16_ts(t_o, tmem_base + q * kTileKeys + h * kHalfKeys + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || h > 0 || k > 0) ? 1u : 0u);
+              }
+              tc_commit(pv_done + 2 * q + h);
+            }
+            if (!ok) break;
+            if (q + 1 == tiles) tc_commit(v_empty + s);
+            if (j + 1 < n_tiles) {
+              if (q == 0) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
+              tc_fence_after();
+              issue_qk(s1, q);
+              if (q + 1 == tiles) {
                 tc_commit(k_empty + s1);
                 if (j + 2 == n_tiles) tc_commit(q_empty);
               }
+            } else {
+              tc_commit(o_final + q);
             }
+            ++qt[q];
           }
         }
-        tc_commit(o_final);
+        for (int q = 0; q < tiles; ++q) ++live_items[q];
         kt += n_tiles;
       }
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax and output
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t t_o = tmem_base + lane_base + kColO;
-    int kt = 0;
+    const int q = warp >> 2;                          // row tile of this warp
+    const int row = (warp & 3) * 32 + lane;           // ... and row of this thread in it
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem_base + lane_base + q * kTileKeys, t_o = tmem_base + lane_base + kColO + q * D;
+    int kt = 0, qt = 0, live_items = 0;               // key tiles so far, those of this row tile, items in which it had rows
     bool ok = true;
 #pragma unroll 1
     for (int items = 0; ok; ++items) {
@@ -285,8 +308,13 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       __syncwarp();
       if (lane == 0) mbar_arrive(item_empty + items % L::kItems);
       if (g.n_tiles == 0) break;
+      if (q >= n_row_tiles(p, g)) {
+        kt += g.n_tiles;
+        continue;
+      }
+      const int half_rows = p.tile_rows / 2;
       int token = 0, head = 0, limit = 0;
-      bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, p.tile_rows, threadIdx.x, &token, &head);
+      bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0 + q * half_rows, half_rows, row, &token, &head);
       if (live) {
         if (p.shared_pass) {
           int q1;
@@ -302,12 +330,14 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       int distrust = 0;                               // > 1: the optimistic pass is skipped
 #pragma unroll 1
       for (int hh = 0; hh < 2 * g.n_tiles; ++hh) {
-        const int t = kt + (hh >> 1), h = hh & 1;
+        const int t = kt + (hh >> 1), tq = qt + (hh >> 1), h = hh & 1;
         const int first = g.key0 + hh * kHalfKeys;
-        SAGE_PAGED_WARP_WAIT_OR(false, s_full + h, t & 1, 31, { ok = false; break; });
-        tc_fence_after();
-        if (h == 0 && first + kTileKeys > g.len) {
-          // The last tile: zeros over what is no value of the sequence.  (Behind the wait for S, which says that the stage's
+        if (h == 0) {
+          SAGE_PAGED_WARP_WAIT_OR(false, s_full + q, tq & 1, 31, { ok = false; break; });
+          tc_fence_after();
+        }
+        if (q == 0 && h == 0 && first + kTileKeys > g.len) {
+          // The last tile: zeros over what is no value of the sequence, by the first row tile (whose P.V comes first).  (Behind the wait for S, which says that the stage's
           // load before this one has long been used: a parity cannot tell phases apart that are two turns away.)
           const int stage = t % kStages;
           SAGE_PAGED_WARP_WAIT_OR(false, v_full + stage, (t / kStages) & 1, 30, { ok = false; break; });
@@ -320,8 +350,8 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         if (warp_live) {
           uint32_t sr[2][32];
-          tmem_ld32(tmem_base + lane_base + h * kHalfKeys, sr[0]);
-          tmem_ld32(tmem_base + lane_base + h * kHalfKeys + 32, sr[1]);
+          tmem_ld32(t_s + h * kHalfKeys, sr[0]);
+          tmem_ld32(t_s + h * kHalfKeys + 32, sr[1]);
           tc_wait_ld();
           const int col_end = live ? limit - first : kHalfKeys;      // columns below it are visible
           const bool masked = __any_sync(0xffffffffu, col_end < kHalfKeys);
@@ -371,7 +401,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (moved) {
               if (hh > 0) {
                 const int hp = h ^ 1;
-                SAGE_PAGED_WARP_WAIT_OR(false, pv_done + hp, (h ? t : t - 1) & 1, 32, { ok = false; break; });
+                SAGE_PAGED_WARP_WAIT_OR(false, pv_done + 2 * q + hp, (h ? tq : tq - 1) & 1, 32, { ok = false; break; });
                 tc_fence_after();
                 const float back = need ? ex2(m - top) : 1.0f;
                 l *= back;
@@ -391,20 +421,20 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (masked) l += exp_pass(std::true_type{}, base);
             else l += exp_pass(std::false_type{}, base);
           }
-          tmem_st32(tmem_base + lane_base + h * kHalfKeys, pk);
+          tmem_st32(t_s + h * kHalfKeys, pk);
           tc_wait_st();
         }
         tc_fence_before();
-        mbar_arrive(p_full + h);
+        mbar_arrive(p_full + 2 * q + h);
       }
       if (!ok) break;
-      SAGE_PAGED_WARP_WAIT_OR(false, o_final, items & 1, 33, { ok = false; break; });
+      SAGE_PAGED_WARP_WAIT_OR(false, o_final + q, live_items & 1, 33, { ok = false; break; });
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (g.slot == 1 && threadIdx.x == 0) {
         p.headers[blockIdx.x] = PartHeader{g.n_parts, g.q0, g.n_q, g.head0, g.row0, p.tile_rows, {0, 0}};
       }
-      const long long at = (static_cast<long long>(blockIdx.x) * 2 + g.slot) * p.tile_rows + threadIdx.x;
+      const long long at = (static_cast<long long>(blockIdx.x) * 2 + g.slot) * p.tile_rows + q * half_rows + row;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t orr[32];
@@ -414,7 +444,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         if (c == D / 32 - 1) {                        // O is in registers: the next item may overwrite it
           tc_fence_before();
-          mbar_arrive(o_free);
+          mbar_arrive(o_free + q);
         }
         if (!live) continue;
         float x[32];
@@ -429,8 +459,10 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
       kt += g.n_tiles;
+      qt += g.n_tiles;
+      ++live_items;
     }
-    if (ok) zero_rest<T>(p, D, threadIdx.x, 128);
+    if (ok) zero_rest<T>(p, D, threadIdx.x, 256);
   }
 #undef SAGE_PAGED_WAIT_OR
 #undef SAGE_PAGED_WARP_WAIT_OR
@@ -444,7 +476,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     if (threadIdx.x == 0) p.status.report(*fail_code ? *fail_code : kStatusWait);
     __syncthreads();
   }
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTileTmemCols);
   }
