@@ -215,11 +215,11 @@ int launch_pass(const sage_paged_kv_t* c, AttnParams p, const PagedPlan& plan, c
   if (plan.tensor) {
     rc = launch_tile<T, D>(tk, tv, p, plan, dt, stream);
     if (rc || !plan.merge) return rc;
-    return launch(sage_paged_merge_kernel<T, D, 8>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>((plan.tile_rows + 7) / 8)), kMergeThreads, 0, stream, p);
+    return launch(sage_paged_merge_columns_kernel<T, D>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>((plan.tile_rows + 31) / 32)), kMergeThreads, 0, stream, p);
   }
   rc = plan.tile_rows == 16 ? launch_rows<T, D, 1>(tk, tv, p, plan, stream) : launch_rows<T, D, 2>(tk, tv, p, plan, stream);
   if (rc || !plan.merge) return rc;
-  return launch(sage_paged_merge_kernel<T, D, 2>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>(plan.tile_rows / 2)), kMergeThreads, 0, stream, p);
+  return launch(sage_paged_merge_rows_kernel<T, D, 2>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>(plan.tile_rows / 2)), kMergeThreads, 0, stream, p);
 }
 
 int dispatch_pass(const sage_paged_kv_t* c, const AttnParams& p, const PagedPlan& plan, char* workspace, cudaStream_t stream) {

@@ -5,7 +5,7 @@
 // stand for its start and end.  The steps of all items, after sequence, kv head after kv head, row tile after row tile, form one line that is cut into equal spans, one per CTA:
 // lengths may differ as they like and all CTAs get the same amount of work.  A span that covers part of an item leaves
 // its result in a slot of the workspace (slot 1 the head of an item, slot 0 anything else: at most one of each per
-// CTA) and a header that tells sage_paged_merge_kernel which parts follow.  Every CTA works this out for itself from kv_lens and
+// CTA) and a header that tells the merge kernels which parts follow.  Every CTA works this out for itself from kv_lens and
 // cu_q, by a block-wide prefix sum; nothing is communicated and the order of all sums is fixed.
 #pragma once
 
@@ -357,29 +357,68 @@ __device__ __forceinline__ void zero_rest(const AttnParams& p, int D, int thread
   }
 }
 
-// One CTA: part `blockIdx.y` of the rows of header `blockIdx.x`.  A warp per row and group of parts; the kRowWarps warps of a row
-// take every kRowWarps-th part, four in flight, and are joined in shared memory in a fixed order.
+// Joins the parts of items.  blockIdx.x: header, blockIdx.y: rows.  Two layouts of a part (tile_rows x D floats), each as its
+// writer stores it in whole lines:
+//   rows (sage_paged_rows_kernel)  row after row; a warp has one row, kWarps / ROWS warps every so many parts of it
+//   columns (sage_paged_tile_kernel, a thread per row)  4 neighbouring values of all rows, then the next 4; here a warp has 32
+//   rows and kVecs of their float4 columns
+// Four parts are in flight together, in the order of the keys: the result does not depend on who came first.
 constexpr int kMergeThreads = 256;
+
+template <int N>
+struct PartSum {
+  float e = -INFINITY, sum = 0.0f, x[N];              // maximum; the row so far is x / sum
+  __device__ __forceinline__ PartSum() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0.0f;
+  }
+  __device__ __forceinline__ void add(const float (&pe)[4], const float (&px)[4][N]) {
+    float top = e;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) top = fmaxf(top, pe[c]);
+    if (top == -INFINITY) return;                     // no visible keys so far
+    const float back = exp2f(e - top);
+    sum *= back;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= back;
+    e = top;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float f = exp2f(pe[c] - top);
+      sum += f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] += f * px[c][i];
+    }
+  }
+  __device__ __forceinline__ void normalise() {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= inv;
+  }
+  __device__ __forceinline__ float lse() const { return sum == 0.0f ? -INFINITY : e + log2f(sum); }
+};
+
+// The row of a merge thread, if it has one that belongs to a sequence.
+__device__ __forceinline__ bool merge_row(const AttnParams& p, const PartHeader& h, int r, int* token, int* head) {
+  if (!row_at(h.token0, h.tokens, h.head0, p.group, h.row0, h.rows, r, token, head)) return false;
+  int q1;
+  return !p.shared_pass || seq_of_token(p, *token, &q1) < p.batch.B;
+}
+
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_rows_kernel(const __grid_constant__ AttnParams p) {
   constexpr int kWarps = kMergeThreads / 32, kRowWarps = kWarps / ROWS, kPer = D / 32;   // values per lane: 4 or 2
   __shared__ float s_o[kWarps][D];
   __shared__ float s_e[kWarps];
   grid_dependency_wait();
   grid_launch_dependents();
   const PartHeader h = p.headers[blockIdx.x];
-  if (h.n_parts < 2) return;
+  if (h.n_parts < 2 || static_cast<long long>(h.tokens) * p.group <= h.row0 + static_cast<int>(blockIdx.y) * ROWS) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.y * ROWS + warp / kRowWarps, w = warp % kRowWarps;
   int token = 0, head = 0;
-  bool live = row_at(h.token0, h.tokens, h.head0, p.group, h.row0, h.rows, r, &token, &head);
-  if (live && p.shared_pass) {
-    int q1;
-    live = seq_of_token(p, token, &q1) < p.batch.B;
-  }
-  float e = -INFINITY, sum = 0.0f, x[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
+  const bool live = merge_row(p, h, r, &token, &head);
+  PartSum<kPer> acc;
   if (live) {
     for (int k0 = w; k0 < h.n_parts; k0 += 4 * kRowWarps) {
       float pe[4], px[4][kPer];
@@ -392,58 +431,69 @@ __global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_kernel(const A
         if (k < h.n_parts) {
           const long long at = ((static_cast<long long>(blockIdx.x) + k) * 2 + (k == 0 ? 1 : 0)) * p.tile_rows + r;
           pe[c] = p.part_e[at];
-          const float* src = p.part_o + at * D + lane * kPer;
-          load_floats(src, px[c]);
+          load_floats(p.part_o + at * D + lane * kPer, px[c]);
         }
       }
-      float top = e;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) top = fmaxf(top, pe[c]);
-      if (top == -INFINITY) continue;                 // no visible keys so far
-      const float back = exp2f(e - top);
-      sum *= back;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] *= back;
-      e = top;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float f = exp2f(pe[c] - top);
-        sum += f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] += f * px[c][i];
-      }
+      acc.add(pe, px);
     }
   }
-  // e: the maximum; the row is x / sum, its log-sum-exp e + log2(sum)
+  acc.normalise();
   if constexpr (kRowWarps > 1) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) s_o[warp][lane * kPer + i] = x[i] * inv;
-    if (lane == 0) s_e[warp] = part_lse(e, sum);
+    const float e = part_lse(acc.e, acc.sum);
+    store_floats(&s_o[warp][lane * kPer], acc.x);
+    if (lane == 0) s_e[warp] = e;
     __syncthreads();
     if (w != 0 || !live) return;
-    float top = -INFINITY;
+    acc = PartSum<kPer>();
 #pragma unroll
-    for (int c = 0; c < kRowWarps; ++c) top = fmaxf(top, s_e[warp + c]);
-    sum = 0.0f;
+    for (int c0 = 0; c0 < kRowWarps; c0 += 4) {
+      float pe[4], px[4][kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
-    e = top;
-    if (top > -INFINITY) {
+      for (int c = 0; c < 4; ++c) {
+        pe[c] = s_e[warp + c0 + c];
+        load_floats(&s_o[warp + c0 + c][lane * kPer], px[c]);
+      }
+      acc.add(pe, px);
+    }
+    acc.normalise();
+  }
+  if (live) write_row<T, kPer>(p, token, head, D, lane * kPer, acc.x, acc.lse(), lane == 0);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_columns_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int kVecs = D / 4 / (kMergeThreads / 32);           // float4 columns per thread: 4 or 2
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const PartHeader h = p.headers[blockIdx.x];
+  if (h.n_parts < 2 || static_cast<long long>(h.tokens) * p.group <= h.row0 + static_cast<int>(blockIdx.y) * 32) return;
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), c0 = (threadIdx.x >> 5) * kVecs;
+  int token = 0, head = 0;
+  if (!merge_row(p, h, r, &token, &head)) return;
+  PartSum<4 * kVecs> acc;
+  for (int k0 = 0; k0 < h.n_parts; k0 += 4) {
+    float pe[4], px[4][4 * kVecs];
 #pragma unroll
-      for (int c = 0; c < kRowWarps; ++c) {
-        const float f = exp2f(s_e[warp + c] - top);
-        sum += f;
+    for (int c = 0; c < 4; ++c) {
+      const int k = k0 + c;
+      pe[c] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] += f * s_o[warp + c][lane * kPer + i];
+      for (int i = 0; i < 4 * kVecs; ++i) px[c][i] = 0.0f;
+      if (k < h.n_parts) {
+        const long long slot = (static_cast<long long>(blockIdx.x) + k) * 2 + (k == 0 ? 1 : 0);
+        pe[c] = p.part_e[slot * p.tile_rows + r];
+        const float4* src = reinterpret_cast<const float4*>(p.part_o) + (slot * (D / 4) + c0) * p.tile_rows + r;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          const float4 v = src[i * p.tile_rows];
+          px[c][4 * i] = v.x; px[c][4 * i + 1] = v.y; px[c][4 * i + 2] = v.z; px[c][4 * i + 3] = v.w;
+        }
       }
     }
+    acc.add(pe, px);
   }
-  if (!live) return;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] *= inv;
-  write_row<T, kPer>(p, token, head, D, lane * kPer, x, sum == 0.0f ? -INFINITY : e + log2f(sum), lane == 0);
+  acc.normalise();
+  write_row<T, 4 * kVecs>(p, token, head, D, 4 * c0, acc.x, acc.lse(), c0 == 0);
 }
 
 }  // namespace paged

@@ -4,12 +4,12 @@
 // row and key against 4 D bytes per key), so they go to the tensor cores through tcgen05.  A CTA owns two tiles of up to 128 rows, the
 // query heads of a GQA group for 128 / group new tokens each (one TMA box), and streams 128-key tiles past both:
 //   warp 8     TMA producer  Q; K and V tiles page by page (a box per page, or per 128 keys of a larger page), two stages
-//   warp 9     MMA issuer    S_q = Q_q.K^T, O_q += P_q.V in halves of 64 keys, fp32 accumulators in TMEM
+//   warp 9+q   MMA issuer    S_q = Q_q.K^T, O_q += P_q.V in halves of 64 keys, fp32 accumulators in TMEM
 //   warps 4q.. softmax of tile q: thread t owns row t, running maximum and sum in fp32, P back into TMEM over S
-// While one tile's rows are at their exponentials the tensor cores work for the other; both take as long (D=128: 1024
-// clocks of products and 1024 of the exponential units per tile).  Two row tiles to a key tile also halve what is fetched
-// through the L2: with one (two CTAs of 128 rows per SM, one stage of K and V each) 128 rows of 32 tiles took 66 us,
-// waiting for loads.  A second tile without rows (fewer than 128 rows in all) is left out.
+// While a tile's rows are at the exponentials of one half the tensor cores work on its other half, and for the other tile
+// (D=128: 1024 clocks of products and 1024 of the exponential units per tile); each tile has an issuer of its own, or one would wait for the
+// other's rows.  Two row tiles to a key tile also halve what is fetched through the L2.  A second tile without rows (fewer
+// than 128 rows in all) is left out.
 // The grid is a persistent CTA per SM over equal spans of key tiles (paged_schedule.cuh); loads and the first Q.K^T of the next item
 // run under the end of this one.  TMEM columns: [128 q, 128 q + 128) S_q, in place P_q (16-bit pairs); [256 + D q, ..) O_q.
 //
@@ -25,7 +25,8 @@
 namespace sage {
 namespace paged {
 
-constexpr int kTileThreads = 320;
+constexpr int kTileThreads = 384;
+constexpr int kSoftmaxWarps = 8;
 constexpr int kTileM = 128;
 constexpr int kHalfKeys = 64;
 constexpr int kTileTmemCols = 512;
@@ -46,7 +47,7 @@ struct TileSmem {
   static constexpr int kOffV = kOffK + kStages * kKVBytes;
   static constexpr int kOffBar = kOffV + kStages * kKVBytes;
   static constexpr int kItems = 2;                    // items ahead
-  static constexpr int kNumBars = 16 + 4 * kStages + 2 * kItems;
+  static constexpr int kNumBars = 18 + 4 * kStages + 2 * kItems;
   static constexpr int kOffSegments = kOffBar + 8 * kNumBars;
   static constexpr int kOffScratch = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
   static constexpr int kOffMisc = kOffScratch + 8 * (kTileThreads / 32 + 4);
@@ -74,15 +75,15 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   uint64_t* q_empty = bars + 1;     // every Q.K^T of the item is complete
   uint64_t* o_final = bars + 2;     // [2] every P.V of the item's row tile is complete
   uint64_t* o_free = bars + 4;      // [2] all 128 threads of the tile hold its O in registers
-  uint64_t* s_full = bars + 6;      // [2] S_q holds Q_q.K^T
-  uint64_t* p_full = bars + 8;      // [2][2] half h of P_q is written (and O_q scaled) by all 128 threads of the tile
-  uint64_t* pv_done = bars + 12;    // [2][2] O_q += P_q.V over half h is complete
-  uint64_t* k_full = bars + 16;
-  uint64_t* v_full = bars + 16 + kStages;
-  uint64_t* k_empty = bars + 16 + 2 * kStages;
-  uint64_t* v_empty = bars + 16 + 3 * kStages;
-  uint64_t* item_full = bars + 16 + 4 * kStages;               // [kItems] the segment is written
-  uint64_t* item_empty = bars + 16 + 4 * kStages + L::kItems;  // ... and read by the MMA warp and the eight softmax warps
+  uint64_t* s_full = bars + 6;      // [2][2] half h of S_q holds Q_q.K_h^T
+  uint64_t* p_full = bars + 10;     // [2][2] half h of P_q is written (and O_q scaled) by all 128 threads of the tile
+  uint64_t* pv_done = bars + 14;    // [2][2] O_q += P_q.V over half h is complete
+  uint64_t* k_full = bars + 18;
+  uint64_t* v_full = bars + 18 + kStages;
+  uint64_t* k_empty = bars + 18 + 2 * kStages;      // (by both issuers)
+  uint64_t* v_empty = bars + 18 + 3 * kStages;
+  uint64_t* item_full = bars + 18 + 4 * kStages;               // [kItems] the segment is written
+  uint64_t* item_empty = bars + 18 + 4 * kStages + L::kItems;  // ... and read by the issuers and the eight softmax warps
   Segment* segments = reinterpret_cast<Segment*>(smem + L::kOffSegments);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
@@ -91,12 +92,12 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (warp == 8 && elect_one()) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int q = 0; q < 2; ++q) {
       mbar_init(o_final + q, 1);
       mbar_init(o_free + q, 128);
-      mbar_init(s_full + q, 1);
       for (int h = 0; h < 2; ++h) {
+        mbar_init(s_full + 2 * q + h, 1);
         mbar_init(p_full + 2 * q + h, 128);
         mbar_init(pv_done + 2 * q + h, 1);
       }
@@ -104,12 +105,12 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     for (int s = 0; s < kStages; ++s) {
       mbar_init(k_full + s, 1);
       mbar_init(v_full + s, 1);
-      mbar_init(k_empty + s, 1);
-      mbar_init(v_empty + s, 1);
+      mbar_init(k_empty + s, 2);
+      mbar_init(v_empty + s, 2);
     }
     for (int s = 0; s < L::kItems; ++s) {
       mbar_init(item_full + s, 1);
-      mbar_init(item_empty + s, 9);
+      mbar_init(item_empty + s, 10);
     }
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -217,78 +218,86 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMA issuer
-    // Order of the tensor cores: QK0(0) QK1(0) | PV0(0) QK0(1) | PV1(0) QK1(1) | PV0(1) QK0(2) | ...
-    if (elect_one()) {
+  } else if (warp < kSoftmaxWarps + 4 && warp > kSoftmaxWarps) {
+    // ------------------------------------------------------------------ MMA issuers
+    // Each for its row tile: QK(0,0) QK(0,1) | PV(0,0) QK(1,0) PV(0,1) QK(1,1) | ...
+    const int q = warp - kSoftmaxWarps - 1;
+    if (q < 2 && elect_one()) {
       constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
-      constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kTileKeys);
+      constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kHalfKeys);
       constexpr uint32_t kIdescPV = umma_idesc(1, kFmt, kFmt, 0, 1, kTileM, D);              // V MN-major
-      int kt = 0;                                     // key tiles so far
-      int qt[2] = {0, 0}, live_items[2] = {0, 0};     // ... and of each row tile; items in which it had rows
+      const uint32_t t_s = tmem_base + q * kTileKeys, t_o = tmem_base + kColO + q * D;
+      int kt = 0, qt = 0, live_items = 0;             // key tiles so far, those of this row tile, items in which it had rows
       bool ok = true;
-      auto issue_qk = [&](int stage, int q) {
-        // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes
+      auto issue_qk = [&](int stage, int h) {
+        // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes, half h of K starts
+        // 64 rows into each slab
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t slab = (k / 4) * L::kSlab;
           const uint64_t dq = umma_smem_desc(smem_u32(s_q + q * L::kQBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-          const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-          mma_f16_ss(tmem_base + q * kTileKeys, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
+          const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab + h * (kHalfKeys * 128)), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+          mma_f16_ss(t_s + h * kHalfKeys, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
         }
-        tc_commit(s_full + q);
+        tc_commit(s_full + 2 * q + h);
       };
 #pragma unroll 1
       for (int items = 0; ok; ++items) {
         SAGE_PAGED_WAIT_OR(false, item_full + items % L::kItems, (items / L::kItems) & 1, 34, { ok = false; break; });
         const int n_tiles = segments[items % L::kItems].n_tiles;
-        const int tiles = n_row_tiles(p, segments[items % L::kItems]);
+        const bool idle = q >= n_row_tiles(p, segments[items % L::kItems]);
         mbar_arrive(item_empty + items % L::kItems);
         if (n_tiles == 0) break;
         SAGE_PAGED_WAIT_OR(false, q_full, items & 1, 24, { ok = false; break; });
+        if (idle) {                                   // lets every stage go as it comes: phases are counted by all
+          for (int j = 0; ok && j < n_tiles; ++j, ++kt) {
+            const int s = kt % kStages;
+            SAGE_PAGED_WAIT_OR(false, k_full + s, (kt / kStages) & 1, 25, { ok = false; break; });
+            mbar_arrive(k_empty + s);
+            SAGE_PAGED_WAIT_OR(false, v_full + s, (kt / kStages) & 1, 27, { ok = false; break; });
+            mbar_arrive(v_empty + s);
+          }
+          mbar_arrive(q_empty);
+          continue;
+        }
         SAGE_PAGED_WAIT_OR(false, k_full + kt % kStages, (kt / kStages) & 1, 25, { ok = false; break; });
         tc_fence_after();
-        for (int q = 0; q < tiles; ++q) issue_qk(kt % kStages, q);
+        issue_qk(kt % kStages, 0);
+        issue_qk(kt % kStages, 1);
         tc_commit(k_empty + kt % kStages);
         if (n_tiles == 1) tc_commit(q_empty);
 #pragma unroll 1
         for (int j = 0; ok && j < n_tiles; ++j) {
           const int t = kt + j, s = t % kStages, s1 = (t + 1) % kStages;
-#pragma unroll 1
-          for (int q = 0; ok && q < tiles; ++q) {
-            const uint32_t t_o = tmem_base + kColO + q * D;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              SAGE_PAGED_WAIT_OR(false, p_full + 2 * q + h, qt[q] & 1, 26, { ok = false; break; });
-              if (q == 0 && h == 0) SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
-              // the first P.V of an item overwrites O: the O of the item before must have been read
-              if (j == 0 && h == 0 && live_items[q] > 0) SAGE_PAGED_WAIT_OR(false, o_free + q, (live_items[q] - 1) & 1, 28, { ok = false; break; });
-              tc_fence_after();
-              // V: [128 keys][64 values] slabs; half h starts 64 rows = 8192 bytes in, an instruction takes 16 rows = 2048 bytes
-              const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes + h * (kHalfKeys * 128)), L::kSlab, 1024, kSwizzle128B);
+          for (int h = 0; h < 2; ++h) {
+            SAGE_PAGED_WAIT_OR(false, p_full + 2 * q + h, qt & 1, 26, { ok = false; break; });
+            if (h == 0) SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
+            // the first P.V of an item overwrites O: the O of the item before must have been read
+            if (j == 0 && h == 0 && live_items > 0) SAGE_PAGED_WAIT_OR(false, o_free + q, (live_items - 1) & 1, 28, { ok = false; break; });
+            tc_fence_after();
+            // V: [128 keys][64 values] slabs; half h starts 64 rows = 8192 bytes in, an instruction takes 16 rows = 2048 bytes
+            const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes + h * (kHalfKeys * 128)), L::kSlab, 1024, kSwizzle128B);
 #pragma unroll
-              for (int k = 0; k < kHalfKeys / 16; ++k) {
-                mma_f16_ts(t_o, tmem_base + q * kTileKeys + h * kHalfKeys + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || h > 0 || k > 0) ? 1u : 0u);
-              }
-              tc_commit(pv_done + 2 * q + h);
+            for (int k = 0; k < kHalfKeys / 16; ++k) {
+              mma_f16_ts(t_o, t_s + h * kHalfKeys + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || h > 0 || k > 0) ? 1u : 0u);
             }
-            if (!ok) break;
-            if (q + 1 == tiles) tc_commit(v_empty + s);
+            tc_commit(pv_done + 2 * q + h);
+            if (h == 1) tc_commit(v_empty + s);
             if (j + 1 < n_tiles) {
-              if (q == 0) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
+              if (h == 0) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
               tc_fence_after();
-              issue_qk(s1, q);
-              if (q + 1 == tiles) {
+              issue_qk(s1, h);
+              if (h == 1) {
                 tc_commit(k_empty + s1);
                 if (j + 2 == n_tiles) tc_commit(q_empty);
               }
-            } else {
-              tc_commit(o_final + q);
             }
-            ++qt[q];
           }
+          ++qt;
         }
-        for (int q = 0; q < tiles; ++q) ++live_items[q];
+        tc_commit(o_final + q);
+        ++live_items;
         kt += n_tiles;
       }
     }
@@ -332,17 +341,15 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       for (int hh = 0; hh < 2 * g.n_tiles; ++hh) {
         const int t = kt + (hh >> 1), tq = qt + (hh >> 1), h = hh & 1;
         const int first = g.key0 + hh * kHalfKeys;
-        if (h == 0) {
-          SAGE_PAGED_WARP_WAIT_OR(false, s_full + q, tq & 1, 31, { ok = false; break; });
-          tc_fence_after();
-        }
-        if (q == 0 && h == 0 && first + kTileKeys > g.len) {
-          // The last tile: zeros over what is no value of the sequence, by the first row tile (whose P.V comes first).  (Behind the wait for S, which says that the stage's
+        SAGE_PAGED_WARP_WAIT_OR(false, s_full + 2 * q + h, tq & 1, 31, { ok = false; break; });
+        tc_fence_after();
+        if (h == 0 && first + kTileKeys > g.len) {
+          // The last tile: zeros over what is no value of the sequence, by both row tiles, either of which may be first.  (Behind the wait for S, which says that the stage's
           // load before this one has long been used: a parity cannot tell phases apart that are two turns away.)
           const int stage = t % kStages;
           SAGE_PAGED_WARP_WAIT_OR(false, v_full + stage, (t / kStages) & 1, 30, { ok = false; break; });
           const int keys = max(g.len - first, 0);
-          for (int i = threadIdx.x; i < (kTileKeys - keys) * kSlabs * 8; i += 128) {
+          for (int i = threadIdx.x & 127; i < (kTileKeys - keys) * kSlabs * 8; i += 128) {
             const int row = keys + i / (kSlabs * 8), x = i % (kSlabs * 8);
             *reinterpret_cast<uint4*>(s_v + stage * L::kKVBytes + (x >> 3) * L::kSlab + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
@@ -434,7 +441,8 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (g.slot == 1 && threadIdx.x == 0) {
         p.headers[blockIdx.x] = PartHeader{g.n_parts, g.q0, g.n_q, g.head0, g.row0, p.tile_rows, {0, 0}};
       }
-      const long long at = (static_cast<long long>(blockIdx.x) * 2 + g.slot) * p.tile_rows + q * half_rows + row;
+      const int slot = blockIdx.x * 2 + g.slot, part_row = q * half_rows + row;
+      float4* part = reinterpret_cast<float4*>(p.part_o) + static_cast<long long>(slot) * p.tile_rows * (D / 4) + part_row;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t orr[32];
@@ -452,8 +460,8 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(orr[i]) * inv;
         if (g.slot >= 0) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) reinterpret_cast<float4*>(p.part_o + at * D + 32 * c)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-          if (c == 0) p.part_e[at] = part_lse(m - kTileBias, l);
+          for (int i = 0; i < 8; ++i) part[(8 * c + i) * p.tile_rows] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          if (c == 0) p.part_e[slot * p.tile_rows + part_row] = part_lse(m - kTileBias, l);
         } else {
           write_row<T, 32>(p, token, head, D, 32 * c, x, l == 0.0f ? -INFINITY : m - kTileBias + log2f(l), c == 0);
         }
