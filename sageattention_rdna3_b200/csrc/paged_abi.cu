@@ -202,6 +202,8 @@ template <typename T, int D>
 int launch_pass(const sage_paged_kv_t* c, AttnParams p, const PagedPlan& plan, char* workspace, cudaStream_t stream) {
   p.tile_rows = plan.tile_rows;
   p.item_cost = plan.item_cost;
+  p.by_group = FastDiv::of(p.group);
+  p.by_tile_rows = FastDiv::of(p.tile_rows);
   p.headers = reinterpret_cast<PartHeader*>(workspace);
   p.part_e = reinterpret_cast<float*>(workspace + plan.header_bytes);
   p.part_o = reinterpret_cast<float*>(workspace + plan.header_bytes + plan.e_bytes);
@@ -235,6 +237,7 @@ int check_attn(const sage_paged_kv_t* cache, const sage_paged_batch_t* batch, in
   if (rc) return rc;
   SAGE_REQUIRE(Hq >= 1 && Hq % cache->Hkv == 0 && Hq / cache->Hkv <= 128, "num_qo_heads must be a multiple of num_kv_heads, at most 128 times it; got %d and %d", Hq, cache->Hkv);
   SAGE_REQUIRE(max_q >= 0 && n_shared >= 0, "negative sizes");
+  SAGE_REQUIRE(static_cast<int64_t>(batch->T) * Hq <= 0x7fff0000, "paged attention: too many rows");
   SAGE_REQUIRE(static_cast<int64_t>(n_shared) * cache->page_size <= 0x3fffffff && static_cast<int64_t>(batch->table_width) * cache->page_size <= 0x3fffffff,
                "a sequence may have at most 2^30 keys");
   SAGE_REQUIRE(n_shared <= batch->table_width || batch->B == 0, "the page table has fewer columns than there are shared pages");

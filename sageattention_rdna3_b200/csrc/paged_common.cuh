@@ -60,6 +60,12 @@ struct Batch {
   }
 };
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // 16-bit types <-> fp32
 __device__ __forceinline__ float2 to_float2(uint32_t w, const __half*) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ float2 to_float2(uint32_t w, const __nv_bfloat16*) {

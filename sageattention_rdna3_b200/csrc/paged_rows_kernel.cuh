@@ -49,11 +49,6 @@ struct RowsSmem {
   static_assert(kTotal <= 232448, "shared memory of an SM");
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -149,21 +144,21 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       boxes = (keys + box_rows - 1) / box_rows;
       pages = lane < boxes ? page_of_key(p, g.b, first + lane * box_rows) : 0;
     };
-    Segment g = it.next();
-    if (g.n_tiles > 0) find_pages(g, 0);
 #pragma unroll 1
     for (int item = 0; ok; ++item) {
       const int slot = item % kItems;
+      const Segment g = it.next();
+      if (g.n_tiles > 0) find_pages(g, 0);
       ok = warp_wait<true>(item_empty + slot, ((item / kItems) & 1) ^ 1u, abort_flag, p.wait_limit_cycles);
       if (!ok) break;
       if (g.n_tiles > 0) {
         const uint32_t s_q = smem_u32(smem + L::kOffQ + slot * L::kQBytes);
         constexpr int kChunks = D / 8;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < kRows * kChunks / 32; ++i) {
           const int r = (i * 32 + lane) / kChunks, c = lane % kChunks;
           int token = 0, head = 0;
-          const bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, kRows, r, &token, &head);
+          const bool live = row_at(p, g.q0, g.n_q, g.head0, g.row0, kRows, r, &token, &head);
           const T* src = static_cast<const T*>(p.q) + (live ? token * p.q_stride_t + head * p.q_stride_h + c * 8 : 0);
           cp_async16(s_q + r * (D * 2) + ((c & ~7) << 4) + (((c ^ r) & 7) << 4), src, live);
         }
@@ -172,32 +167,26 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       cp_async_arrive(item_full + slot);
       if (lane == 0) mbar_arrive(item_full + slot);
       if (g.n_tiles == 0) break;
-      const Segment now = g;
 #pragma unroll 1
-      for (int j = 0; j < now.n_tiles; ++j, ++tiles) {
+      for (int j = 0; j < g.n_tiles; ++j, ++tiles) {
         const int stage = tiles % kStages;
         ok = warp_wait<true>(empty + stage, ((tiles / kStages) & 1) ^ 1u, abort_flag, p.wait_limit_cycles);
         if (!ok) break;
         uint8_t* dst = smem + stage * L::kStage;
         const int checked = checked_page(p, pages);
         if (leader) mbar_arrive_expect_tx(full + stage, boxes * box_rows * D * 2 * 2);
+#pragma unroll 1
         for (int x = 0; x < boxes; ++x) {
           const int page = __shfl_sync(0xffffffffu, checked, x);
           if (leader) {
 #pragma unroll
             for (int c = 0; c < kSlabs; ++c) {
-              tma_load_4d(dst + c * L::kSlab + x * box_rows * 128, &tm_k, full + stage, c * 64, first & slot_mask, now.kv_head, page);
-              tma_load_4d(dst + (kSlabs + c) * L::kSlab + x * box_rows * 128, &tm_v, full + stage, c * 64, first & slot_mask, now.kv_head, page);
+              tma_load_4d(dst + c * L::kSlab + x * box_rows * 128, &tm_k, full + stage, c * 64, first & slot_mask, g.kv_head, page);
+              tma_load_4d(dst + (kSlabs + c) * L::kSlab + x * box_rows * 128, &tm_v, full + stage, c * 64, first & slot_mask, g.kv_head, page);
             }
           }
         }
-        // the pages of the next tile arrive while its stage is waited for
-        if (j + 1 < now.n_tiles) {
-          find_pages(now, j + 1);
-        } else {
-          g = it.next();
-          if (g.n_tiles > 0) find_pages(g, 0);
-        }
+        if (j + 1 < g.n_tiles) find_pages(g, j + 1);  // (they arrive while the stage is waited for)
       }
     }
     if (!ok) {
@@ -242,7 +231,7 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         int token, head, lim = 0;
-        bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, kRows, mt * 16 + half * 8 + lane / 4, &token, &head);
+        bool live = row_at(p, g.q0, g.n_q, g.head0, g.row0, kRows, mt * 16 + half * 8 + lane / 4, &token, &head);
         if (live) {
           if (p.shared_pass) {
             int q1;
@@ -429,18 +418,21 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     if (g.slot == 1 && threadIdx.x == 0) {
       p.headers[blockIdx.x] = PartHeader{g.n_parts, g.q0, g.n_q, g.head0, g.row0, kRows, {0, 0}};
     }
-#pragma unroll
-    for (int pass = 0; pass < 2 * MT; ++pass) {       // rows 8 * pass to 8 * pass + 7
-      if (pass * 8 >= live_rows) break;
+#pragma unroll 1
+    for (int pass = 0; pass * 8 < live_rows; ++pass) {          // rows 8 * pass to 8 * pass + 7
       if (pass > 0 && !warps_sync()) break;           // the buffer has been read
       float* dst = s_join + (warp * 8 + lane / 4) * L::kJoinStride + (lane % 4) * 2;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
-        const float* x = &o[pass / 2][n][2 * (pass % 2)];
-        *reinterpret_cast<float2*>(dst + n * 8) = make_float2(x[0], x[1]);
+        float2 x = make_float2(o[0][n][0], o[0][n][1]);
+#pragma unroll
+        for (int i = 1; i < 2 * MT; ++i) {
+          if (pass == i) x = make_float2(o[i / 2][n][2 * (i % 2)], o[i / 2][n][2 * (i % 2) + 1]);
+        }
+        *reinterpret_cast<float2*>(dst + n * 8) = x;
       }
       if (!warps_sync()) break;
-#pragma unroll
+#pragma unroll 1
       for (int i = threadIdx.x; i < 8 * D / 4; i += 128) {
         const int r8 = i / (D / 4), r = pass * 8 + r8, col = (i - r8 * (D / 4)) * 4;
         if (r >= live_rows) break;
@@ -455,7 +447,7 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           out[0] += f * y.x; out[1] += f * y.y; out[2] += f * y.z; out[3] += f * y.w;
           sum += f * s_l[w * kRows + r];
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
 #pragma unroll
         for (int c = 0; c < 4; ++c) out[c] *= inv;
         if (g.slot >= 0) {
@@ -464,7 +456,7 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           if (col == 0) p.part_e[at] = part_lse(top - kBias, sum);
         } else {
           int token, head;
-          bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0, kRows, r, &token, &head);
+          bool live = row_at(p, g.q0, g.n_q, g.head0, g.row0, kRows, r, &token, &head);
           if (live && p.shared_pass) {
             int q1;
             live = seq_of_token(p, token, &q1) < p.batch.B;

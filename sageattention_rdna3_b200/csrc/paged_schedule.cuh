@@ -16,6 +16,30 @@ namespace paged {
 
 constexpr int kTileKeys = 128;
 
+// Division of numbers below 2^31 by a constant that the host knows: a multiplication and a shift.
+struct FastDiv {
+  uint32_t mul;                 // 0: the divisor is 1
+  int shift;
+  __host__ static FastDiv of(int d) {
+    FastDiv f{0, 0};
+    int s = 0;
+    while ((2 << s) <= d) ++s;                        // 2^s <= d < 2^(s+1)
+    if ((1 << s) == d) {
+      if (s > 0) f = FastDiv{0x80000000u, s - 1};
+    } else {
+      f = FastDiv{static_cast<uint32_t>(((1ull << (32 + s)) + d - 1) / d), s};
+    }
+    return f;
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return mul == 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), mul) >> shift);
+  }
+};
+
+// (Small code matters here: a kernel of this file runs for tens of microseconds, and its instructions come from the L2 or
+// from memory at first.  What is called once an item stands once, in loops that are not unrolled.)
+__device__ __noinline__ long long floor_div(long long a, long long b) { return a / b; }
+
 struct AttnParams {
   const void* q;
   long long q_stride_t, q_stride_h;
@@ -33,6 +57,7 @@ struct AttnParams {
   int shared_pass;              // 1: one sequence of all T tokens against the shared keys; 0: every sequence against its keys behind them
   int Hq, Hkv, group;           // group = Hq / Hkv
   int tile_rows;                // rows of a row tile
+  FastDiv by_group, by_tile_rows;
   int item_cost;                // steps that stand for the start and end of an item
   int causal;
   int zero_rest;                // write zeros to rows that belong to no sequence
@@ -80,7 +105,7 @@ __device__ __forceinline__ Seq seq_at(const AttnParams& p, int b) {
     s.key0 = p.shared_len;
     s.len = clipped_len(p, b);
   }
-  s.row_tiles = static_cast<int>((static_cast<long long>(s.n_q) * p.group + p.tile_rows - 1) / p.tile_rows);
+  s.row_tiles = p.by_tile_rows(s.n_q * p.group + p.tile_rows - 1);
   s.key_tiles = max(1, (s.len - s.key0 + kTileKeys - 1) / kTileKeys);
   return s;
 }
@@ -101,6 +126,7 @@ __device__ __forceinline__ int seq_of_token(const AttnParams& p, int token, int*
     return token;
   }
   int lo = 0, hi = p.batch.B;
+#pragma unroll 1
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (p.batch.cu_q[mid] <= token) lo = mid;
@@ -114,7 +140,8 @@ __device__ __forceinline__ int seq_of_token(const AttnParams& p, int token, int*
 // The span of a CTA and where it starts; found once by all threads together.
 struct Span {
   long long t, t_end;           // steps
-  long long total;
+  long long share;              // CTA c owns share steps, the first `extra` one more
+  int extra;
   int ctas;                     // CTAs that have steps at all
   int b;                        // sequence of step t ...
   long long before;             // ... and the steps before that sequence
@@ -127,6 +154,7 @@ __device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratc
   const int per = (n + kThreads - 1) / kThreads;
   const int first = threadIdx.x * per, last = min(first + per, n);
   long long mine = 0;
+#pragma unroll 1
   for (int b = first; b < last; ++b) {
     mine += steps_of(p, seq_at(p, b));
     if (blockIdx.x == 0 && !p.shared_pass && p.batch.kv_lens[b] > clipped_len(p, b)) p.status.report(kStatusBadLength);
@@ -148,15 +176,18 @@ __device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratc
   }
   upto += base;
   Span s;
-  s.total = total;
   s.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-  const bool idle = static_cast<int>(blockIdx.x) >= s.ctas;
-  s.t = idle ? 0 : total * blockIdx.x / s.ctas;
-  s.t_end = idle ? 0 : total * (blockIdx.x + 1) / s.ctas;
+  const int c = blockIdx.x;
+  const bool idle = c >= s.ctas;
+  s.share = total < 0x7fffffffLL ? static_cast<int>(total) / max(s.ctas, 1) : floor_div(total, s.ctas);
+  s.extra = static_cast<int>(total - s.share * s.ctas);
+  s.t = idle ? 0 : s.share * c + min(c, s.extra);
+  s.t_end = idle ? 0 : s.t + s.share + (c < s.extra ? 1 : 0);
   // The thread whose sequences hold step t walks through them.
   if (!idle && s.t >= upto - mine && s.t < upto) {
     long long before = upto - mine;
     int b = first;
+#pragma unroll 1
     while (true) {
       const long long steps = steps_of(p, seq_at(p, b));
       if (s.t < before + steps) break;
@@ -208,20 +239,23 @@ struct SegmentIter {
     seq.key_tiles = __shfl_sync(0xffffffffu, mine.key_tiles, from);
     steps = steps_of(p, seq);
   }
-  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span), base(-32) {
-    if (s.t < s.t_end) find(s.b);
-  }
+  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span), base(-32), steps(-1) {}
   __device__ __forceinline__ Segment next() {
     Segment g;
     g.n_tiles = 0;
+#pragma unroll 1
     while (s.t < s.t_end && g.n_tiles == 0) {
-      while (s.t >= s.before + steps) {               // (sequences without new tokens have no steps)
-        s.before += steps;
-        find(++s.b);
+#pragma unroll 1
+      while (steps < 0 || s.t >= s.before + steps) {  // (sequences without new tokens have no steps)
+        if (steps >= 0) {
+          s.before += steps;
+          ++s.b;
+        }
+        find(s.b);
       }
       const int item_steps = seq.key_tiles + p.item_cost;
       const long long r = s.t - s.before;
-      const int item = static_cast<int>(r / item_steps);
+      const int item = r < 0x7fffffffLL ? static_cast<int>(r) / item_steps : static_cast<int>(floor_div(r, item_steps));
       const int at = static_cast<int>(r - static_cast<long long>(item) * item_steps);
       const int count = static_cast<int>(min(static_cast<long long>(item_steps - at), s.t_end - s.t));
       const int tile = max(at - p.item_cost, 0);
@@ -231,7 +265,7 @@ struct SegmentIter {
       g.n_q = seq.n_q;
       g.len = seq.len;
       g.key0 = seq.key0 + tile * kTileKeys;
-      g.kv_head = item / seq.row_tiles;
+      g.kv_head = seq.row_tiles == 1 ? item : item / seq.row_tiles;
       g.head0 = g.kv_head * p.group;
       g.row0 = (item - g.kv_head * seq.row_tiles) * p.tile_rows;
       g.b = s.b;
@@ -242,9 +276,9 @@ struct SegmentIter {
         g.slot = -1;
       } else {
         g.slot = 1;
-        // the CTA that owns the last step e of the item: the largest c with total * c / ctas <= e
-        const long long e = s.t + item_steps - at - 1;
-        const long long c = ((e + 1) * s.ctas - 1) / s.total;
+        // the CTA that owns the last step of the item
+        const long long e = s.t + item_steps - at - 1, longer = s.extra * (s.share + 1);
+        const long long c = e < longer ? floor_div(e, s.share + 1) : s.extra + floor_div(e - longer, s.share);
         g.n_parts = static_cast<int>(c) - static_cast<int>(blockIdx.x) + 1;
       }
       s.t += count;
@@ -254,12 +288,12 @@ struct SegmentIter {
 };
 
 // Row r of a tile -> new token (counted in the batch) and query head; false if the row is empty.
-__device__ __forceinline__ bool row_at(int token0, int tokens, int head0, int group, int row0, int rows, int r, int* token, int* head) {
+__device__ __forceinline__ bool row_at(const AttnParams& p, int token0, int tokens, int head0, int row0, int rows, int r, int* token, int* head) {
   if (r >= rows) return false;
   const int flat = row0 + r;
-  const int i = flat / group;
+  const int i = p.by_group(flat);
   *token = token0 + i;
-  *head = head0 + flat - i * group;
+  *head = head0 + flat - i * p.group;
   return i < tokens;
 }
 
@@ -278,10 +312,10 @@ __device__ __forceinline__ void join_weights(float e, float prior, float* w, flo
     *joined = -INFINITY;
     return;
   }
-  const float a = exp2f(e - top), b = exp2f(prior - top), sum = a + b;
-  *w = a / sum;
-  *w_prior = b / sum;
-  *joined = top + log2f(sum);
+  const float a = ex2(e - top), b = ex2(prior - top), inv = __fdividef(1.0f, a + b);
+  *w = a * inv;
+  *w_prior = b * inv;
+  *joined = top + log2f(a + b);
 }
 
 template <int N>
@@ -347,8 +381,10 @@ __device__ __forceinline__ void zero_rest(const AttnParams& p, int D, int thread
   const int first = min(max(p.batch.cu_q[0], 0), p.batch.T), last = min(max(p.batch.cu_q[p.batch.B], 0), p.batch.T);
   const int rest = first + p.batch.T - last;
   const int vecs = p.Hq * (D / 8);
+#pragma unroll 1
   for (int i = blockIdx.x; i < rest; i += gridDim.x) {
     const int token = i < first ? i : last + i - first;
+#pragma unroll 1
     for (int v = thread; v < vecs; v += threads) {
       const int head = v / (D / 8);
       *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + token * p.o_stride_t + head * p.o_stride_h + (v - head * (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
@@ -377,21 +413,21 @@ struct PartSum {
 #pragma unroll
     for (int c = 0; c < 4; ++c) top = fmaxf(top, pe[c]);
     if (top == -INFINITY) return;                     // no visible keys so far
-    const float back = exp2f(e - top);
+    const float back = ex2(e - top);
     sum *= back;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] *= back;
     e = top;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float f = exp2f(pe[c] - top);
+      const float f = ex2(pe[c] - top);
       sum += f;
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] += f * px[c][i];
     }
   }
   __device__ __forceinline__ void normalise() {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] *= inv;
   }
@@ -400,7 +436,7 @@ struct PartSum {
 
 // The row of a merge thread, if it has one that belongs to a sequence.
 __device__ __forceinline__ bool merge_row(const AttnParams& p, const PartHeader& h, int r, int* token, int* head) {
-  if (!row_at(h.token0, h.tokens, h.head0, p.group, h.row0, h.rows, r, token, head)) return false;
+  if (!row_at(p, h.token0, h.tokens, h.head0, h.row0, h.rows, r, token, head)) return false;
   int q1;
   return !p.shared_pass || seq_of_token(p, *token, &q1) < p.batch.B;
 }
@@ -420,6 +456,7 @@ __global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_rows_kernel(co
   const bool live = merge_row(p, h, r, &token, &head);
   PartSum<kPer> acc;
   if (live) {
+#pragma unroll 1
     for (int k0 = w; k0 < h.n_parts; k0 += 4 * kRowWarps) {
       float pe[4], px[4][kPer];
 #pragma unroll
@@ -471,6 +508,7 @@ __global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_columns_kernel
   int token = 0, head = 0;
   if (!merge_row(p, h, r, &token, &head)) return;
   PartSum<4 * kVecs> acc;
+#pragma unroll 1
   for (int k0 = 0; k0 < h.n_parts; k0 += 4) {
     float pe[4], px[4][4 * kVecs];
 #pragma unroll

@@ -4,19 +4,19 @@
 // row and key against 4 D bytes per key), so they go to the tensor cores through tcgen05.  A CTA owns two tiles of up to 128 rows, the
 // query heads of a GQA group for 128 / group new tokens each (one TMA box), and streams 128-key tiles past both:
 //   warp 8     TMA producer  Q; K and V tiles page by page (a box per page, or per 128 keys of a larger page), two stages
-//   warp 9+q   MMA issuer    S_q = Q_q.K^T, O_q += P_q.V in halves of 64 keys, fp32 accumulators in TMEM
+//   warp 9+q   MMA issuer    S_q = Q_q.K^T, O_q += P_q.V, fp32 accumulators in TMEM
 //   warps 4q.. softmax of tile q: thread t owns row t, running maximum and sum in fp32, P back into TMEM over S
-// While a tile's rows are at the exponentials of one half the tensor cores work on its other half, and for the other tile
-// (D=128: 1024 clocks of products and 1024 of the exponential units per tile); each tile has an issuer of its own, or one would wait for the
-// other's rows.  Two row tiles to a key tile also halve what is fetched through the L2.  A second tile without rows (fewer
-// than 128 rows in all) is left out.
+// While one tile's rows are at their exponentials the tensor cores work for the other (D=128: 1024 clocks of products and 1024 of
+// the exponential units per tile); each tile has an issuer of its own, or one would wait for the other's rows.  Two row
+// tiles to a key tile also halve what is fetched through the L2.  A second tile without rows (fewer than 128 rows in all)
+// is left out.
 // The grid is a persistent CTA per SM over equal spans of key tiles (paged_schedule.cuh); loads and the first Q.K^T of the next item
 // run under the end of this one.  TMEM columns: [128 q, 128 q + 128) S_q, in place P_q (16-bit pairs); [256 + D q, ..) O_q.
 //
 // Masks: a row sees the keys below its limit.  Behind the last key of a sequence pages hold anything; the softmax warps
 // write zeros over those rows of V before the product reads them (0 * NaN is NaN), and pages behind it are not
 // loaded at all.  Weights are 2^(s - m + 7): an optimistic pass takes them against the maximum so far, which moves only when
-// 64 of them add up to more than 2^15, and for fp16 the smallest numbers (2^-24) are 2^-31 of the largest weight.
+// 128 of them add up to more than 2^15, and for fp16 the smallest numbers (2^-24) are 2^-31 of the largest weight.
 // P is rounded to the type of V; the sum is taken before that.
 #pragma once
 
@@ -28,13 +28,12 @@ namespace paged {
 constexpr int kTileThreads = 384;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kTileM = 128;
-constexpr int kHalfKeys = 64;
 constexpr int kTileTmemCols = 512;
 constexpr int kColO = 256;
 constexpr float kTileBias = 7.0f;                     // log2 of the largest weight while the maximum stands still
 constexpr float kTileLazy = 8.0f;                     // growth of the maximum that is let pass: weights up to 2^15
 constexpr float kTileSumMax = 32768.0f;
-constexpr float kTileRefusedLazy = 2.0f;              // 64 weights add up to more than 2^15: one is above 2^9
+constexpr float kTileRefusedLazy = 1.0f;              // 128 weights add up to more than 2^15: one is above 2^8
 
 template <int D>
 struct TileSmem {
@@ -47,7 +46,7 @@ struct TileSmem {
   static constexpr int kOffV = kOffK + kStages * kKVBytes;
   static constexpr int kOffBar = kOffV + kStages * kKVBytes;
   static constexpr int kItems = 2;                    // items ahead
-  static constexpr int kNumBars = 18 + 4 * kStages + 2 * kItems;
+  static constexpr int kNumBars = 10 + 4 * kStages + 2 * kItems;
   static constexpr int kOffSegments = kOffBar + 8 * kNumBars;
   static constexpr int kOffScratch = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
   static constexpr int kOffMisc = kOffScratch + 8 * (kTileThreads / 32 + 4);
@@ -74,16 +73,15 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   uint64_t* q_full = bars + 0;
   uint64_t* q_empty = bars + 1;     // every Q.K^T of the item is complete
   uint64_t* o_final = bars + 2;     // [2] every P.V of the item's row tile is complete
-  uint64_t* o_free = bars + 4;      // [2] all 128 threads of the tile hold its O in registers
-  uint64_t* s_full = bars + 6;      // [2][2] half h of S_q holds Q_q.K_h^T
-  uint64_t* p_full = bars + 10;     // [2][2] half h of P_q is written (and O_q scaled) by all 128 threads of the tile
-  uint64_t* pv_done = bars + 14;    // [2][2] O_q += P_q.V over half h is complete
-  uint64_t* k_full = bars + 18;
-  uint64_t* v_full = bars + 18 + kStages;
-  uint64_t* k_empty = bars + 18 + 2 * kStages;      // (by both issuers)
-  uint64_t* v_empty = bars + 18 + 3 * kStages;
-  uint64_t* item_full = bars + 18 + 4 * kStages;               // [kItems] the segment is written
-  uint64_t* item_empty = bars + 18 + 4 * kStages + L::kItems;  // ... and read by the issuers and the eight softmax warps
+  uint64_t* o_free = bars + 4;      // [2] all four warps of the tile hold its O in registers
+  uint64_t* s_full = bars + 6;      // [2] S_q holds Q_q.K^T, and every P.V before it is complete
+  uint64_t* p_full = bars + 8;      // [2] P_q is written (and O_q scaled) by all four warps of the tile
+  uint64_t* k_full = bars + 10;
+  uint64_t* v_full = bars + 10 + kStages;
+  uint64_t* k_empty = bars + 10 + 2 * kStages;      // (by both issuers)
+  uint64_t* v_empty = bars + 10 + 3 * kStages;
+  uint64_t* item_full = bars + 10 + 4 * kStages;               // [kItems] the segment is written
+  uint64_t* item_empty = bars + 10 + 4 * kStages + L::kItems;  // ... and read by the issuers and the eight softmax warps
   Segment* segments = reinterpret_cast<Segment*>(smem + L::kOffSegments);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
@@ -95,12 +93,9 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     mbar_init(q_empty, 2);
     for (int q = 0; q < 2; ++q) {
       mbar_init(o_final + q, 1);
-      mbar_init(o_free + q, 128);
-      for (int h = 0; h < 2; ++h) {
-        mbar_init(s_full + 2 * q + h, 1);
-        mbar_init(p_full + 2 * q + h, 128);
-        mbar_init(pv_done + 2 * q + h, 1);
-      }
+      mbar_init(o_free + q, 4);
+      mbar_init(s_full + q, 1);
+      mbar_init(p_full + q, 4);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(k_full + s, 1);
@@ -149,6 +144,76 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     action;                                                                         \
   }
 
+  // ------------------------------------------------------------------ MMA issuers
+  // Each for its row tile: QK(0) | PV(0) QK(1) | PV(1) QK(2) | ...  The tile is a constant of the code: the operands of tensor
+  // instructions are uniform registers, and addresses that depend on the thread's warp number would be moved there one by one.
+  auto issue_products = [&](auto tile_tag) {
+    constexpr int q = decltype(tile_tag)::value;
+    constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+    constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kTileKeys);
+    constexpr uint32_t kIdescPV = umma_idesc(1, kFmt, kFmt, 0, 1, kTileM, D);              // V MN-major
+    const uint32_t t_s = tmem_base + q * kTileKeys, t_o = tmem_base + kColO + q * D;
+    int kt = 0, qt = 0, live_items = 0;             // key tiles so far, those of this row tile, items in which it had rows
+    bool ok = true;
+    auto issue_qk = [&](int stage) {
+      // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t slab = (k / 4) * L::kSlab;
+        const uint64_t dq = umma_smem_desc(smem_u32(s_q + q * L::kQBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+        const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+        mma_f16_ss(t_s, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
+      }
+      tc_commit(s_full + q);
+      tc_commit(k_empty + stage);
+    };
+#pragma unroll 1
+    for (int items = 0; ok; ++items) {
+      SAGE_PAGED_WAIT_OR(false, item_full + items % L::kItems, (items / L::kItems) & 1, 34, { ok = false; break; });
+      const int n_tiles = segments[items % L::kItems].n_tiles;
+      const bool idle = q >= n_row_tiles(p, segments[items % L::kItems]);
+      mbar_arrive(item_empty + items % L::kItems);
+      if (n_tiles == 0) break;
+      SAGE_PAGED_WAIT_OR(false, q_full, items & 1, 24, { ok = false; break; });
+      if (idle) {                                   // lets every stage go as it comes: phases are counted by all
+        for (int j = 0; ok && j < n_tiles; ++j, ++kt) {
+          const int s = kt % kStages;
+          SAGE_PAGED_WAIT_OR(false, k_full + s, (kt / kStages) & 1, 25, { ok = false; break; });
+          mbar_arrive(k_empty + s);
+          SAGE_PAGED_WAIT_OR(false, v_full + s, (kt / kStages) & 1, 27, { ok = false; break; });
+          mbar_arrive(v_empty + s);
+        }
+        mbar_arrive(q_empty);
+        continue;
+      }
+      SAGE_PAGED_WAIT_OR(false, k_full + kt % kStages, (kt / kStages) & 1, 25, { ok = false; break; });
+      tc_fence_after();
+      issue_qk(kt % kStages);
+      if (n_tiles == 1) tc_commit(q_empty);
+      // the first P.V of an item overwrites O: the O of the item before must have been read
+      if (live_items > 0) SAGE_PAGED_WAIT_OR(false, o_free + q, (live_items - 1) & 1, 28, { ok = false; break; });
+#pragma unroll 1
+      for (int j = 0; j < n_tiles; ++j, ++qt) {
+        const int t = kt + j, s = t % kStages, s1 = (t + 1) % kStages;
+        // (the loads first: what follows P is the chain that the softmax waits for)
+        SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
+        if (j + 1 < n_tiles) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
+        SAGE_PAGED_WAIT_OR(false, p_full + q, qt & 1, 26, { ok = false; break; });
+        tc_fence_after();
+        // V: [128 keys][64 values] slabs; an instruction takes 16 rows = 2048 bytes
+        const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes), L::kSlab, 1024, kSwizzle128B);
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k) mma_f16_ts(t_o, t_s + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || k > 0) ? 1u : 0u);
+        if (j + 1 < n_tiles) issue_qk(s1);
+        else tc_commit(o_final + q);
+        tc_commit(v_empty + s);
+        if (j + 2 == n_tiles) tc_commit(q_empty);
+      }
+      ++live_items;
+      kt += n_tiles;
+    }
+  };
+
   if (dead_on_arrival) {
     // nothing to do
   } else if (warp == 8) {
@@ -168,6 +233,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     };
     auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int head) {
       if (leader) mbar_arrive_expect_tx(bar, boxes * box_rows * D * 2);
+#pragma unroll 1
       for (int i = 0; i < boxes; ++i) {
         const int id = __shfl_sync(0xffffffffu, pages, i);
         if (leader) {
@@ -176,11 +242,11 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
     };
-    Segment g = it.next();
-    if (g.n_tiles > 0) find_pages(g, 0);
 #pragma unroll 1
     for (int items = 0; ok; ++items) {
       const int slot = items % L::kItems;
+      const Segment g = it.next();
+      if (g.n_tiles > 0) find_pages(g, 0);
       SAGE_PAGED_WARP_WAIT_OR(true, item_empty + slot, ((items / L::kItems) & 1) ^ 1u, 20, { ok = false; break; });
       if (lane == 0) {
         segments[slot] = g;
@@ -192,116 +258,34 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (leader) {
         const int tiles = n_row_tiles(p, g), half_rows = p.tile_rows / 2;
         mbar_arrive_expect_tx(q_full, tiles * half_rows * D * 2);
+#pragma unroll 1
         for (int q = 0; q < tiles; ++q) {
 #pragma unroll
           for (int c = 0; c < kSlabs; ++c)
-            tma_load_3d(s_q + q * L::kQBytes + c * L::kSlab, &tm_q, q_full, c * 64, g.head0, g.q0 + (g.row0 + q * half_rows) / p.group);
+            tma_load_3d(s_q + q * L::kQBytes + c * L::kSlab, &tm_q, q_full, c * 64, g.head0, g.q0 + p.by_group(g.row0 + q * half_rows));
         }
       }
       __syncwarp();
-      const Segment now = g;
 #pragma unroll 1
-      for (int j = 0; j < now.n_tiles; ++j, ++kt) {
+      for (int j = 0; j < g.n_tiles; ++j, ++kt) {
         const int s = kt % kStages;
         SAGE_PAGED_WARP_WAIT_OR(true, k_empty + s, ((kt / kStages) & 1) ^ 1u, 23, { ok = false; break; });
         pages = checked_page(p, pages);
-        load(&tm_k, s_k + s * L::kKVBytes, k_full + s, now.kv_head);
+        load(&tm_k, s_k + s * L::kKVBytes, k_full + s, g.kv_head);
         SAGE_PAGED_WARP_WAIT_OR(true, v_empty + s, ((kt / kStages) & 1) ^ 1u, 21, { ok = false; break; });
-        load(&tm_v, s_v + s * L::kKVBytes, v_full + s, now.kv_head);
-        // the pages of the next tile arrive while its stage is waited for
-        if (j + 1 < now.n_tiles) {
-          find_pages(now, j + 1);
-        } else {
-          g = it.next();
-          if (g.n_tiles > 0) find_pages(g, 0);
-        }
+        load(&tm_v, s_v + s * L::kKVBytes, v_full + s, g.kv_head);
+        if (j + 1 < g.n_tiles) find_pages(g, j + 1);  // (they arrive while the stage is waited for)
       }
     }
     __syncwarp();
-  } else if (warp < kSoftmaxWarps + 4 && warp > kSoftmaxWarps) {
-    // ------------------------------------------------------------------ MMA issuers
-    // Each for its row tile: QK(0,0) QK(0,1) | PV(0,0) QK(1,0) PV(0,1) QK(1,1) | ...
-    const int q = warp - kSoftmaxWarps - 1;
-    if (q < 2 && elect_one()) {
-      constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
-      constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kHalfKeys);
-      constexpr uint32_t kIdescPV = umma_idesc(1, kFmt, kFmt, 0, 1, kTileM, D);              // V MN-major
-      const uint32_t t_s = tmem_base + q * kTileKeys, t_o = tmem_base + kColO + q * D;
-      int kt = 0, qt = 0, live_items = 0;             // key tiles so far, those of this row tile, items in which it had rows
-      bool ok = true;
-      auto issue_qk = [&](int stage, int h) {
-        // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes, half h of K starts
-        // 64 rows into each slab
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t slab = (k / 4) * L::kSlab;
-          const uint64_t dq = umma_smem_desc(smem_u32(s_q + q * L::kQBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-          const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab + h * (kHalfKeys * 128)), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-          mma_f16_ss(t_s + h * kHalfKeys, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
-        }
-        tc_commit(s_full + 2 * q + h);
-      };
-#pragma unroll 1
-      for (int items = 0; ok; ++items) {
-        SAGE_PAGED_WAIT_OR(false, item_full + items % L::kItems, (items / L::kItems) & 1, 34, { ok = false; break; });
-        const int n_tiles = segments[items % L::kItems].n_tiles;
-        const bool idle = q >= n_row_tiles(p, segments[items % L::kItems]);
-        mbar_arrive(item_empty + items % L::kItems);
-        if (n_tiles == 0) break;
-        SAGE_PAGED_WAIT_OR(false, q_full, items & 1, 24, { ok = false; break; });
-        if (idle) {                                   // lets every stage go as it comes: phases are counted by all
-          for (int j = 0; ok && j < n_tiles; ++j, ++kt) {
-            const int s = kt % kStages;
-            SAGE_PAGED_WAIT_OR(false, k_full + s, (kt / kStages) & 1, 25, { ok = false; break; });
-            mbar_arrive(k_empty + s);
-            SAGE_PAGED_WAIT_OR(false, v_full + s, (kt / kStages) & 1, 27, { ok = false; break; });
-            mbar_arrive(v_empty + s);
-          }
-          mbar_arrive(q_empty);
-          continue;
-        }
-        SAGE_PAGED_WAIT_OR(false, k_full + kt % kStages, (kt / kStages) & 1, 25, { ok = false; break; });
-        tc_fence_after();
-        issue_qk(kt % kStages, 0);
-        issue_qk(kt % kStages, 1);
-        tc_commit(k_empty + kt % kStages);
-        if (n_tiles == 1) tc_commit(q_empty);
-#pragma unroll 1
-        for (int j = 0; ok && j < n_tiles; ++j) {
-          const int t = kt + j, s = t % kStages, s1 = (t + 1) % kStages;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            SAGE_PAGED_WAIT_OR(false, p_full + 2 * q + h, qt & 1, 26, { ok = false; break; });
-            if (h == 0) SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
-            // the first P.V of an item overwrites O: the O of the item before must have been read
-            if (j == 0 && h == 0 && live_items > 0) SAGE_PAGED_WAIT_OR(false, o_free + q, (live_items - 1) & 1, 28, { ok = false; break; });
-            tc_fence_after();
-            // V: [128 keys][64 values] slabs; half h starts 64 rows = 8192 bytes in, an instruction takes 16 rows = 2048 bytes
-            const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes + h * (kHalfKeys * 128)), L::kSlab, 1024, kSwizzle128B);
-#pragma unroll
-            for (int k = 0; k < kHalfKeys / 16; ++k) {
-              mma_f16_ts(t_o, t_s + h * kHalfKeys + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || h > 0 || k > 0) ? 1u : 0u);
-            }
-            tc_commit(pv_done + 2 * q + h);
-            if (h == 1) tc_commit(v_empty + s);
-            if (j + 1 < n_tiles) {
-              if (h == 0) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
-              tc_fence_after();
-              issue_qk(s1, h);
-              if (h == 1) {
-                tc_commit(k_empty + s1);
-                if (j + 2 == n_tiles) tc_commit(q_empty);
-              }
-            }
-          }
-          ++qt;
-        }
-        tc_commit(o_final + q);
-        ++live_items;
-        kt += n_tiles;
-      }
-    }
+  } else if (warp == kSoftmaxWarps + 1) {
+    if (elect_one()) issue_products(std::integral_constant<int, 0>{});
     __syncwarp();
+  } else if (warp == kSoftmaxWarps + 2) {
+    if (elect_one()) issue_products(std::integral_constant<int, 1>{});
+    __syncwarp();
+  } else if (warp == kSoftmaxWarps + 3) {
+    // (a warpgroup has four)
   } else {
     // ------------------------------------------------------------------ softmax and output
     const int q = warp >> 2;                          // row tile of this warp
@@ -323,7 +307,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       const int half_rows = p.tile_rows / 2;
       int token = 0, head = 0, limit = 0;
-      bool live = row_at(g.q0, g.n_q, g.head0, p.group, g.row0 + q * half_rows, half_rows, row, &token, &head);
+      bool live = row_at(p, g.q0, g.n_q, g.head0, g.row0 + q * half_rows, half_rows, row, &token, &head);
       if (live) {
         if (p.shared_pass) {
           int q1;
@@ -335,84 +319,94 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
       const bool warp_live = __any_sync(0xffffffffu, live);
+      const int warp_limit = __reduce_min_sync(0xffffffffu, live ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.0f;
       int distrust = 0;                               // > 1: the optimistic pass is skipped
+      bool settled = false;                           // every row of the warp has a maximum
+      const f32x2_t scale2 = pack2(p.score_scale, p.score_scale);
 #pragma unroll 1
-      for (int hh = 0; hh < 2 * g.n_tiles; ++hh) {
-        const int t = kt + (hh >> 1), tq = qt + (hh >> 1), h = hh & 1;
-        const int first = g.key0 + hh * kHalfKeys;
-        SAGE_PAGED_WARP_WAIT_OR(false, s_full + 2 * q + h, tq & 1, 31, { ok = false; break; });
+      for (int j = 0; j < g.n_tiles; ++j) {
+        const int t = kt + j, first = g.key0 + j * kTileKeys;
+        SAGE_PAGED_WARP_WAIT_OR(false, s_full + q, (qt + j) & 1, 31, { ok = false; break; });
         tc_fence_after();
-        if (h == 0 && first + kTileKeys > g.len) {
-          // The last tile: zeros over what is no value of the sequence, by both row tiles, either of which may be first.  (Behind the wait for S, which says that the stage's
-          // load before this one has long been used: a parity cannot tell phases apart that are two turns away.)
+        if (first + kTileKeys > g.len) {
+          // The last tile: zeros over what is no value of the sequence, by both row tiles, either of which may be first.  (Behind
+          // the wait for S, which says that the stage's load before this one has long been used: a parity cannot tell
+          // phases apart that are two turns away.)
           const int stage = t % kStages;
           SAGE_PAGED_WARP_WAIT_OR(false, v_full + stage, (t / kStages) & 1, 30, { ok = false; break; });
           const int keys = max(g.len - first, 0);
+#pragma unroll 1
           for (int i = threadIdx.x & 127; i < (kTileKeys - keys) * kSlabs * 8; i += 128) {
-            const int row = keys + i / (kSlabs * 8), x = i % (kSlabs * 8);
-            *reinterpret_cast<uint4*>(s_v + stage * L::kKVBytes + (x >> 3) * L::kSlab + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+            const int r = keys + i / (kSlabs * 8), x = i % (kSlabs * 8);
+            *reinterpret_cast<uint4*>(s_v + stage * L::kKVBytes + (x >> 3) * L::kSlab + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();                   // the tensor cores read it through the async proxy
         }
         if (warp_live) {
-          uint32_t sr[2][32];
-          tmem_ld32(t_s + h * kHalfKeys, sr[0]);
-          tmem_ld32(t_s + h * kHalfKeys + 32, sr[1]);
-          tc_wait_ld();
-          const int col_end = live ? limit - first : kHalfKeys;      // columns below it are visible
-          const bool masked = __any_sync(0xffffffffu, col_end < kHalfKeys);
-          uint32_t pk[32];
-          const f32x2_t scale2 = pack2(p.score_scale, p.score_scale);
-          auto exp_pass = [&](auto masked_tag, float base) -> float {
-            constexpr bool kMasked = decltype(masked_tag)::value;
+          // Weights of 32 columns against `base`, packed; returns their sum.
+          auto weigh = [&](const uint32_t (&sr)[32], float base, auto keep, uint32_t* pk) -> f32x2_t {
             const f32x2_t neg = pack2(kTileBias - base, kTileBias - base);
             f32x2_t acc = pack2(0.0f, 0.0f);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int i = 0; i < 16; ++i) {
+              const float2 x = unpack2(ffma2(pack2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), scale2, neg));
+              float2 w = make_float2(ex2(x.x), ex2(x.y));
+              keep(2 * i, &w.x);
+              keep(2 * i + 1, &w.y);
+              acc = fadd2(acc, pack2(w.x, w.y));
+              pk[i] = from_float2(w.x, w.y, static_cast<const T*>(nullptr));
+            }
+            return acc;
+          };
+          const bool masked = first + kTileKeys > warp_limit;
+          const bool attempt = settled && !masked && distrust < 2;
+          bool done = false;
+          if (attempt) {
+            // P stays in registers until the sum has been looked at: S would be needed again.  The next columns are on
+            // their way while these are worked on.
+            uint32_t sr[2][32], pk[64];
+            f32x2_t acc = pack2(0.0f, 0.0f);
+            tmem_ld32(t_s, sr[0]);
+            tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 x = unpack2(ffma2(pack2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, neg));
-                float2 w = make_float2(ex2(x.x), ex2(x.y));
-                if constexpr (kMasked) {
-                  if (32 * c + 2 * i >= col_end) w.x = 0.0f;
-                  if (32 * c + 2 * i + 1 >= col_end) w.y = 0.0f;
-                }
-                acc = fadd2(acc, pack2(w.x, w.y));
-                pk[16 * c + i] = from_float2(w.x, w.y, static_cast<const T*>(nullptr));
-              }
+            for (int c = 0; c < 4; ++c) {
+              if (c < 3) tmem_ld32(t_s + 32 * (c + 1), sr[(c + 1) & 1]);
+              acc = fadd2(acc, weigh(sr[c & 1], m, [](int, float*) {}, pk + 16 * c));
+              if (c < 3) tc_wait_ld();
             }
             const float2 a = unpack2(acc);
-            return a.x + a.y;
-          };
-          bool done = false;
-          const bool attempt = hh > 0 && !masked && distrust < 2 && !__any_sync(0xffffffffu, m == -INFINITY);
-          if (attempt) {
-            const float sum = exp_pass(std::false_type{}, m);
+            const float sum = a.x + a.y;
             done = !__any_sync(0xffffffffu, !(sum <= kTileSumMax));
-            if (done) l += sum;
+            if (done) {
+              l += sum;
+              tmem_st32(t_s, *reinterpret_cast<const uint32_t(*)[32]>(pk));
+              tmem_st32(t_s + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+            }
             distrust = done ? max(distrust - 1, 0) : min(distrust + 2, 4);
           }
           if (!done) {
+            const int col_end = live ? limit - first : kTileKeys;    // columns below it are visible
             float top = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t sr[32];
+              tmem_ld32(t_s + 32 * c, sr);
+              tc_wait_ld();
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
-                const float x = __uint_as_float(sr[c][i]) * p.score_scale;
+                const float x = __uint_as_float(sr[i]) * p.score_scale;
                 if (32 * c + i < col_end) top = fmaxf(top, x);
               }
+            }
             const bool need = top > m + (attempt ? kTileRefusedLazy : kTileLazy) || (m == -INFINITY && top > m);
             const bool moved = __any_sync(0xffffffffu, need);
-            if (!attempt && hh > 0) distrust = moved ? min(distrust + 1, 4) : max(distrust - 1, 0);
+            if (!attempt && j > 0) distrust = moved ? min(distrust + 1, 4) : max(distrust - 1, 0);
             if (moved) {
-              if (hh > 0) {
-                const int hp = h ^ 1;
-                SAGE_PAGED_WARP_WAIT_OR(false, pv_done + 2 * q + hp, (h ? tq : tq - 1) & 1, 32, { ok = false; break; });
-                tc_fence_after();
+              if (j > 0) {                            // (O is at rest: s_full)
                 const float back = need ? ex2(m - top) : 1.0f;
                 l *= back;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                   uint32_t orr[32];
                   tmem_ld32(t_o + 32 * c, orr);
@@ -424,26 +418,36 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               }
               if (need) m = top;
             }
+            settled = !__any_sync(0xffffffffu, m == -INFINITY);
             const float base = m == -INFINITY ? 0.0f : m;            // (a row that has seen nothing yet)
-            if (masked) l += exp_pass(std::true_type{}, base);
-            else l += exp_pass(std::false_type{}, base);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {             // (P of these columns goes where columns before them were)
+              uint32_t sr[32], pk[16];
+              tmem_ld32(t_s + 32 * c, sr);
+              tc_wait_ld();
+              const float2 a = unpack2(weigh(sr, base, [&](int i, float* w) {
+                if (32 * c + i >= col_end) *w = 0.0f;
+              }, pk));
+              l += a.x + a.y;
+              tmem_st16(t_s + 16 * c, pk);
+            }
           }
-          tmem_st32(t_s + h * kHalfKeys, pk);
           tc_wait_st();
         }
         tc_fence_before();
-        mbar_arrive(p_full + 2 * q + h);
+        __syncwarp();                                 // (an arrival per warp: 128 of them on one word take turns)
+        if (lane == 0) mbar_arrive(p_full + q);
       }
       if (!ok) break;
       SAGE_PAGED_WARP_WAIT_OR(false, o_final + q, live_items & 1, 33, { ok = false; break; });
       tc_fence_after();
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
       if (g.slot == 1 && threadIdx.x == 0) {
         p.headers[blockIdx.x] = PartHeader{g.n_parts, g.q0, g.n_q, g.head0, g.row0, p.tile_rows, {0, 0}};
       }
       const int slot = blockIdx.x * 2 + g.slot, part_row = q * half_rows + row;
       float4* part = reinterpret_cast<float4*>(p.part_o) + static_cast<long long>(slot) * p.tile_rows * (D / 4) + part_row;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t orr[32];
         if (warp_live) {
@@ -452,7 +456,8 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         if (c == D / 32 - 1) {                        // O is in registers: the next item may overwrite it
           tc_fence_before();
-          mbar_arrive(o_free + q);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(o_free + q);
         }
         if (!live) continue;
         float x[32];
