@@ -6,17 +6,18 @@
 //   warp 8     TMA producer  Q; K and V tiles page by page (a box per page, or per 128 keys of a larger page), two stages
 //   warp 9+q   MMA issuer    S_q = Q_q.K^T, O_q += P_q.V, fp32 accumulators in TMEM
 //   warps 4q.. softmax of tile q: thread t owns row t, running maximum and sum in fp32, P back into TMEM over S
-// While one tile's rows are at their exponentials the tensor cores work for the other (D=128: 1024 clocks of products and 1024 of
-// the exponential units per tile); each tile has an issuer of its own, or one would wait for the other's rows.  Two row
-// tiles to a key tile also halve what is fetched through the L2.  A second tile without rows (fewer than 128 rows in all)
-// is left out.
+// Q.K^T of one half of a key tile runs while the softmax is at the other half, and each row tile has an issuer of its own, or one would
+// wait for the other's rows: with Q.K^T of whole key tiles the scores of the next tile came only when P.V was through,
+// and the same work as below took 159 us instead of 133 (though 64 columns are read from shared memory at 3/4 of
+// the tensor cores' rate).  Two row tiles to a key tile also halve what is fetched through the L2.  A second tile without rows (fewer
+// than 128 rows in all) is left out.
 // The grid is a persistent CTA per SM over equal spans of key tiles (paged_schedule.cuh); loads and the first Q.K^T of the next item
 // run under the end of this one.  TMEM columns: [128 q, 128 q + 128) S_q, in place P_q (16-bit pairs); [256 + D q, ..) O_q.
 //
 // Masks: a row sees the keys below its limit.  Behind the last key of a sequence pages hold anything; the softmax warps
 // write zeros over those rows of V before the product reads them (0 * NaN is NaN), and pages behind it are not
 // loaded at all.  Weights are 2^(s - m + 7): an optimistic pass takes them against the maximum so far, which moves only when
-// 128 of them add up to more than 2^15, and for fp16 the smallest numbers (2^-24) are 2^-31 of the largest weight.
+// 64 of them add up to more than 2^15, and for fp16 the smallest numbers (2^-24) are 2^-31 of the largest weight.
 // P is rounded to the type of V; the sum is taken before that.
 #pragma once
 
@@ -28,12 +29,17 @@ namespace paged {
 constexpr int kTileThreads = 384;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kTileM = 128;
+constexpr int kHalfKeys = 64;
 constexpr int kTileTmemCols = 512;
 constexpr int kColO = 256;
 constexpr float kTileBias = 7.0f;                     // log2 of the largest weight while the maximum stands still
 constexpr float kTileLazy = 8.0f;                     // growth of the maximum that is let pass: weights up to 2^15
 constexpr float kTileSumMax = 32768.0f;
-constexpr float kTileRefusedLazy = 1.0f;              // 128 weights add up to more than 2^15: one is above 2^8
+constexpr float kTileRefusedLazy = 2.0f;              // 64 weights add up to more than 2^15: one is above 2^9
+
+// Every fourth pair of weights is computed without the exponential unit (exp2_by_polynomial).  us, 128 rows of 32 heads on 8
+// against 65536 shared keys, D=128 / D=64: none 136 / 120, every eighth 131 / 117, fourth 133 / 113, third 133 / 115.
+constexpr int kHandEvery = 4;
 
 template <int D>
 struct TileSmem {
@@ -46,12 +52,34 @@ struct TileSmem {
   static constexpr int kOffV = kOffK + kStages * kKVBytes;
   static constexpr int kOffBar = kOffV + kStages * kKVBytes;
   static constexpr int kItems = 2;                    // items ahead
-  static constexpr int kNumBars = 10 + 4 * kStages + 2 * kItems;
+  static constexpr int kNumBars = 18 + 4 * kStages + 2 * kItems;
   static constexpr int kOffSegments = kOffBar + 8 * kNumBars;
   static constexpr int kOffScratch = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
   static constexpr int kOffMisc = kOffScratch + 8 * (kTileThreads / 32 + 4);
   static constexpr int kTotal = kOffMisc + 16;
 };
+
+// 2^x for two numbers on the multipliers instead of the exponential unit: x = n + f with f in [-1/2, 1/2] by adding and
+// taking away 1.5 2^23, 2^f by a polynomial of degree 5 (fitted for the smallest largest relative error, 2^-23.7 in exact arithmetic), n
+// into the exponent.  Below 2^-126 it stays there.  `high` collects the largest x: above 16 the result is not to be
+// used.  Not a number comes out as 3.4e38.
+__device__ __forceinline__ float2 exp2_by_polynomial(float x0, float x1, float* high) {
+  *high = fmaxf(*high, fmaxf(x0, x1));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
+  auto both = [](float c) { return pack2(c, c); };
+  const f32x2_t x = pack2(x0, x1);
+  const f32x2_t t = fadd2(x, both(12582912.0f));
+  const f32x2_t f = ffma2(fadd2(t, both(-12582912.0f)), both(-1.0f), x);
+  f32x2_t y = ffma2(f, both(0.001327647191654736f), both(0.009675541333844113f));
+  y = ffma2(f, y, both(0.05550713273732967f));
+  y = ffma2(f, y, both(0.24022119723855265f));
+  y = ffma2(f, y, both(0.6931469670646163f));
+  y = ffma2(f, y, both(1.0000000716546804f));
+  const float2 n = unpack2(t), r = unpack2(y);
+  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
+}
 
 // Row tiles of a segment that have rows.
 __device__ __forceinline__ int n_row_tiles(const AttnParams& p, const Segment& g) {
@@ -74,14 +102,15 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   uint64_t* q_empty = bars + 1;     // every Q.K^T of the item is complete
   uint64_t* o_final = bars + 2;     // [2] every P.V of the item's row tile is complete
   uint64_t* o_free = bars + 4;      // [2] all four warps of the tile hold its O in registers
-  uint64_t* s_full = bars + 6;      // [2] S_q holds Q_q.K^T, and every P.V before it is complete
-  uint64_t* p_full = bars + 8;      // [2] P_q is written (and O_q scaled) by all four warps of the tile
-  uint64_t* k_full = bars + 10;
-  uint64_t* v_full = bars + 10 + kStages;
-  uint64_t* k_empty = bars + 10 + 2 * kStages;      // (by both issuers)
-  uint64_t* v_empty = bars + 10 + 3 * kStages;
-  uint64_t* item_full = bars + 10 + 4 * kStages;               // [kItems] the segment is written
-  uint64_t* item_empty = bars + 10 + 4 * kStages + L::kItems;  // ... and read by the issuers and the eight softmax warps
+  uint64_t* s_full = bars + 6;      // [2][2] half h of S_q holds Q_q.K_h^T
+  uint64_t* p_full = bars + 10;     // [2][2] half h of P_q is written (and O_q scaled) by all four warps of the tile
+  uint64_t* pv_done = bars + 14;    // [2][2] O_q += P_q.V over half h is complete
+  uint64_t* k_full = bars + 18;
+  uint64_t* v_full = bars + 18 + kStages;
+  uint64_t* k_empty = bars + 18 + 2 * kStages;      // (by both issuers)
+  uint64_t* v_empty = bars + 18 + 3 * kStages;
+  uint64_t* item_full = bars + 18 + 4 * kStages;               // [kItems] the segment is written
+  uint64_t* item_empty = bars + 18 + 4 * kStages + L::kItems;  // ... and read by the issuers and the eight softmax warps
   Segment* segments = reinterpret_cast<Segment*>(smem + L::kOffSegments);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
@@ -94,8 +123,11 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     for (int q = 0; q < 2; ++q) {
       mbar_init(o_final + q, 1);
       mbar_init(o_free + q, 4);
-      mbar_init(s_full + q, 1);
-      mbar_init(p_full + q, 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(s_full + 2 * q + h, 1);
+        mbar_init(p_full + 2 * q + h, 4);
+        mbar_init(pv_done + 2 * q + h, 1);
+      }
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(k_full + s, 1);
@@ -145,27 +177,28 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   }
 
   // ------------------------------------------------------------------ MMA issuers
-  // Each for its row tile: QK(0) | PV(0) QK(1) | PV(1) QK(2) | ...  The tile is a constant of the code: the operands of tensor
+  // Each for its row tile, in halves of 64 keys: QK(0,0) QK(0,1) | PV(0,0) QK(1,0) | PV(0,1) QK(1,1) | ...  The tile is a constant of the code: the operands of tensor
   // instructions are uniform registers, and addresses that depend on the thread's warp number would be moved there one by one.
   auto issue_products = [&](auto tile_tag) {
     constexpr int q = decltype(tile_tag)::value;
     constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
-    constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kTileKeys);
+    constexpr uint32_t kIdescQK = umma_idesc(1, kFmt, kFmt, 0, 0, kTileM, kHalfKeys);
     constexpr uint32_t kIdescPV = umma_idesc(1, kFmt, kFmt, 0, 1, kTileM, D);              // V MN-major
     const uint32_t t_s = tmem_base + q * kTileKeys, t_o = tmem_base + kColO + q * D;
     int kt = 0, qt = 0, live_items = 0;             // key tiles so far, those of this row tile, items in which it had rows
     bool ok = true;
-    auto issue_qk = [&](int stage) {
-      // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes
+    auto issue_qk = [&](int stage, int h) {
+      // slabs of [128 rows][64 values], 8 rows = 1024 bytes; an instruction takes 16 values = 32 bytes, half h of K starts
+      // 64 rows into each slab
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const uint32_t slab = (k / 4) * L::kSlab;
         const uint64_t dq = umma_smem_desc(smem_u32(s_q + q * L::kQBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-        const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab), 16, 1024, kSwizzle128B) + 2 * (k % 4);
-        mma_f16_ss(t_s, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
+        const uint64_t dk = umma_smem_desc(smem_u32(s_k + stage * L::kKVBytes + slab + h * (kHalfKeys * 128)), 16, 1024, kSwizzle128B) + 2 * (k % 4);
+        mma_f16_ss(t_s + h * kHalfKeys, dq, dk, kIdescQK, k > 0 ? 1u : 0u);
       }
-      tc_commit(s_full + q);
-      tc_commit(k_empty + stage);
+      tc_commit(s_full + 2 * q + h);
+      if (h == 1) tc_commit(k_empty + stage);
     };
 #pragma unroll 1
     for (int items = 0; ok; ++items) {
@@ -188,7 +221,8 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       SAGE_PAGED_WAIT_OR(false, k_full + kt % kStages, (kt / kStages) & 1, 25, { ok = false; break; });
       tc_fence_after();
-      issue_qk(kt % kStages);
+      issue_qk(kt % kStages, 0);
+      issue_qk(kt % kStages, 1);
       if (n_tiles == 1) tc_commit(q_empty);
       // the first P.V of an item overwrites O: the O of the item before must have been read
       if (live_items > 0) SAGE_PAGED_WAIT_OR(false, o_free + q, (live_items - 1) & 1, 28, { ok = false; break; });
@@ -198,14 +232,21 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         // (the loads first: what follows P is the chain that the softmax waits for)
         SAGE_PAGED_WAIT_OR(false, v_full + s, (t / kStages) & 1, 27, { ok = false; break; });
         if (j + 1 < n_tiles) SAGE_PAGED_WAIT_OR(false, k_full + s1, ((t + 1) / kStages) & 1, 29, { ok = false; break; });
-        SAGE_PAGED_WAIT_OR(false, p_full + q, qt & 1, 26, { ok = false; break; });
-        tc_fence_after();
-        // V: [128 keys][64 values] slabs; an instruction takes 16 rows = 2048 bytes
-        const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes), L::kSlab, 1024, kSwizzle128B);
 #pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k) mma_f16_ts(t_o, t_s + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || k > 0) ? 1u : 0u);
-        if (j + 1 < n_tiles) issue_qk(s1);
-        else tc_commit(o_final + q);
+        for (int h = 0; h < 2; ++h) {
+          SAGE_PAGED_WAIT_OR(false, p_full + 2 * q + h, qt & 1, 26, { ok = false; break; });
+          tc_fence_after();
+          // V: [128 keys][64 values] slabs; half h starts 64 rows = 8192 bytes in, an instruction takes 16 rows = 2048 bytes
+          const uint64_t dv = umma_smem_desc(smem_u32(s_v + s * L::kKVBytes + h * (kHalfKeys * 128)), L::kSlab, 1024, kSwizzle128B);
+#pragma unroll
+          for (int k = 0; k < kHalfKeys / 16; ++k) {
+            mma_f16_ts(t_o, t_s + h * kHalfKeys + 8 * k, dv + 128 * k, kIdescPV, (j > 0 || h > 0 || k > 0) ? 1u : 0u);
+          }
+          tc_commit(pv_done + 2 * q + h);
+          if (j + 1 < n_tiles) issue_qk(s1, h);
+        }
+        if (!ok) break;
+        if (j + 1 == n_tiles) tc_commit(o_final + q);
         tc_commit(v_empty + s);
         if (j + 2 == n_tiles) tc_commit(q_empty);
       }
@@ -325,11 +366,12 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       bool settled = false;                           // every row of the warp has a maximum
       const f32x2_t scale2 = pack2(p.score_scale, p.score_scale);
 #pragma unroll 1
-      for (int j = 0; j < g.n_tiles; ++j) {
-        const int t = kt + j, first = g.key0 + j * kTileKeys;
-        SAGE_PAGED_WARP_WAIT_OR(false, s_full + q, (qt + j) & 1, 31, { ok = false; break; });
+      for (int hh = 0; hh < 2 * g.n_tiles; ++hh) {
+        const int h = hh & 1, t = kt + (hh >> 1), tq = qt + (hh >> 1), first = g.key0 + hh * kHalfKeys;
+        const uint32_t t_sh = t_s + h * kHalfKeys;
+        SAGE_PAGED_WARP_WAIT_OR(false, s_full + 2 * q + h, tq & 1, 31, { ok = false; break; });
         tc_fence_after();
-        if (first + kTileKeys > g.len) {
+        if (h == 0 && first + kTileKeys > g.len) {
           // The last tile: zeros over what is no value of the sequence, by both row tiles, either of which may be first.  (Behind
           // the wait for S, which says that the stage's load before this one has long been used: a parity cannot tell
           // phases apart that are two turns away.)
@@ -345,13 +387,16 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         if (warp_live) {
           // Weights of 32 columns against `base`, packed; returns their sum.
-          auto weigh = [&](const uint32_t (&sr)[32], float base, auto keep, uint32_t* pk) -> f32x2_t {
+          float high = -INFINITY;
+          auto weigh = [&](const uint32_t (&sr)[32], float base, auto keep, auto by_hand, uint32_t* pk) -> f32x2_t {
             const f32x2_t neg = pack2(kTileBias - base, kTileBias - base);
             f32x2_t acc = pack2(0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float2 x = unpack2(ffma2(pack2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), scale2, neg));
-              float2 w = make_float2(ex2(x.x), ex2(x.y));
+              float2 w;
+              if (by_hand(i)) w = exp2_by_polynomial(x.x, x.y, &high);
+              else w = make_float2(ex2(x.x), ex2(x.y));
               keep(2 * i, &w.x);
               keep(2 * i + 1, &w.y);
               acc = fadd2(acc, pack2(w.x, w.y));
@@ -359,39 +404,33 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
             return acc;
           };
-          const bool masked = first + kTileKeys > warp_limit;
+          const bool masked = first + kHalfKeys > warp_limit;
           const bool attempt = settled && !masked && distrust < 2;
           bool done = false;
           if (attempt) {
-            // P stays in registers until the sum has been looked at: S would be needed again.  The next columns are on
-            // their way while these are worked on.
-            uint32_t sr[2][32], pk[64];
-            f32x2_t acc = pack2(0.0f, 0.0f);
-            tmem_ld32(t_s, sr[0]);
+            // (P stays in registers until the sum has been looked at: S would be needed again)
+            uint32_t sr[2][32], pk[32];
+            tmem_ld32(t_sh, sr[0]);
+            tmem_ld32(t_sh + 32, sr[1]);
             tc_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c < 3) tmem_ld32(t_s + 32 * (c + 1), sr[(c + 1) & 1]);
-              acc = fadd2(acc, weigh(sr[c & 1], m, [](int, float*) {}, pk + 16 * c));
-              if (c < 3) tc_wait_ld();
-            }
-            const float2 a = unpack2(acc);
+            auto by_hand = [](int i) { return i % kHandEvery == kHandEvery - 1; };
+            const f32x2_t acc = weigh(sr[0], m, [](int, float*) {}, by_hand, pk);
+            const float2 a = unpack2(fadd2(acc, weigh(sr[1], m, [](int, float*) {}, by_hand, pk + 16)));
             const float sum = a.x + a.y;
-            done = !__any_sync(0xffffffffu, !(sum <= kTileSumMax));
+            done = !__any_sync(0xffffffffu, !(sum <= kTileSumMax) || high > 16.0f);
             if (done) {
               l += sum;
-              tmem_st32(t_s, *reinterpret_cast<const uint32_t(*)[32]>(pk));
-              tmem_st32(t_s + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+              tmem_st32(t_sh, pk);
             }
             distrust = done ? max(distrust - 1, 0) : min(distrust + 2, 4);
           }
           if (!done) {
-            const int col_end = live ? limit - first : kTileKeys;    // columns below it are visible
+            const int col_end = live ? limit - first : kHalfKeys;    // columns below it are visible
             float top = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
               uint32_t sr[32];
-              tmem_ld32(t_s + 32 * c, sr);
+              tmem_ld32(t_sh + 32 * c, sr);
               tc_wait_ld();
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
@@ -401,9 +440,11 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
             const bool need = top > m + (attempt ? kTileRefusedLazy : kTileLazy) || (m == -INFINITY && top > m);
             const bool moved = __any_sync(0xffffffffu, need);
-            if (!attempt && j > 0) distrust = moved ? min(distrust + 1, 4) : max(distrust - 1, 0);
+            if (!attempt && hh > 0) distrust = moved ? min(distrust + 1, 4) : max(distrust - 1, 0);
             if (moved) {
-              if (j > 0) {                            // (O is at rest: s_full)
+              if (hh > 0) {
+                SAGE_PAGED_WARP_WAIT_OR(false, pv_done + 2 * q + (h ^ 1), (h ? tq : tq - 1) & 1, 32, { ok = false; break; });
+                tc_fence_after();
                 const float back = need ? ex2(m - top) : 1.0f;
                 l *= back;
 #pragma unroll 1
@@ -421,22 +462,22 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             settled = !__any_sync(0xffffffffu, m == -INFINITY);
             const float base = m == -INFINITY ? 0.0f : m;            // (a row that has seen nothing yet)
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {             // (P of these columns goes where columns before them were)
+            for (int c = 0; c < 2; ++c) {             // (P of these columns goes where columns before them were)
               uint32_t sr[32], pk[16];
-              tmem_ld32(t_s + 32 * c, sr);
+              tmem_ld32(t_sh + 32 * c, sr);
               tc_wait_ld();
               const float2 a = unpack2(weigh(sr, base, [&](int i, float* w) {
                 if (32 * c + i >= col_end) *w = 0.0f;
-              }, pk));
+              }, [](int) { return false; }, pk));
               l += a.x + a.y;
-              tmem_st16(t_s + 16 * c, pk);
+              tmem_st16(t_sh + 16 * c, pk);
             }
           }
           tc_wait_st();
         }
         tc_fence_before();
         __syncwarp();                                 // (an arrival per warp: 128 of them on one word take turns)
-        if (lane == 0) mbar_arrive(p_full + q);
+        if (lane == 0) mbar_arrive(p_full + 2 * q + h);
       }
       if (!ok) break;
       SAGE_PAGED_WARP_WAIT_OR(false, o_final + q, live_items & 1, 33, { ok = false; break; });
