@@ -119,7 +119,7 @@ Batch batch_of(const sage_paged_batch_t* b, const sage_paged_kv_t* c) {
 struct PagedPlan {
   bool tensor = false;          // sage_paged_tile_kernel
   int tile_rows = 0;
-  int item_cost = 0;
+  int item_cost = 0, tile_cost = 1, light_cost = 1;
   int grid = 0;
   bool merge = false;           // an item may be cut
   int64_t header_bytes = 0, e_bytes = 0, o_bytes = 0;
@@ -136,10 +136,18 @@ int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t t
   const int64_t rows = std::min(max_q, tokens) * group;
   plan->tensor = rows > 32;
   plan->tile_rows = plan->tensor ? 2 * (kTileM / group) * group : rows <= 16 ? 16 : 32;
+  // Steps.  With few rows a key tile costs the same whatever the rows; on tensor cores, us per key tile with one / two row
+  // tiles: D=128 1.64 / 2.07, D=64 1.37 / 1.80.
   // What the start and end of an item cost, in key tiles.  us of the attention kernel with 0 / 1 / 2 / 3: 64 sequences of 60 to
   // 16000 keys, a token each, 157 / 148 / 150 / 152; 32 of 500 to 6000, 3 to 5 tokens (32 rows) 94 / 88 / 81 / 78; chunks of
   // prompts (128 rows) 244 / 235 / 223 / 222; 128 sequences of 1 to 1000 keys, a token each, 47 / 40 / 40 / 43.
-  plan->item_cost = plan->tensor ? 2 : plan->tile_rows == 16 ? 1 : 3;
+  if (plan->tensor) {
+    plan->item_cost = 12;
+    plan->tile_cost = 5;
+    plan->light_cost = 4;
+  } else {
+    plan->item_cost = plan->tile_rows == 16 ? 1 : 3;
+  }
   const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
   const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
   plan->grid = static_cast<int>(std::min<int64_t>(sms, std::min<int64_t>(row_tiles * c->Hkv, sms) * tiles));
@@ -202,6 +210,8 @@ template <typename T, int D>
 int launch_pass(const sage_paged_kv_t* c, AttnParams p, const PagedPlan& plan, char* workspace, cudaStream_t stream) {
   p.tile_rows = plan.tile_rows;
   p.item_cost = plan.item_cost;
+  p.tile_cost = plan.tile_cost;
+  p.light_cost = plan.light_cost;
   p.by_group = FastDiv::of(p.group);
   p.by_tile_rows = FastDiv::of(p.tile_rows);
   p.headers = reinterpret_cast<PartHeader*>(workspace);

@@ -3,7 +3,7 @@
 // An item is one row tile of one kv head of one sequence: up to `tile_rows` rows (new token, query head of the group) that
 // read the same keys.  Its steps are tiles of 128 keys, at least one (an item without keys writes zeros), behind `item_cost` more that
 // stand for its start and end.  The steps of all items, after sequence, kv head after kv head, row tile after row tile, form one line that is cut into equal spans, one per CTA:
-// lengths may differ as they like and all CTAs get the same amount of work.  A span that covers part of an item leaves
+// lengths may differ as they like and all CTAs get the same amount of work.  A key tile belongs to the CTA that has its first step.  A span that covers part of an item leaves
 // its result in a slot of the workspace (slot 1 the head of an item, slot 0 anything else: at most one of each per
 // CTA) and a header that tells the merge kernels which parts follow.  Every CTA works this out for itself from kv_lens and
 // cu_q, by a block-wide prefix sum; nothing is communicated and the order of all sums is fixed.
@@ -38,7 +38,11 @@ struct FastDiv {
 
 // (Small code matters here: a kernel of this file runs for tens of microseconds, and its instructions come from the L2 or
 // from memory at first.  What is called once an item stands once, in loops that are not unrolled.)
-__device__ __noinline__ long long floor_div(long long a, long long b) { return a / b; }
+__device__ __noinline__ long long long_div(long long a, long long b) { return a / b; }
+__device__ __forceinline__ long long floor_div(long long a, long long b) {
+  if (a <= 0x7fffffffLL && b <= 0x7fffffffLL) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return long_div(a, b);
+}
 
 struct AttnParams {
   const void* q;
@@ -59,6 +63,8 @@ struct AttnParams {
   int tile_rows;                // rows of a row tile
   FastDiv by_group, by_tile_rows;
   int item_cost;                // steps that stand for the start and end of an item
+  int tile_cost;                // steps of a key tile; and ...
+  int light_cost;               // ... where the item has at most half the rows of a row tile
   int causal;
   int zero_rest;                // write zeros to rows that belong to no sequence
   float score_scale;            // sm_scale * log2(e)
@@ -81,7 +87,8 @@ struct PartHeader {             // of the part in slot 1 of a CTA, if it is the 
 struct Seq {
   int q0, n_q;                  // new tokens
   int key0, len;                // keys [key0, len)
-  int row_tiles, key_tiles;
+  int row_tiles;
+  long long head_steps;         // steps of one kv head
 };
 
 __device__ __forceinline__ int n_seqs(const AttnParams& p) { return p.shared_pass ? 1 : p.batch.B; }
@@ -89,6 +96,15 @@ __device__ __forceinline__ int n_seqs(const AttnParams& p) { return p.shared_pas
 __device__ __forceinline__ int clipped_len(const AttnParams& p, int b) {
   const long long most = static_cast<long long>(p.batch.table_width) << p.batch.page_log2;
   return static_cast<int>(min(static_cast<long long>(max(p.batch.kv_lens[b], 0)), most));
+}
+
+// Key tiles of row tile `rt`, and the steps of one of them.
+__device__ __forceinline__ void item_of(const AttnParams& p, const Seq& s, int rt, int* tiles, int* cost) {
+  const int last_row = (rt + 1) * p.tile_rows;
+  int end = s.len;
+  if (p.causal && !p.shared_pass) end -= max(0, s.n_q - (p.by_group(last_row - 1) + 1));
+  *tiles = max(1, (end - s.key0 + kTileKeys - 1) / kTileKeys);
+  *cost = s.n_q * p.group - rt * p.tile_rows > p.tile_rows / 2 ? p.tile_cost : p.light_cost;
 }
 
 __device__ __forceinline__ Seq seq_at(const AttnParams& p, int b) {
@@ -106,13 +122,17 @@ __device__ __forceinline__ Seq seq_at(const AttnParams& p, int b) {
     s.len = clipped_len(p, b);
   }
   s.row_tiles = p.by_tile_rows(s.n_q * p.group + p.tile_rows - 1);
-  s.key_tiles = max(1, (s.len - s.key0 + kTileKeys - 1) / kTileKeys);
+  s.head_steps = 0;
+#pragma unroll 1
+  for (int rt = 0; rt < s.row_tiles; ++rt) {
+    int tiles, cost;
+    item_of(p, s, rt, &tiles, &cost);
+    s.head_steps += p.item_cost + static_cast<long long>(tiles) * cost;
+  }
   return s;
 }
 
-__device__ __forceinline__ long long steps_of(const AttnParams& p, const Seq& s) {
-  return static_cast<long long>(s.row_tiles) * (s.key_tiles + p.item_cost) * p.Hkv;
-}
+__device__ __forceinline__ long long steps_of(const AttnParams& p, const Seq& s) { return s.head_steps * p.Hkv; }
 
 // Keys that a new token sees: [0, limit).
 __device__ __forceinline__ int visible_keys(const AttnParams& p, int b, int q1, int token) {
@@ -176,10 +196,12 @@ __device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratc
   }
   upto += base;
   Span s;
-  s.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  // (a CTA has at least the steps of a key tile: none that stands inside an item is without one)
+  const long long most = p.tile_cost == 1 ? total : floor_div(total, p.tile_cost);
+  s.ctas = total == 0 ? 0 : static_cast<int>(max(1LL, min(static_cast<long long>(gridDim.x), most)));
   const int c = blockIdx.x;
   const bool idle = c >= s.ctas;
-  s.share = total < 0x7fffffffLL ? static_cast<int>(total) / max(s.ctas, 1) : floor_div(total, s.ctas);
+  s.share = floor_div(total, max(s.ctas, 1));
   s.extra = static_cast<int>(total - s.share * s.ctas);
   s.t = idle ? 0 : s.share * c + min(c, s.extra);
   s.t_end = idle ? 0 : s.t + s.share + (c < s.extra ? 1 : 0);
@@ -223,7 +245,10 @@ struct SegmentIter {
   int base;                     // lane i holds sequence base + i
   Seq mine;
   Seq seq;                      // of s.b
-  long long steps;
+  long long steps;              // of seq; -1: not looked at yet
+  int head, rt, tiles, cost;    // the item at hand
+  long long item_at;            // its first step
+  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span), base(-32), steps(-1), head(-1) {}
   __device__ __forceinline__ void find(int b) {
     const int lane = threadIdx.x & 31;
     if (b >= base + 32) {
@@ -236,10 +261,10 @@ struct SegmentIter {
     seq.key0 = p.shared_pass ? 0 : p.shared_len;
     seq.len = __shfl_sync(0xffffffffu, mine.len, from);
     seq.row_tiles = __shfl_sync(0xffffffffu, mine.row_tiles, from);
-    seq.key_tiles = __shfl_sync(0xffffffffu, mine.key_tiles, from);
+    seq.head_steps = __shfl_sync(0xffffffffu, mine.head_steps, from);
     steps = steps_of(p, seq);
+    head = -1;
   }
-  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span), base(-32), steps(-1) {}
   __device__ __forceinline__ Segment next() {
     Segment g;
     g.n_tiles = 0;
@@ -253,35 +278,48 @@ struct SegmentIter {
         }
         find(s.b);
       }
-      const int item_steps = seq.key_tiles + p.item_cost;
-      const long long r = s.t - s.before;
-      const int item = r < 0x7fffffffLL ? static_cast<int>(r) / item_steps : static_cast<int>(floor_div(r, item_steps));
-      const int at = static_cast<int>(r - static_cast<long long>(item) * item_steps);
-      const int count = static_cast<int>(min(static_cast<long long>(item_steps - at), s.t_end - s.t));
-      const int tile = max(at - p.item_cost, 0);
-      g.n_tiles = at + count - p.item_cost - tile;    // 0: nothing but the set-up of the item, which the CTA with its first tile does
-      if (g.n_tiles < 0) g.n_tiles = 0;
+      if (head < 0) {                                 // the head by division, its row tile step by step
+        head = static_cast<int>(floor_div(s.t - s.before, seq.head_steps));
+        item_at = s.before + head * seq.head_steps;
+        rt = 0;
+        item_of(p, seq, rt, &tiles, &cost);
+      }
+#pragma unroll 1
+      while (s.t >= item_at + p.item_cost + static_cast<long long>(tiles) * cost) {
+        item_at += p.item_cost + static_cast<long long>(tiles) * cost;
+        if (++rt == seq.row_tiles) {
+          rt = 0;
+          ++head;
+        }
+        item_of(p, seq, rt, &tiles, &cost);
+      }
+      const long long item_end = item_at + p.item_cost + static_cast<long long>(tiles) * cost;
+      const long long first_tile = item_at + p.item_cost, stop = min(item_end, s.t_end);
+      // tiles whose first step is in [t, stop)
+      const int lo = s.t <= first_tile ? 0 : static_cast<int>(s.t - first_tile + cost - 1) / cost;
+      const int hi = stop <= first_tile ? 0 : static_cast<int>(stop - first_tile + cost - 1) / cost;
+      g.n_tiles = hi - lo;
       g.q0 = seq.q0;
       g.n_q = seq.n_q;
       g.len = seq.len;
-      g.key0 = seq.key0 + tile * kTileKeys;
-      g.kv_head = seq.row_tiles == 1 ? item : item / seq.row_tiles;
-      g.head0 = g.kv_head * p.group;
-      g.row0 = (item - g.kv_head * seq.row_tiles) * p.tile_rows;
+      g.key0 = seq.key0 + lo * kTileKeys;
+      g.kv_head = head;
+      g.head0 = head * p.group;
+      g.row0 = rt * p.tile_rows;
       g.b = s.b;
       g.n_parts = 1;
-      if (tile > 0) {
+      if (lo > 0) {
         g.slot = 0;
-      } else if (g.n_tiles == seq.key_tiles) {
+      } else if (hi == tiles) {
         g.slot = -1;
       } else {
         g.slot = 1;
-        // the CTA that owns the last step of the item
-        const long long e = s.t + item_steps - at - 1, longer = s.extra * (s.share + 1);
+        // the CTA that has the first step of the last tile
+        const long long e = item_end - cost, longer = s.extra * (s.share + 1);
         const long long c = e < longer ? floor_div(e, s.share + 1) : s.extra + floor_div(e - longer, s.share);
         g.n_parts = static_cast<int>(c) - static_cast<int>(blockIdx.x) + 1;
       }
-      s.t += count;
+      s.t = stop;
     }
     return g;
   }
