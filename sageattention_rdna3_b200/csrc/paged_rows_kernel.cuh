@@ -31,8 +31,8 @@ template <int D, int MT>
 struct RowsSmem {
   static constexpr int kRows = 16 * MT;
   static constexpr int kStages = D == 128 ? 3 : 6;
-  static constexpr int kSlab = kTileKeys * 128;       // 128 keys x 64 values, 128-byte swizzle
-  static constexpr int kStage = 2 * (D / 64) * kSlab; // K and V of a tile
+  static constexpr int kTile = kTileKeys * D * 2;     // K or V: box after box, each [D / 64][keys][64 values], 128-byte swizzle
+  static constexpr int kStage = 2 * kTile;
   static constexpr int kItems = 2;                    // items ahead: segment and rows of Q
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kJoinRows = 8;                 // rows that the warps join at a time
@@ -44,7 +44,7 @@ struct RowsSmem {
   static constexpr int kOffBar = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
   static constexpr int kNumBars = 2 * kStages + 2 * kItems + 1;
   static constexpr int kOffScratch = kOffBar + kNumBars * 8;
-  static constexpr int kOffMisc = kOffScratch + (kRowsThreads / 32 + 4) * 8;
+  static constexpr int kOffMisc = kOffScratch + static_cast<int>(sizeof(SpanScratch));
   static constexpr int kTotal = kOffMisc + 16;
   static_assert(kTotal <= 232448, "shared memory of an SM");
 };
@@ -78,9 +78,9 @@ __device__ __forceinline__ int checked_page(const AttnParams& p, int page) {
   return 0;
 }
 
-// 16 bytes from global to shared memory, zeros if !ok; counted on an mbarrier by cp_async_arrive.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+// 16 bytes from global to shared memory; counted on an mbarrier by cp_async_arrive.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -90,7 +90,7 @@ template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
   using L = RowsSmem<D, MT>;
-  constexpr int kRows = L::kRows, kStages = L::kStages, kItems = L::kItems, kSlabs = D / 64;
+  constexpr int kRows = L::kRows, kStages = L::kStages, kItems = L::kItems;
   constexpr float kBias = std::is_same<T, __half>::value ? 15.0f : 0.0f;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -118,14 +118,14 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     tma_prefetch_desc(&tm_v);
   }
   grid_dependency_wait();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == kRowsThreads - 1) {               // (a thread that has no sequence to look up, as a rule)
     // a wait of an earlier launch that ran out and was not looked at yet: this launch does nothing (as attn_kernel.cuh)
     const int before = p.status.word != nullptr ? *reinterpret_cast<volatile int*>(p.status.word) : 0;
     *abort_flag = misaligned || (before & 15) == 2;
     if (misaligned) p.status.report(kStatusMisaligned);
     p.headers[blockIdx.x].n_parts = 0;
   }
-  const Span span = find_span<kRowsThreads>(p, reinterpret_cast<long long*>(smem + L::kOffScratch));
+  const Span span = find_span<kRowsThreads>(p, reinterpret_cast<SpanScratch*>(smem + L::kOffScratch));
   grid_launch_dependents();
   if (*abort_flag) return;
 
@@ -152,15 +152,18 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       ok = warp_wait<true>(item_empty + slot, ((item / kItems) & 1) ^ 1u, abort_flag, p.wait_limit_cycles);
       if (!ok) break;
       if (g.n_tiles > 0) {
-        const uint32_t s_q = smem_u32(smem + L::kOffQ + slot * L::kQBytes);
-        constexpr int kChunks = D / 8;
-#pragma unroll 1
-        for (int i = 0; i < kRows * kChunks / 32; ++i) {
-          const int r = (i * 32 + lane) / kChunks, c = lane % kChunks;
-          int token = 0, head = 0;
-          const bool live = row_at(p, g.q0, g.n_q, g.head0, g.row0, kRows, r, &token, &head);
-          const T* src = static_cast<const T*>(p.q) + (live ? token * p.q_stride_t + head * p.q_stride_h + c * 8 : 0);
-          cp_async16(s_q + r * (D * 2) + ((c & ~7) << 4) + (((c ^ r) & 7) << 4), src, live);
+        // Rows without a token stay what they are: no row's result depends on another's.
+        constexpr int kPerRow = 32 / kRows, kChunks = D / 8 / kPerRow;         // lanes of a row, 16-byte pieces of each
+        const int r = lane / kPerRow, c0 = lane % kPerRow * kChunks;
+        int token = 0, head = 0;
+        if (row_at(p, g.q0, g.n_q, g.head0, g.row0, kRows, r, &token, &head)) {
+          const T* src = static_cast<const T*>(p.q) + token * p.q_stride_t + head * p.q_stride_h;
+          const uint32_t s_q = smem_u32(smem + L::kOffQ + slot * L::kQBytes) + r * (D * 2);
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i) {
+            const int c = c0 + i;
+            cp_async16(s_q + ((c & ~7) << 4) + (((c ^ r) & 7) << 4), src + c * 8);
+          }
         }
       }
       if (lane == 0) segments[slot] = g;
@@ -179,11 +182,8 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         for (int x = 0; x < boxes; ++x) {
           const int page = __shfl_sync(0xffffffffu, checked, x);
           if (leader) {
-#pragma unroll
-            for (int c = 0; c < kSlabs; ++c) {
-              tma_load_4d(dst + c * L::kSlab + x * box_rows * 128, &tm_k, full + stage, c * 64, first & slot_mask, g.kv_head, page);
-              tma_load_4d(dst + (kSlabs + c) * L::kSlab + x * box_rows * 128, &tm_v, full + stage, c * 64, first & slot_mask, g.kv_head, page);
-            }
+            tma_load_5d(dst + x * box_rows * (D * 2), &tm_k, full + stage, 0, first & slot_mask, 0, g.kv_head, page);
+            tma_load_5d(dst + L::kTile + x * box_rows * (D * 2), &tm_v, full + stage, 0, first & slot_mask, 0, g.kv_head, page);
           }
         }
         if (j + 1 < g.n_tiles) find_pages(g, j + 1);  // (they arrive while the stage is waited for)
@@ -201,6 +201,10 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   }
 
   // -------------------------------------------------------------------- work
+  // Where this warp's 32 keys of a tile are: `at`, keys 16-31 `upper` behind 0-15, the next 64 values `slab` behind.
+  const int box_rows = min(1 << p.batch.page_log2, kTileKeys);
+  const uint32_t slab = box_rows * 128, upper = box_rows == 16 ? 16 * D * 2 : 16 * 128;
+  const uint32_t at = (warp * kUnitKeys & ~(box_rows - 1)) * (D * 2) + (warp * kUnitKeys & (box_rows - 1)) * 128;
   float* s_join = reinterpret_cast<float*>(smem + L::kOffJoin);
   float* s_m = reinterpret_cast<float*>(smem + L::kOffStats);
   float* s_l = s_m + kRowsWarps * kRows;
@@ -279,7 +283,7 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       const int first = g.key0 + j * kTileKeys + warp * kUnitKeys;
       const int keys = min(kUnitKeys, g.len - first);
       if (keys > 0) {
-        const uint32_t s_k = smem_u32(smem + stage * L::kStage) + warp * (kUnitKeys * 128), s_v = s_k + kSlabs * L::kSlab;
+        const uint32_t s_k = smem_u32(smem + stage * L::kStage) + at, s_v = s_k + L::kTile;
 
         // S = Q.K^T: 4 groups of 8 keys
         float s[MT][4][4];
@@ -304,10 +308,10 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll
           for (int n2 = 0; n2 < 2; ++n2) {
             // matrices: (keys 0-7, values 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15) of a 16 x 16 block
-            const int key = n2 * 16 + (lane >> 4) * 8 + (lane & 7);
+            const int key = (lane >> 4) * 8 + (lane & 7);
             const int chunk = (k % 4) * 2 + ((lane >> 3) & 1);
             uint32_t b[4];
-            ldmatrix_x4(s_k + (k / 4) * L::kSlab + key * 128 + ((chunk ^ (key & 7)) << 4), b);
+            ldmatrix_x4(s_k + (k / 4) * slab + n2 * upper + key * 128 + ((chunk ^ (key & 7)) << 4), b);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               mma_16816(s[mt][2 * n2], a[mt], b[0], b[1], static_cast<const T*>(nullptr));
@@ -385,10 +389,10 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll
           for (int n2 = 0; n2 < D / 16; ++n2) {
             // matrices: (keys 0-7, values 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15) of a 16 x 16 block, transposed
-            const int key = k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+            const int key = ((lane >> 3) & 1) * 8 + (lane & 7);
             const int chunk = (n2 % 4) * 2 + (lane >> 4);
             uint32_t b[4];
-            ldmatrix_x4_trans(s_v + (n2 / 4) * L::kSlab + key * 128 + ((chunk ^ (key & 7)) << 4), b);
+            ldmatrix_x4_trans(s_v + (n2 / 4) * slab + k * upper + key * 128 + ((chunk ^ (key & 7)) << 4), b);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               mma_16816(o[mt][2 * n2], pf[mt][k], b[0] & mask0, b[1] & mask1, static_cast<const T*>(nullptr));

@@ -164,12 +164,20 @@ struct Span {
   int extra;
   int ctas;                     // CTAs that have steps at all
   int b;                        // sequence of step t ...
-  long long before;             // ... and the steps before that sequence
+  long long before;             // ... the steps before that sequence, and the sequence
+  Seq seq;
+};
+struct SpanScratch {            // in shared memory
+  long long warp_steps[16];
+  long long before;
+  Seq seq;
+  int b;
 };
 
-// `scratch`: shared memory for kThreads / 32 + 4 long longs.  Ends with a barrier.
+// Ends with a barrier.
 template <int kThreads>
-__device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratch) {
+__device__ __forceinline__ Span find_span(const AttnParams& p, SpanScratch* scratch) {
+  static_assert(kThreads <= 512, "");
   const int n = n_seqs(p);
   const int per = (n + kThreads - 1) / kThreads;
   const int first = threadIdx.x * per, last = min(first + per, n);
@@ -186,13 +194,13 @@ __device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratc
     const long long other = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += other;
   }
-  if (lane == 31) scratch[warp] = upto;
+  if (lane == 31) scratch->warp_steps[warp] = upto;
   __syncthreads();
   long long total = 0, base = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) base += scratch[w];
-    total += scratch[w];
+    if (w < warp) base += scratch->warp_steps[w];
+    total += scratch->warp_steps[w];
   }
   upto += base;
   Span s;
@@ -209,19 +217,23 @@ __device__ __forceinline__ Span find_span(const AttnParams& p, long long* scratc
   if (!idle && s.t >= upto - mine && s.t < upto) {
     long long before = upto - mine;
     int b = first;
+    Seq seq;
 #pragma unroll 1
     while (true) {
-      const long long steps = steps_of(p, seq_at(p, b));
+      seq = seq_at(p, b);
+      const long long steps = steps_of(p, seq);
       if (s.t < before + steps) break;
       before += steps;
       ++b;
     }
-    scratch[kThreads / 32] = b;
-    scratch[kThreads / 32 + 1] = before;
+    scratch->b = b;
+    scratch->before = before;
+    scratch->seq = seq;
   }
   __syncthreads();
-  s.b = idle ? 0 : static_cast<int>(scratch[kThreads / 32]);
-  s.before = idle ? 0 : scratch[kThreads / 32 + 1];
+  s.b = scratch->b;
+  s.before = scratch->before;
+  s.seq = scratch->seq;
   return s;
 }
 
@@ -245,13 +257,15 @@ struct SegmentIter {
   int base;                     // lane i holds sequence base + i
   Seq mine;
   Seq seq;                      // of s.b
-  long long steps;              // of seq; -1: not looked at yet
+  long long steps;              // of seq
   int head, rt, tiles, cost;    // the item at hand
   long long item_at;            // its first step
-  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span), base(-32), steps(-1), head(-1) {}
+  __device__ __forceinline__ SegmentIter(const AttnParams& pp, const Span& span) : p(pp), s(span), base(-32), seq(span.seq), head(-1) {
+    steps = s.t < s.t_end ? steps_of(p, seq) : 0;
+  }
   __device__ __forceinline__ void find(int b) {
     const int lane = threadIdx.x & 31;
-    if (b >= base + 32) {
+    if (base < 0 || b >= base + 32) {
       base = b;
       if (b + lane < n_seqs(p)) mine = seq_at(p, b + lane);
     }
@@ -271,12 +285,9 @@ struct SegmentIter {
 #pragma unroll 1
     while (s.t < s.t_end && g.n_tiles == 0) {
 #pragma unroll 1
-      while (steps < 0 || s.t >= s.before + steps) {  // (sequences without new tokens have no steps)
-        if (steps >= 0) {
-          s.before += steps;
-          ++s.b;
-        }
-        find(s.b);
+      while (s.t >= s.before + steps) {               // (sequences without new tokens have no steps)
+        s.before += steps;
+        find(++s.b);
       }
       if (head < 0) {                                 // the head by division, its row tile step by step
         head = static_cast<int>(floor_div(s.t - s.before, seq.head_steps));

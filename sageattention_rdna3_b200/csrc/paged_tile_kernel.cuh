@@ -55,7 +55,7 @@ struct TileSmem {
   static constexpr int kNumBars = 18 + 4 * kStages + 2 * kItems;
   static constexpr int kOffSegments = kOffBar + 8 * kNumBars;
   static constexpr int kOffScratch = kOffSegments + kItems * static_cast<int>(sizeof(Segment));
-  static constexpr int kOffMisc = kOffScratch + 8 * (kTileThreads / 32 + 4);
+  static constexpr int kOffMisc = kOffScratch + static_cast<int>(sizeof(SpanScratch));
   static constexpr int kTotal = kOffMisc + 16;
 };
 
@@ -150,7 +150,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     tmem_alloc(tmem_slot, kTileTmemCols);
     tmem_relinquish();
   }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == kTileThreads - 1) {               // (a thread that has no sequence to look up, as a rule)
     const int before = p.status.word != nullptr ? *reinterpret_cast<volatile int*>(p.status.word) : 0;
     *abort_flag = misaligned || (before & 15) == 2;
     *fail_code = 0;
@@ -158,7 +158,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     p.headers[blockIdx.x].n_parts = 0;
   }
   tc_fence_before();
-  const Span span = find_span<kTileThreads>(p, reinterpret_cast<long long*>(smem + L::kOffScratch));
+  const Span span = find_span<kTileThreads>(p, reinterpret_cast<SpanScratch*>(smem + L::kOffScratch));
   tc_fence_after();
   grid_launch_dependents();
   const uint32_t tmem_base = *tmem_slot;
