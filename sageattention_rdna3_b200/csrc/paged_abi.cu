@@ -150,7 +150,8 @@ int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t t
   }
   const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
   const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
-  plan->grid = static_cast<int>(std::min<int64_t>(sms, std::min<int64_t>(row_tiles * c->Hkv, sms) * tiles));
+  const int64_t slots = static_cast<int64_t>(sms) * (plan->tensor ? 1 : rows_ctas_per_sm(c->D, plan->tile_rows / 16));
+  plan->grid = static_cast<int>(std::min<int64_t>(slots, std::min<int64_t>(row_tiles * c->Hkv, slots) * tiles));
   plan->merge = tiles > 1;
   plan->header_bytes = round16(static_cast<int64_t>(plan->grid) * sizeof(PartHeader));
   plan->e_bytes = round16(static_cast<int64_t>(plan->grid) * 2 * plan->tile_rows * sizeof(float));
@@ -214,9 +215,10 @@ int encode_pages(CUtensorMap* map, CUtensorMapDataType dt, const sage_paged_kv_t
   if (tensor) return encode_strided_16bit(map, dt, base, c->D, c->page_size, c->Hkv, c->num_pages, slot, head, page, rows, what);
   const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(c->page_size), static_cast<cuuint64_t>(c->D / 64), static_cast<cuuint64_t>(c->Hkv),
                               static_cast<cuuint64_t>(c->num_pages)};
-  // (a dimension of extent 1 may carry any stride in the caller's tensor; it gets that of a whole page)
-  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot) * 2, 128, static_cast<cuuint64_t>(c->Hkv > 1 ? head : page) * 2,
-                                 static_cast<cuuint64_t>(page) * 2};
+  // (a dimension of extent 1 may carry any stride in the caller's tensor; it gets the span of the others)
+  if (c->num_pages == 1) page = std::max(slot * c->page_size, c->Hkv > 1 ? head * c->Hkv : 0);
+  if (c->Hkv == 1) head = page;
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot) * 2, 128, static_cast<cuuint64_t>(head) * 2, static_cast<cuuint64_t>(page) * 2};
   const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(c->D / 64), 1, 1};
   return encode_map(map, dt, 5, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, what);
 }
@@ -241,7 +243,8 @@ int launch_pass(const sage_paged_kv_t* c, AttnParams p, const PagedPlan& plan, c
   if (plan.tensor) {
     rc = launch_tile<T, D>(tk, tv, p, plan, dt, stream);
     if (rc || !plan.merge) return rc;
-    return launch(sage_paged_merge_columns_kernel<T, D>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>((plan.tile_rows + 31) / 32)), kMergeThreads, 0, stream, p);
+    return launch(sage_paged_merge_columns_kernel<T, D>, dim3(static_cast<unsigned>(plan.grid), static_cast<unsigned>((plan.tile_rows + 31) / 32), MergeColumns<D>::kBlocks),
+                  kMergeThreads, 0, stream, p);
   }
   rc = plan.tile_rows == 16 ? launch_rows<T, D, 1>(tk, tv, p, plan, stream) : launch_rows<T, D, 2>(tk, tv, p, plan, stream);
   if (rc || !plan.merge) return rc;

@@ -27,10 +27,14 @@ constexpr int kRowsThreads = 160;
 constexpr int kRowsWarps = 4;                         // that compute
 constexpr int kUnitKeys = 32;                         // keys of a tile that one of them takes
 
+// CTAs of an SM.  A key tile of D=64 is half the bytes and two thirds of the instructions of one of D=128: two CTAs share the SM.
+// (With 32 rows their shared memory does not fit.)
+constexpr int rows_ctas_per_sm(int D, int MT) { return D == 64 && MT == 1 ? 2 : 1; }
+
 template <int D, int MT>
 struct RowsSmem {
   static constexpr int kRows = 16 * MT;
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kStages = D == 128 || MT == 1 ? 3 : 6;
   static constexpr int kTile = kTileKeys * D * 2;     // K or V: box after box, each [D / 64][keys][64 values], 128-byte swizzle
   static constexpr int kStage = 2 * kTile;
   static constexpr int kItems = 2;                    // items ahead: segment and rows of Q
@@ -46,7 +50,7 @@ struct RowsSmem {
   static constexpr int kOffScratch = kOffBar + kNumBars * 8;
   static constexpr int kOffMisc = kOffScratch + static_cast<int>(sizeof(SpanScratch));
   static constexpr int kTotal = kOffMisc + 16;
-  static_assert(kTotal <= 232448, "shared memory of an SM");
+  static_assert((kTotal + 1024) * rows_ctas_per_sm(D, MT) <= 233472, "shared memory of an SM");
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -87,7 +91,7 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 }
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kRowsThreads, 1)
+__global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm(D, MT))
 sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
   using L = RowsSmem<D, MT>;
   constexpr int kRows = L::kRows, kStages = L::kStages, kItems = L::kItems;

@@ -446,7 +446,7 @@ __device__ __forceinline__ void zero_rest(const AttnParams& p, int D, int thread
 // writer stores it in whole lines:
 //   rows (sage_paged_rows_kernel)  row after row; a warp has one row, kWarps / ROWS warps every so many parts of it
 //   columns (sage_paged_tile_kernel, a thread per row)  4 neighbouring values of all rows, then the next 4; here a warp has 32
-//   rows and kVecs of their float4 columns
+//   rows and kVecs of their float4 columns (blockIdx.z: which)
 // Four parts are in flight together, in the order of the keys: the result does not depend on who came first.
 constexpr int kMergeThreads = 256;
 
@@ -457,10 +457,11 @@ struct PartSum {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = 0.0f;
   }
-  __device__ __forceinline__ void add(const float (&pe)[4], const float (&px)[4][N]) {
+  template <int K>
+  __device__ __forceinline__ void add(const float (&pe)[K], const float (&px)[K][N]) {
     float top = e;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) top = fmaxf(top, pe[c]);
+    for (int c = 0; c < K; ++c) top = fmaxf(top, pe[c]);
     if (top == -INFINITY) return;                     // no visible keys so far
     const float back = ex2(e - top);
     sum *= back;
@@ -468,7 +469,7 @@ struct PartSum {
     for (int i = 0; i < N; ++i) x[i] *= back;
     e = top;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < K; ++c) {
       const float f = ex2(pe[c] - top);
       sum += f;
 #pragma unroll
@@ -546,22 +547,29 @@ __global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_rows_kernel(co
   if (live) write_row<T, kPer>(p, token, head, D, lane * kPer, acc.x, acc.lse(), lane == 0);
 }
 
+template <int D>
+struct MergeColumns {
+  static constexpr int kVecs = 2;                      // float4 columns of a thread; with 4 / 1 the join of 9 parts of 256 rows each takes
+  static constexpr int kFlight = 4;                    // 9.8 / 10 us instead of 8.5; parts in flight: with 2 / 8 9.5 / 10.5
+  static constexpr int kBlocks = D / 4 / (kMergeThreads / 32 * kVecs);   // of 32 rows
+};
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeThreads) sage_paged_merge_columns_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int kVecs = D / 4 / (kMergeThreads / 32);           // float4 columns per thread: 4 or 2
+  using M = MergeColumns<D>;
+  constexpr int kVecs = M::kVecs, kFlight = M::kFlight;
   grid_dependency_wait();
   grid_launch_dependents();
   const PartHeader h = p.headers[blockIdx.x];
   if (h.n_parts < 2 || static_cast<long long>(h.tokens) * p.group <= h.row0 + static_cast<int>(blockIdx.y) * 32) return;
-  const int r = blockIdx.y * 32 + (threadIdx.x & 31), c0 = (threadIdx.x >> 5) * kVecs;
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), c0 = (blockIdx.z * (kMergeThreads / 32) + (threadIdx.x >> 5)) * kVecs;
   int token = 0, head = 0;
   if (!merge_row(p, h, r, &token, &head)) return;
   PartSum<4 * kVecs> acc;
 #pragma unroll 1
-  for (int k0 = 0; k0 < h.n_parts; k0 += 4) {
-    float pe[4], px[4][4 * kVecs];
+  for (int k0 = 0; k0 < h.n_parts; k0 += kFlight) {
+    float pe[kFlight], px[kFlight][4 * kVecs];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < kFlight; ++c) {
       const int k = k0 + c;
       pe[c] = -INFINITY;
 #pragma unroll
