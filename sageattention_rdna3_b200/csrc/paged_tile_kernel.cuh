@@ -81,6 +81,13 @@ __device__ __forceinline__ float2 exp2_by_polynomial(float x0, float x1, float* 
                      __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
 }
 
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
 // Row tiles of a segment that have rows.
 __device__ __forceinline__ int n_row_tiles(const AttnParams& p, const Segment& g) {
   return static_cast<long long>(g.n_q) * p.group - g.row0 > p.tile_rows / 2 ? 2 : 1;
@@ -386,13 +393,13 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           fence_proxy_async_smem();                   // the tensor cores read it through the async proxy
         }
         if (warp_live) {
-          // Weights of 32 columns against `base`, packed; returns their sum.
+          // Weights of some columns against `base`, packed; returns their sum.
           float high = -INFINITY;
-          auto weigh = [&](const uint32_t (&sr)[32], float base, auto keep, auto by_hand, uint32_t* pk) -> f32x2_t {
+          auto weigh = [&](auto& sr, float base, auto keep, auto by_hand, uint32_t* pk) -> f32x2_t {
             const f32x2_t neg = pack2(kTileBias - base, kTileBias - base);
             f32x2_t acc = pack2(0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < static_cast<int>(sizeof(sr) / 8); ++i) {
               const float2 x = unpack2(ffma2(pack2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), scale2, neg));
               float2 w;
               if (by_hand(i)) w = exp2_by_polynomial(x.x, x.y, &high);
@@ -426,16 +433,17 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           }
           if (!done) {
             const int col_end = live ? limit - first : kHalfKeys;    // columns below it are visible
+            // (16 columns at a time: this path is taken once or twice an item, and its instructions have to be fetched)
             float top = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-              uint32_t sr[32];
-              tmem_ld32(t_sh + 32 * c, sr);
+            for (int c = 0; c < kHalfKeys; c += 16) {
+              uint32_t sr[16];
+              tmem_ld16(t_sh + c, sr);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
+              for (int i = 0; i < 16; ++i) {
                 const float x = __uint_as_float(sr[i]) * p.score_scale;
-                if (32 * c + i < col_end) top = fmaxf(top, x);
+                if (c + i < col_end) top = fmaxf(top, x);
               }
             }
             const bool need = top > m + (attempt ? kTileRefusedLazy : kTileLazy) || (m == -INFINITY && top > m);
@@ -448,13 +456,13 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 const float back = need ? ex2(m - top) : 1.0f;
                 l *= back;
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                  uint32_t orr[32];
-                  tmem_ld32(t_o + 32 * c, orr);
+                for (int c = 0; c < D; c += 16) {
+                  uint32_t orr[16];
+                  tmem_ld16(t_o + c, orr);
                   tc_wait_ld();
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * back);
-                  tmem_st32(t_o + 32 * c, orr);
+                  for (int i = 0; i < 16; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * back);
+                  tmem_st16(t_o + c, orr);
                 }
               }
               if (need) m = top;
@@ -462,15 +470,15 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             settled = !__any_sync(0xffffffffu, m == -INFINITY);
             const float base = m == -INFINITY ? 0.0f : m;            // (a row that has seen nothing yet)
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {             // (P of these columns goes where columns before them were)
-              uint32_t sr[32], pk[16];
-              tmem_ld32(t_sh + 32 * c, sr);
+            for (int c = 0; c < kHalfKeys; c += 16) {                // (P of these columns goes where columns before them were)
+              uint32_t sr[16], pk[8];
+              tmem_ld16(t_sh + c, sr);
               tc_wait_ld();
               const float2 a = unpack2(weigh(sr, base, [&](int i, float* w) {
-                if (32 * c + i >= col_end) *w = 0.0f;
+                if (c + i >= col_end) *w = 0.0f;
               }, [](int) { return false; }, pk));
               l += a.x + a.y;
-              tmem_st16(t_sh + 16 * c, pk);
+              tmem_st8(t_sh + c / 2, pk);
             }
           }
           tc_wait_st();
