@@ -136,17 +136,17 @@ int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t t
   const int64_t rows = std::min(max_q, tokens) * group;
   plan->tensor = rows > 32;
   plan->tile_rows = plan->tensor ? 2 * (kTileM / group) * group : rows <= 16 ? 16 : 32;
-  // Steps.  With few rows a key tile costs the same whatever the rows; on tensor cores, us per key tile with one / two row
-  // tiles: D=128 1.64 / 2.07, D=64 1.37 / 1.80.
-  // What the start and end of an item cost, in key tiles.  us of the attention kernel with 0 / 1 / 2 / 3: 64 sequences of 60 to
-  // 16000 keys, a token each, 157 / 148 / 150 / 152; 32 of 500 to 6000, 3 to 5 tokens (32 rows) 94 / 88 / 81 / 78; chunks of
-  // prompts (128 rows) 244 / 235 / 223 / 222; 128 sequences of 1 to 1000 keys, a token each, 47 / 40 / 40 / 43.
+  // Steps.  With few rows a key tile costs the same whatever the rows.  On tensor cores a key tile with one / two row tiles takes, D=128,
+  // 1.64 / 2.07 us, D=64 1.37 / 1.80; us of chunks of prompts next to single tokens, the costs taken as 2 to 5 / 3 to 5 / 4 to 5 /
+  // 5 to 5 / 3 to 4: 246 / 179 / 165 / 170 / 162.  The start and end of an item, in key tiles (0 / 1 / 2 / 3): 16 rows, 64 sequences of 60 to
+  // 16000 keys, 147 / 147 / 149 / 150, 128 of 1 to 1000 37 / 30 / 32 / 35; 32 rows, 32 sequences of 500 to 6000 keys, 2 / 3 / 4:
+  // 68 / 70 / 72.
   if (plan->tensor) {
-    plan->item_cost = 12;
-    plan->tile_cost = 5;
-    plan->light_cost = 4;
+    plan->item_cost = 10;
+    plan->tile_cost = 4;
+    plan->light_cost = 3;
   } else {
-    plan->item_cost = plan->tile_rows == 16 ? 1 : 3;
+    plan->item_cost = plan->tile_rows == 16 ? 1 : 2;
   }
   const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
   const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
@@ -311,6 +311,7 @@ int sage_paged_attn(const sage_paged_kv_t* cache, const sage_paged_batch_t* batc
   p.zero_rest = zero_rest != 0;
   p.score_scale = sm_scale * 1.4426950408889634f;
   p.wait_limit_cycles = g_wait_limit_cycles.load(std::memory_order_relaxed);
+  p.test_drop_load = g_test_drop_v_load.load(std::memory_order_relaxed) != 0 && p.wait_limit_cycles < sage::kWaitLimitCycles;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   if (n_shared == 0) return dispatch_pass(cache, p, plan.own, ws, st);

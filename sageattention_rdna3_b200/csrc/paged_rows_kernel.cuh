@@ -181,7 +181,8 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         if (!ok) break;
         uint8_t* dst = smem + stage * L::kStage;
         const int checked = checked_page(p, pages);
-        if (leader) mbar_arrive_expect_tx(full + stage, boxes * box_rows * D * 2 * 2);
+        if (p.test_drop_load && tiles == 0) boxes = 0;                       // failure-detection test: this stage never fills
+        else if (leader) mbar_arrive_expect_tx(full + stage, boxes * box_rows * D * 2 * 2);
 #pragma unroll 1
         for (int x = 0; x < boxes; ++x) {
           const int page = __shfl_sync(0xffffffffu, checked, x);

@@ -1,12 +1,14 @@
 // How attention over a paged cache is cut into work for a fixed grid, without the host knowing a length.
 //
 // An item is one row tile of one kv head of one sequence: up to `tile_rows` rows (new token, query head of the group) that
-// read the same keys.  Its steps are tiles of 128 keys, at least one (an item without keys writes zeros), behind `item_cost` more that
-// stand for its start and end.  The steps of all items, after sequence, kv head after kv head, row tile after row tile, form one line that is cut into equal spans, one per CTA:
-// lengths may differ as they like and all CTAs get the same amount of work.  A key tile belongs to the CTA that has its first step.  A span that covers part of an item leaves
-// its result in a slot of the workspace (slot 1 the head of an item, slot 0 anything else: at most one of each per
-// CTA) and a header that tells the merge kernels which parts follow.  Every CTA works this out for itself from kv_lens and
-// cu_q, by a block-wide prefix sum; nothing is communicated and the order of all sums is fixed.
+// read the same keys, those up to the last key that its last token sees.  It costs `item_cost` steps for its start and end
+// and then some per tile of 128 keys (at least one tile: an item without keys writes zeros).  The steps of all items, sequence
+// after sequence, kv head after kv head, row tile after row tile, form one line that is cut into equal spans, one per CTA:
+// lengths may differ as they like and all CTAs get the same amount of work.  A key tile belongs to the CTA that has its first
+// step.  A span that covers part of an item leaves its result in a slot of the workspace (slot 1 the head of an item, slot 0
+// anything else: at most one of each per CTA) and a header that tells the merge kernels which parts follow.  Every CTA works
+// this out for itself from kv_lens and cu_q, by a block-wide prefix sum; nothing is communicated and the order of all sums is
+// fixed.
 #pragma once
 
 #include "paged_common.cuh"
@@ -72,6 +74,7 @@ struct AttnParams {
   float* part_e;                // [grid][2][tile rows]
   struct PartHeader* headers;   // [grid]
   long long wait_limit_cycles;
+  int test_drop_load;           // test hook: one load of the first key tile is left out
 };
 
 struct PartHeader {             // of the part in slot 1 of a CTA, if it is the head of an item that others finish

@@ -321,7 +321,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         pages = checked_page(p, pages);
         load(&tm_k, s_k + s * L::kKVBytes, k_full + s, g.kv_head);
         SAGE_PAGED_WARP_WAIT_OR(true, v_empty + s, ((kt / kStages) & 1) ^ 1u, 21, { ok = false; break; });
-        load(&tm_v, s_v + s * L::kKVBytes, v_full + s, g.kv_head);
+        if (!(p.test_drop_load && kt == 0)) load(&tm_v, s_v + s * L::kKVBytes, v_full + s, g.kv_head);   // (failure-detection test)
         if (j + 1 < g.n_tiles) find_pages(g, j + 1);  // (they arrive while the stage is waited for)
       }
     }

@@ -377,6 +377,116 @@ def test_a_prompt_and_its_answer(layout):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_len", [1, 60])
+def test_many_sequences(q_len):
+    """More sequences than a block has threads, some of them without new tokens or without keys."""
+    dev = torch.device("cuda")
+    n = 700
+    q_lens = [q_len if i == 300 else (i % 3 if q_len > 1 else 1) for i in range(n)]
+    kv_lens = [m + (7 * i) % 61 if i % 11 else m for i, m in enumerate(q_lens)]
+    batch = PagedBatch(q_lens, kv_lens, 4, 1, 64, 16, "NHD", F16, dev)
+    o, lse = run(batch)
+    compare(batch, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_len", [1, 5, 150])
+def test_result_over_q_and_a_cache_of_one_page(q_len):
+    """out may be q itself: a row of it is read by the CTAs that write it, and only before they do."""
+    dev = torch.device("cuda")
+    batch = PagedBatch([q_len] * 4, [q_len + 900 * i for i in range(4)], 8, 2, 128, 16, "HND", BF16, dev)
+    table, lens = batch.args()
+    cu = batch.cu_q()
+    want = sageattn_paged(batch.q.to(dev), batch.cache(), table, lens, cu_q=cu)
+    q = batch.q.to(dev)
+    assert sageattn_paged(q, batch.cache(), table, lens, cu_q=cu, out=q) is q
+    assert torch.equal(q, want)
+    for Hkv in (1, 2):
+        one = PagedBatch([min(q_len, 200)], [200], 4, Hkv, 64, 256, "NHD", F16, dev, spare=0)
+        assert one.n_pages == 1
+        o, lse = run(one)
+        compare(one, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_offsets_beyond_32_bits(layout):
+    """A cache of more than 2^31 values, the sequences in its last pages."""
+    dev = torch.device("cuda")
+    page, Hkv, D = 256, 8, 128
+    n_pages = 2 ** 31 // (page * Hkv * D) + 40
+    shape = (n_pages, Hkv, page, D) if layout == "HND" else (n_pages, page, Hkv, D)
+    k_pages, v_pages = (torch.empty(shape, dtype=BF16, device=dev) for _ in range(2))
+    cache = PagedKV(k_pages, v_pages, layout)
+    batch = PagedBatch([1, 70], [600, 1000], 16, Hkv, D, page, layout, BF16, dev)
+    table, lens = batch.args()
+    moved = table.clone()
+    used = batch.n_pages
+    for b, c in enumerate(batch.counts):
+        moved[b, :c] += n_pages - used
+    k_pages[n_pages - used:], v_pages[n_pages - used:] = batch.k_pages.to(dev), batch.v_pages.to(dev)
+    o, lse = sageattn_paged(batch.q.to(dev), cache, moved, lens, cu_q=batch.cu_q(), return_lse=True)
+    check_status(dev)
+    compare(batch, o, lse)
+    # and what is appended goes there too
+    k, v = (H.randn((71, Hkv, D), s, BF16, dev) for s in (1, 2))
+    paged_kv_append(cache, k, v, moved, lens, cu_q=batch.cu_q())
+    check_status(dev)
+    t = 0
+    for b, m in enumerate(batch.q_lens):
+        for j in range(batch.kv_lens[b] - m, batch.kv_lens[b]):
+            pid, slot = int(moved[b, j // page]), j % page
+            at = (pid, slice(None), slot) if layout == "HND" else (pid, slot)
+            if t % 10 == 0:
+                assert torch.equal(k_pages[at], k[t]) and torch.equal(v_pages[at], v[t])
+            t += 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_len", [1, 7, 60])
+def test_a_wait_that_runs_out_is_reported(q_len):
+    """A load that never comes (the test hook leaves it out): the kernel ends after its bound with a status, the next call says
+    so, and the one after that works."""
+    lib = _native.load_abi()
+    dev = torch.device("cuda")
+    batch = PagedBatch([q_len] * 3, [q_len + 500] * 3, 4, 2, 128, 16, "NHD", F16, dev)
+    table, lens = batch.args()
+    args = (batch.q.to(dev), batch.cache(), table, lens)
+    want = sageattn_paged(*args, cu_q=batch.cu_q(), max_q=q_len)
+    check_status(dev)
+    lib.sage_test_set_wait_limit_us(20000)
+    lib.sage_test_drop_v_load(1)
+    try:
+        sageattn_paged(*args, cu_q=batch.cu_q(), max_q=q_len)
+        torch.cuda.synchronize()
+    finally:
+        lib.sage_test_drop_v_load(0)
+        lib.sage_test_set_wait_limit_us(0)
+    with pytest.raises(RuntimeError, match="device status.*call after"):
+        sageattn_paged(*args, cu_q=batch.cu_q(), max_q=q_len)
+    assert torch.equal(sageattn_paged(*args, cu_q=batch.cu_q(), max_q=q_len), want)
+    check_status(dev)
+
+
+@pytest.mark.gpu
+def test_checked_at_once_if_asked(monkeypatch):
+    monkeypatch.setenv("SAGEATTN_B200_CHECK_STATUS", "1")
+    dev = torch.device("cuda")
+    batch = PagedBatch([1, 1], [20, 30], 4, 2, 64, 16, "NHD", F16, dev)
+    cache, (table, lens) = batch.cache(), batch.args()
+    o, lse = run(batch)
+    compare(batch, o, lse)
+    table[0, 0] = -1
+    with pytest.raises(RuntimeError, match="device status 3"):
+        sageattn_paged(batch.q.to(dev), cache, table, lens)
+    k = H.randn((2, 2, 64), 1, F16, dev)
+    table[0, 1] = -1
+    with pytest.raises(RuntimeError, match="device status 3"):
+        paged_kv_append(cache, k, k, table, lens)
+    check_status(dev)
+
+
+@pytest.mark.gpu
 def test_another_device_than_the_current_one():
     if torch.cuda.device_count() < 2:
         pytest.skip("needs a second GPU")
