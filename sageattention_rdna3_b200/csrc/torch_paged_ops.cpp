@@ -1,14 +1,17 @@
 // torch.ops.sageattention.* of the operators around a growing cache: a thin wrapper that turns tensors into the pointers,
 // sizes and strides of include/sage_paged_b200.h.
 #include <Python.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 #include <torch/types.h>
@@ -49,7 +52,7 @@ void check_vectors(const at::Tensor& t, const char* name) {
 }
 
 void check_int32(const at::Tensor& t, const at::Tensor& like, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kInt && t.device() == like.device() && t.stride(-1) == 1, name,
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.device() == like.device() && (t.size(-1) <= 1 || t.stride(-1) == 1), name,
               " must be an int32 tensor on the device of the cache with a contiguous last dim");
 }
 
@@ -276,6 +279,11 @@ void paged_attn(const at::Tensor& q, at::Tensor& o, const at::Tensor& k_pages, c
   check_rows(q, k_pages, -1, "query");
   check_rows(o, k_pages, q.size(1), "output");
   TORCH_CHECK(o.size(0) == q.size(0), "query and output differ in length");
+  // Each row of q is read by the thread blocks that write the same row of o and no others: o may be q, but not a shifted q.
+  at::assert_no_internal_overlap(o);
+  at::assert_no_partial_overlap(o, q);
+  at::assert_no_overlap(o, k_pages);
+  at::assert_no_overlap(o, v_pages);
   const sage_paged_batch_t batch = batch_of(page_table, kv_lens, cu_q, q.size(0), k_pages);
   const int Hq = size_of(q.size(1), "heads"), longest = size_of(max_q, "max_q");
   int n_shared = 0;
@@ -336,7 +344,7 @@ bool plain(PyObject* o, const at::Tensor** out, bool none = false) {
   if (!THPVariable_CheckExact(o)) return false;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (at::isTensorSubclassLike(t) || t.layout() != at::kStrided || !t.is_cuda() || t.unsafeGetTensorImpl()->has_symbolic_sizes_strides() ||
-      t.is_neg() || t.is_conj()) {
+      t.is_neg() || t.is_conj() || torch::autograd::isFwGradDefined(t)) {
     return false;
   }
   *out = &t;
@@ -359,6 +367,8 @@ bool vectors(const at::Tensor& t) {
   }
   return true;
 }
+
+at::Tensor new_like(const at::Tensor& t) { return at::detail::empty_cuda(t.sizes(), t.scalar_type(), t.device(), c10::nullopt); }
 
 bool needs_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
@@ -458,8 +468,8 @@ PyObject* sage_rotary_plain(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
   } else {
     pybind11::gil_scoped_release no_gil;
     c10::cuda::CUDAGuard guard(q->device());
-    qo = at::empty(q->sizes(), q->options());
-    if (k != nullptr) ko = at::empty(k->sizes(), k->options());
+    qo = new_like(*q);
+    if (k != nullptr) ko = new_like(*k);
     const sage_strided_t qs = strided_of(*q, layout), qos = strided_of(qo, layout);
     sage_strided_t ks{}, kos{};
     if (k != nullptr) {
@@ -517,7 +527,7 @@ PyObject* sage_paged_append_plain(PyObject*, PyObject* const* args, Py_ssize_t n
     const sage_paged_batch_t batch = batch_of(*table, *lens, cu != nullptr ? c10::optional<at::Tensor>(*cu) : c10::nullopt, T, *kp);
     sage_rows_t qs{}, qo{};
     if (q != nullptr) {
-      out = at::empty(q->sizes(), q->options());
+      out = new_like(*q);
       qs = rows_of(*q);
       qo = rows_of(out);
     }
@@ -558,8 +568,8 @@ PyObject* sage_paged_attn_plain(PyObject*, PyObject* const* args, Py_ssize_t nar
     const sage_paged_kv_t cache = cache_of(*kp, *vp, layout);
     const sage_paged_batch_t batch = batch_of(*table, *lens, cu != nullptr ? c10::optional<at::Tensor>(*cu) : c10::nullopt, T, *kp);
     const int heads = size_of(Hq, "heads"), n_shared = shared != nullptr ? size_of(shared->size(0), "shared pages") : 0;
-    out = at::empty(q->sizes(), q->options());
-    if (want_lse) lse = at::empty({T, Hq}, q->options().dtype(at::kFloat));
+    out = new_like(*q);
+    if (want_lse) lse = at::detail::empty_cuda({T, Hq}, at::kFloat, q->device(), c10::nullopt);
     const int64_t bytes = sage_paged_workspace_bytes(&cache, &batch, heads, max_q, n_shared);
     TORCH_CHECK(bytes >= 0, "paged_attn failed: ", sage_last_error());
     const c10::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes));

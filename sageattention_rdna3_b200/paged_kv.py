@@ -40,6 +40,7 @@ class PagedKV:
         assert k.dim() == 4 and k.shape == v.shape, "k_pages and v_pages must be 4-D tensors of the same shape."
         assert k.dtype == v.dtype and k.dtype in (torch.float16, torch.bfloat16), "pages must both be fp16 or bf16."
         assert k.device == v.device, "k_pages and v_pages must be on the same device."
+        assert not (k.requires_grad or v.requires_grad), "pages must not require a gradient: the paged cache has none."
         assert self.head_dim in (64, 128), f"head_dim must be 64 or 128, got {self.head_dim}."
         assert self.page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}, got {self.page_size}."
         assert k.size(0) > 0 and self.num_kv_heads > 0, "the cache needs a page and a head."
@@ -189,7 +190,8 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
     rounding.
 
     Returns ``[T, Hq, D]``, with ``return_lse`` also the natural log-sum-exp ``[T, Hq]`` (fp32).  Rows that belong to no sequence are
-    zero (-inf); given ``out``, which receives the result, they are left as they were there.  Keys and values behind a
+    zero (-inf); given ``out``, which receives the result, they are left as they were there.  ``out`` may be ``q``, but must not
+    overlap it otherwise, nor the cache.  Keys and values behind a
     sequence's last one may be anything, NaN too.  Lengths beyond the page table are cut to it, page indices
     outside the cache are read as page 0, and both are reported like the errors of ``sageattn``, by the next call or
     ``check_status()``.  No gradient."""
@@ -215,8 +217,8 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
         assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, (
             "out must have the shape, dtype and device of q.")
         assert out.stride(2) == 1 and out.data_ptr() % 16 == 0 and all(
-            n <= 1 or s % 8 == 0 for n, s in zip(out.shape[:2], out.stride()[:2])), (
-            f"out needs a contiguous last dim and 16-byte aligned rows; got strides {out.stride()}.")
+            n <= 1 or (s % 8 == 0 and s > 0) for n, s in zip(out.shape[:2], out.stride()[:2])), (
+            f"out needs a contiguous last dim, 16-byte aligned rows and a place for every row; got strides {out.stride()}.")
     assert dev.type == "cuda", "the cache must be on a CUDA device."
     ops = _native.load_ops()
     _raise_pending(dev)

@@ -183,6 +183,8 @@ def test_refused_caches():
             PagedKV(k, v)
     with pytest.raises(AssertionError):
         PagedKV(ok, ok, "BSHD")
+    with pytest.raises(AssertionError, match="gradient"):
+        PagedKV(ok, ok.clone().requires_grad_())
 
 
 class SagePagedKV(ctypes.Structure):

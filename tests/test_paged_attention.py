@@ -409,6 +409,33 @@ def test_result_over_q_and_a_cache_of_one_page(q_len):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("short_way", [True, False])
+def test_lengths_that_are_a_column(short_way):
+    dev = torch.device("cuda")
+    cache = PagedKV(*(torch.randn(4, 16, 2, 64, device=dev).to(F16) for _ in range(2)))
+    q = torch.randn(1, 4, 64, device=dev).to(F16)
+    table = torch.arange(4, dtype=torch.int32, device=dev)[None]
+    lens = torch.tensor([[50, 7]], dtype=torch.int32, device=dev)
+    out = None if short_way else torch.empty_like(q)
+    got = sageattn_paged(q, cache, table, lens[:, 0], out=out)          # one element, a stride of two
+    assert torch.equal(got, sageattn_paged(q, cache, table, lens[:, 0].contiguous()))
+
+
+@pytest.mark.gpu
+def test_results_that_overlap_are_refused():
+    dev = torch.device("cuda")
+    cache = PagedKV.allocate(4, 16, 2, 64, dtype=F16)
+    table, lens = torch.zeros(3, 2, dtype=torch.int32, device=dev), torch.ones(3, dtype=torch.int32, device=dev)
+    rows = torch.zeros(4, 4, 64, dtype=F16, device=dev)
+    for q, out in ((rows[:3], rows[1:]), (rows[:3], cache.k_pages.view(-1, 4, 64)[:3]), (rows[:3], cache.v_pages.view(-1, 4, 64)[5:8])):
+        with pytest.raises(RuntimeError, match="memory"):
+            sageattn_paged(q, cache, table, lens, out=out)
+    with pytest.raises(AssertionError, match="every row"):
+        sageattn_paged(rows[:3], cache, table, lens, out=rows[:1].expand(3, 4, 64))
+    check_status(dev)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["NHD", "HND"])
 def test_offsets_beyond_32_bits(layout):
     """A cache of more than 2^31 values, the sequences in its last pages."""
