@@ -130,7 +130,7 @@ def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table
     Rows that belong to no sequence (T may be padded) are not stored, and zero in the returned q.  A page index
     outside the cache, a position outside the page table or more new tokens than ``kv_lens`` says are not stored either; they
     are reported like the errors of ``sageattn``, by the next call or ``check_status()``.  Two sequences that share a page
-    must not append to it at once."""
+    must not append to it at once, and k, v and q must not lie in the cache."""
     assert isinstance(cache, PagedKV), "cache must be a PagedKV."
     assert rotary is None or (isinstance(rotary, RotaryAxes) and rotary.head_dim == cache.head_dim), (
         "rotary must come from rotary_axes() with the head_dim of the cache.")
