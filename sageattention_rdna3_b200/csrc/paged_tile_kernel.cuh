@@ -272,18 +272,19 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     SegmentIter it(p, span);
     int kt = 0;
     bool ok = true;
-    int first = 0, boxes = 0, pages = 0;              // of the next tile: first key, boxes; lane i holds the page of box i
-    auto find_pages = [&](const Segment& g, int j) {
-      first = g.key0 + j * kTileKeys;
-      const int keys = min(max(g.len - first, 0), kTileKeys);
-      boxes = (keys + box_rows - 1) / box_rows;
-      pages = lane < boxes ? page_of_key(p, g.b, first + lane * box_rows) : 0;
+    // Pages are looked up 32 at a time, as by the few rows' producer.
+    const int block_tiles = 32 * box_rows / kTileKeys;
+    int first = 0, boxes = 0, at_box = 0;             // of the tile at hand: first key, boxes, the first one's place among the pages at hand
+    int pages = 0, checked = 0;
+    auto find_pages = [&](const Segment& g, int j) {  // from tile j on
+      const int key = g.key0 + j * kTileKeys + lane * box_rows;
+      if (key < g.len) pages = page_of_key(p, g.b, key);
     };
     auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int head) {
       if (leader) mbar_arrive_expect_tx(bar, boxes * box_rows * D * 2);
 #pragma unroll 1
       for (int i = 0; i < boxes; ++i) {
-        const int id = __shfl_sync(0xffffffffu, pages, i);
+        const int id = __shfl_sync(0xffffffffu, checked, at_box + i);
         if (leader) {
 #pragma unroll
           for (int c = 0; c < kSlabs; ++c) tma_load_4d(dst + c * L::kSlab + i * box_rows * 128, map, bar, c * 64, first & slot_mask, head, id);
@@ -318,11 +319,17 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       for (int j = 0; j < g.n_tiles; ++j, ++kt) {
         const int s = kt % kStages;
         SAGE_PAGED_WARP_WAIT_OR(true, k_empty + s, ((kt / kStages) & 1) ^ 1u, 23, { ok = false; break; });
-        pages = checked_page(p, pages);
+        const int in_block = j & (block_tiles - 1);
+        if (in_block == 0) {
+          checked = checked_page(p, pages);
+          if (j + block_tiles < g.n_tiles) find_pages(g, j + block_tiles);
+        }
+        first = g.key0 + j * kTileKeys;
+        boxes = (min(max(g.len - first, 0), kTileKeys) + box_rows - 1) / box_rows;
+        at_box = in_block * kTileKeys / box_rows;
         load(&tm_k, s_k + s * L::kKVBytes, k_full + s, g.kv_head);
         SAGE_PAGED_WARP_WAIT_OR(true, v_empty + s, ((kt / kStages) & 1) ^ 1u, 21, { ok = false; break; });
         if (!(p.test_drop_load && kt == 0)) load(&tm_v, s_v + s * L::kKVBytes, v_full + s, g.kv_head);   // (failure-detection test)
-        if (j + 1 < g.n_tiles) find_pages(g, j + 1);  // (they arrive while the stage is waited for)
       }
     }
     __syncwarp();
