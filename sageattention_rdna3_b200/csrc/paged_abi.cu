@@ -138,15 +138,17 @@ int plan_pass(PagedPlan* plan, const sage_paged_kv_t* c, int64_t seqs, int64_t t
   plan->tile_rows = plan->tensor ? 2 * (kTileM / group) * group : rows <= 16 ? 16 : 32;
   // Steps.  With few rows a key tile costs the same whatever the rows.  On tensor cores a key tile with one / two row tiles takes, D=128,
   // 1.64 / 2.07 us, D=64 1.37 / 1.80; us of chunks of prompts next to single tokens, the costs taken as 2 to 5 / 3 to 5 / 4 to 5 /
-  // 5 to 5 / 3 to 4: 246 / 179 / 165 / 170 / 162.  The start and end of an item, in key tiles (0 / 1 / 2 / 3): 16 rows, 64 sequences of 60 to
-  // 16000 keys, 147 / 147 / 149 / 150, 128 of 1 to 1000 37 / 30 / 32 / 35; 32 rows, 32 sequences of 500 to 6000 keys, 2 / 3 / 4:
-  // 68 / 70 / 72.
+  // 5 to 5 / 3 to 4: 246 / 179 / 165 / 170 / 162.  With few rows the start and end of an item take a key
+  // tile for every 8 rows, which the warps join one after the other (the most rows that an item may have: counted for every item by the
+  // device the small calls lost 0.1 to 1.7 us).  us for 0 / 1 / 2 key tiles, 4 rows, 64 sequences of 60 to 16000 keys:
+  // 137 / 125 / 126; for 1 / 2 / 3 / 4, 12 to 20 rows, 32 sequences of 500 to 6000 keys: 70 / 66 / 64 / 66; for 2 / 3 / 4, 24 rows, 128 sequences
+  // of up to 800: 92 / 84 / 86, 32 rows, 64 sequences of 50 to 3000: 115 / 104 / 98.
   if (plan->tensor) {
     plan->item_cost = 10;
     plan->tile_cost = 4;
     plan->light_cost = 3;
   } else {
-    plan->item_cost = plan->tile_rows == 16 ? 1 : 2;
+    plan->item_cost = static_cast<int>((rows + 7) / 8);
   }
   const int64_t tiles = std::max<int64_t>(1, (max_keys + kTileKeys - 1) / kTileKeys);
   const int64_t row_tiles = tokens * group / plan->tile_rows + seqs;
