@@ -46,8 +46,9 @@ const char* sage_last_error(void);
 /* The `status` word of the attention entry points (optional, a device int32 the caller zeroes):
  * the kernels write a non-zero code there when they had to give up (1 = shared memory misaligned,
  * 2 + 16*k = the bounded wait on barrier k ran out) and return instead of hanging; CTAs that start
- * while the word is already non-zero return at once, so a failed launch costs about one wait bound
- * and later launches do nothing until the caller has read and cleared the word.  With status ==
+ * while the word holds such a code return at once, so a failed launch costs about one wait bound
+ * and later launches do nothing until the caller has read and cleared the word.  (The codes of refused
+ * arguments in sage_paged_b200.h stop no launch.)  With status ==
  * NULL such a failure goes unreported and the output is left partly unwritten.  The reference has
  * no counterpart (its launchers check nothing after the launch, csrc/attn_gfx11.cu:2069-2273).
  *

@@ -18,7 +18,8 @@ extern "C" {
 
 #define SAGE_DTYPE_F32 2             /* sage_apply_rotary only */
 
-/* Status codes that the kernels of this file write, next to those of sage_b200.h. */
+/* Status codes that the kernels of this file write, next to those of sage_b200.h: arguments of one call.  Unlike those they
+ * stop neither the call nor one behind it. */
 #define SAGE_STATUS_BAD_PAGE 3       /* a page index outside the cache */
 #define SAGE_STATUS_BAD_LENGTH 4     /* more keys than the row of the page table holds, or more new tokens than keys */
 

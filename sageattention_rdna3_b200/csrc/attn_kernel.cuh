@@ -402,10 +402,10 @@ sage_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     tmem_relinquish();
   }
   if (threadIdx.x == 0) {
-    // A status word that is already set means an earlier CTA of this launch (or an earlier launch
+    // A code in the status word may mean that an earlier CTA of this launch (or an earlier launch
     // the caller has not looked at yet) gave up: this CTA leaves through the abort path at once, so a
     // failing launch costs about one wait bound and not one per wave of CTAs.
-    *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
+    *abort_flag = (p.status != nullptr && status_stops(*reinterpret_cast<volatile int*>(p.status))) ? 1 : 0;
     *fail_code = 0;
   }
   if (warp == 4 && elect_one()) {        // the same thread as above: elect.sync is deterministic

@@ -125,7 +125,7 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   if (threadIdx.x == kRowsThreads - 1) {               // (a thread that has no sequence to look up, as a rule)
     // a wait of an earlier launch that ran out and was not looked at yet: this launch does nothing (as attn_kernel.cuh)
     const int before = p.status.word != nullptr ? *reinterpret_cast<volatile int*>(p.status.word) : 0;
-    *abort_flag = misaligned || (before & 15) == 2;
+    *abort_flag = misaligned || status_stops(before);
     if (misaligned) p.status.report(kStatusMisaligned);
     p.headers[blockIdx.x].n_parts = 0;
   }

@@ -159,7 +159,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   }
   if (threadIdx.x == kTileThreads - 1) {               // (a thread that has no sequence to look up, as a rule)
     const int before = p.status.word != nullptr ? *reinterpret_cast<volatile int*>(p.status.word) : 0;
-    *abort_flag = misaligned || (before & 15) == 2;
+    *abort_flag = misaligned || status_stops(before);
     *fail_code = 0;
     if (misaligned) p.status.report(kStatusMisaligned);
     p.headers[blockIdx.x].n_parts = 0;

@@ -144,7 +144,7 @@ sage_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     tmem_relinquish();
   }
   if (threadIdx.x == 0) {
-    *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
+    *abort_flag = (p.status != nullptr && status_stops(*reinterpret_cast<volatile int*>(p.status))) ? 1 : 0;
     *fail_code = 0;
   }
   tc_fence_before();

@@ -14,6 +14,10 @@
 
 namespace sage {
 
+// Codes in the status word of a device.  A launch that gave up (1, or 2 + 16 * wait) stops those behind it until the host has looked;
+// arguments that one call refused (3, 4: pages and lengths of a paged cache) concern no other.
+__device__ __forceinline__ bool status_stops(int code) { return code != 0 && code != 3 && code != 4; }
+
 // About one second at 1.9 GHz; a whole attention launch is a few milliseconds.
 constexpr long long kWaitLimitCycles = 2000000000LL;
 

@@ -1,0 +1,72 @@
+"""Edges of the operators around a growing cache: what one call leaves for another, rows that see nothing, slots that are not in
+use, results that overlap, and calls that come with more of autograd than the cache has."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+import helpers as H
+from paged_helpers import PagedBatch
+from sageattention_rdna3_b200 import (PagedKV, _native, apply_rotary, check_status, core, paged_kv_append, rotary_axes, sageattn,
+                                      sageattn_paged)
+from test_paged_attention import compare
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def clear_status(dev):
+    torch.cuda.synchronize()
+    core._status_word(dev).zero_()
+    core._status_mirror(dev)[1][0] = 0
+    torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------- what one call leaves for another
+
+# head_dim, heads, length, kernel: plain, persistent and paired launches of both kernels
+SAGEATTN_CALLS = [(64, 2, 200, "int8"), (128, 2, 200, "direct"), (128, 20, 4000, "int8"), (64, 10, 4096, "int8"), (128, 148, 1280, "direct")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", [3, 4])
+@pytest.mark.parametrize("case", SAGEATTN_CALLS, ids=[str(i) for i in range(len(SAGEATTN_CALLS))])
+def test_a_page_code_stops_no_other_call(case, code):
+    """A bad page of one call (the host has not seen it yet) leaves what runs behind it alone."""
+    D, heads, n, kernel = case
+    dev = torch.device("cuda", 0)
+    q, k, v = (H.randn((1, heads, n, D), s, F16, dev) for s in (1, 2, 3))
+    want = torch.empty_like(q)
+    sageattn(q, k, v, kernel=kernel, out=want)
+    check_status(dev)
+    got = torch.full_like(q, 7.0)
+    core._status_word(dev).fill_(code)
+    try:
+        sageattn(q, k, v, kernel=kernel, out=got)
+        torch.cuda.synchronize()
+        assert int(core._status_word(dev)) == code and int(core._status_mirror(dev)[1][0]) == 0
+    finally:
+        clear_status(dev)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_sageattn_behind_a_bad_page():
+    """As a program meets it: the append and the call behind it are both in the stream before the first has run."""
+    dev = torch.device("cuda", 0)
+    cache = PagedKV.allocate(4, 16, 2, 64, dtype=F16)
+    table, lens = torch.full((3, 1), 99, dtype=torch.int32, device=dev), torch.ones(3, dtype=torch.int32, device=dev)
+    rows = torch.ones(3, 2, 64, dtype=F16, device=dev)
+    q = H.randn((1, 2, 300, 64), 1, F16, dev)
+    want = torch.empty_like(q)
+    sageattn(q, q, q, out=want, kernel="int8")
+    check_status(dev)
+    got = torch.full_like(q, 7.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_kv_append(cache, rows, rows, table, lens)
+        sageattn(q, q, q, out=got, kernel="int8")
+    got.fill_(7.0)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="device status 3"):
+        check_status(dev)
+    assert torch.equal(got, want)
+    check_status(dev)
