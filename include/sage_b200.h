@@ -53,8 +53,8 @@ const char* sage_last_error(void);
  * no counterpart (its launchers check nothing after the launch, csrc/attn_gfx11.cu:2069-2273).
  *
  * sage_set_status_mirror: a word in MAPPED PINNED HOST memory (cudaHostAlloc; the pointer must be
- * usable on the current device) that a failing attention kernel of the current device also writes
- * its code to, next to the `status` word of the call.  A host that never synchronises can poll it
+ * usable on the current device) that receives what the `status` word of a failing call on the
+ * current device then holds.  A host that never synchronises can poll it
  * between calls.  NULL switches the mirror off.  Kernels launched without a `status` word do not
  * write it.  No counterpart in the reference.
  *

@@ -19,7 +19,7 @@ extern "C" {
 #define SAGE_DTYPE_F32 2             /* sage_apply_rotary only */
 
 /* Status codes that the kernels of this file write, next to those of sage_b200.h: arguments of one call.  Unlike those they
- * stop neither the call nor one behind it. */
+ * stop neither the call nor one behind it, and give way to them in the word; otherwise the first code stays. */
 #define SAGE_STATUS_BAD_PAGE 3       /* a page index outside the cache */
 #define SAGE_STATUS_BAD_LENGTH 4     /* more keys than the row of the page table holds, or more new tokens than keys */
 

@@ -85,7 +85,7 @@ struct AttnParams {
   int lse_add;                  // 1: ... added to lse_add_scale times what `lse` holds
   float lse_add_scale;
   int* status;                  // optional device word, stays 0 on success
-  int* status_host;             // optional word in mapped pinned host memory that receives the same code
+  int* status_host;             // optional word in mapped pinned host memory that receives what `status` holds
   long long wait_limit_cycles;  // bound of every barrier wait, in SM clocks
   int test_drop_v_load;         // test hook: the producer never loads V of the first KV tile
   // Persistent ("stream-K") variant only: the (query tile, KV tile) steps of the whole problem are
@@ -315,7 +315,7 @@ sage_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 
   if ((smem_u32(smem) & 1023u) != 0u) {        // swizzled tiles need 1024-byte alignment
     grid_dependency_wait();
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kStatusSmemMisaligned);
+    if (threadIdx.x == 0) report_status(p.status, nullptr, kStatusSmemMisaligned);
     return;
   }
 
@@ -981,14 +981,7 @@ sage_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     // A wait gave up.  Let copies and MMAs that are still in flight land before the shared memory
     // and TMEM of this CTA are handed back, then report.
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
-    if (threadIdx.x == 0) {
-      const int code = *fail_code ? *fail_code : kStatusWaitTimeout;
-      if (p.status) atomicCAS(p.status, 0, code);
-      if (p.status_host) {              // the host can see the failure without synchronising
-        *reinterpret_cast<volatile int*>(p.status_host) = code;
-        __threadfence_system();
-      }
-    }
+    if (threadIdx.x == 0) report_status(p.status, p.status_host, *fail_code ? *fail_code : kStatusWaitTimeout);
     __syncthreads();
   }
   if (warp == 5) {

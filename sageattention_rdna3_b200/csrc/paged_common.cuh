@@ -35,16 +35,8 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* tmap, 
 
 struct Status {
   int* word;                    // optional device word, stays 0 on success
-  int* host;                    // optional word in mapped pinned host memory that receives the same code
-  __device__ __forceinline__ void report(int code) const {
-    if (word != nullptr) {
-      atomicCAS(word, 0, code);
-      if (host != nullptr) {
-        *reinterpret_cast<volatile int*>(host) = code;
-        __threadfence_system();
-      }
-    }
-  }
+  int* host;                    // optional word in mapped pinned host memory that receives what the device word holds
+  __device__ __forceinline__ void report(int code) const { report_status(word, host, code); }
 };
 
 struct Batch {

@@ -95,7 +95,7 @@ sage_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const int lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0u) {        // swizzled tiles need 1024-byte alignment
     grid_dependency_wait();
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kStatusSmemMisaligned);
+    if (threadIdx.x == 0) report_status(p.status, nullptr, kStatusSmemMisaligned);
     return;
   }
   uint8_t* s_q = smem + L::kOffQ;
@@ -516,14 +516,7 @@ sage_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   if (*abort_flag) {
     // As in sage_attn_kernel: copies and MMAs in flight land before shared memory and TMEM are handed back.
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
-    if (threadIdx.x == 0) {
-      const int code = *fail_code ? *fail_code : kStatusWaitTimeout;
-      if (p.status) atomicCAS(p.status, 0, code);
-      if (p.status_host) {
-        *reinterpret_cast<volatile int*>(p.status_host) = code;
-        __threadfence_system();
-      }
-    }
+    if (threadIdx.x == 0) report_status(p.status, p.status_host, *fail_code ? *fail_code : kStatusWaitTimeout);
     __syncthreads();
   }
   if (warp == 9) {

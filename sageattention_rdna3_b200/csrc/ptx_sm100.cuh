@@ -18,6 +18,25 @@ namespace sage {
 // arguments that one call refused (3, 4: pages and lengths of a paged cache) concern no other.
 __device__ __forceinline__ bool status_stops(int code) { return code != 0 && code != 3 && code != 4; }
 
+// Leaves a code in the status word of the device (optional) and in its mirror in mapped host memory (optional, only with a word).  The
+// first code stays, but one that stops launches takes the place of one that does not.  The mirror gets what the word holds:
+// whoever writes it looks at the word again afterwards, so that the last to write has seen the last code.
+inline __device__ __noinline__ void report_status(int* word, int* host, int code) {
+  if (word == nullptr) return;
+  int seen = atomicCAS(word, 0, code);
+  if (seen != 0 && status_stops(code) && !status_stops(seen)) atomicCAS(word, seen, code);
+  if (host == nullptr) return;
+  volatile int* held = word;
+  seen = *held;
+  for (int i = 0; i < 4; ++i) {                        // (a word changes twice, and once more if the host clears it meanwhile)
+    *reinterpret_cast<volatile int*>(host) = seen != 0 ? seen : code;
+    __threadfence_system();
+    const int now = *held;
+    if (now == seen) break;
+    seen = now;
+  }
+}
+
 // About one second at 1.9 GHz; a whole attention launch is a few milliseconds.
 constexpr long long kWaitLimitCycles = 2000000000LL;
 

@@ -70,3 +70,63 @@ def test_sageattn_behind_a_bad_page():
         check_status(dev)
     assert torch.equal(got, want)
     check_status(dev)
+
+
+@pytest.fixture
+def dropped_load():
+    """A wait that runs out, by the library's test hook."""
+    lib = _native.load_abi()
+    lib.sage_test_set_wait_limit_us(20000)
+    lib.sage_test_drop_v_load(1)
+    yield
+    lib.sage_test_drop_v_load(0)
+    lib.sage_test_set_wait_limit_us(0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [1, 60, "sageattn"])
+def test_a_wait_that_runs_out_is_not_hidden_by_a_page_code(what, dropped_load):
+    """The word keeps the more serious code, the mirror what the word holds, and the launch behind does nothing."""
+    dev = torch.device("cuda", 0)
+    word, mirror = core._status_word(dev), core._status_mirror(dev)[1]
+    if what == "sageattn":
+        q = H.randn((1, 2, 300, 128), 1, F16, dev)
+        call = lambda: sageattn(q, q, q, kernel="int8")                     # noqa: E731
+    else:
+        batch = PagedBatch([what] * 2, [what + 500] * 2, 4, 2, 128, 16, "NHD", F16, dev)
+        table, lens = batch.args()
+        args = (batch.q.to(dev), batch.cache(), table, lens)
+        call = lambda: sageattn_paged(*args, cu_q=batch.cu_q(), max_q=what)  # noqa: E731
+    torch.cuda.synchronize()
+    word.fill_(3)
+    try:
+        call()
+        torch.cuda.synchronize()
+        first = int(word)
+        assert first % 16 == 2 and int(mirror[0]) == first
+        mirror[0] = 0                                                        # (or the next call would raise before its launch)
+        call()
+        torch.cuda.synchronize()
+        assert int(word) == first
+    finally:
+        clear_status(dev)
+
+
+@pytest.mark.gpu
+def test_a_page_code_does_not_replace_a_wait():
+    """... nor is a wait's code taken for the page's, whichever is reported first."""
+    dev = torch.device("cuda", 0)
+    batch = PagedBatch([1, 1], [20, 40], 2, 2, 64, 16, "NHD", F16, dev)
+    table, lens = batch.args()
+    table[1, 2] = -1
+    k = H.randn((2, 2, 64), 1, F16, dev)
+    cache = batch.cache()
+    core._prepare_status(dev)
+    word, mirror = core._status_word(dev), core._status_mirror(dev)[1]
+    try:
+        word.fill_(2 + 16 * 20)
+        paged_kv_append(cache, k, k, table, lens)
+        torch.cuda.synchronize()
+        assert int(word) == 2 + 16 * 20 and int(mirror[0]) == 2 + 16 * 20
+    finally:
+        clear_status(dev)
