@@ -373,11 +373,14 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           limit = p.causal ? max(0, g.len - (g.q0 + g.n_q - 1 - token)) : g.len;
         }
       }
-      const bool warp_live = __any_sync(0xffffffffu, live);
+      // Rows without a token hold whatever an earlier kernel left in shared memory, or tokens of another sequence: they have no
+      // vote below, or the bits of the others would depend on it.
+      const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+      const bool warp_live = live_rows != 0;
       const int warp_limit = __reduce_min_sync(0xffffffffu, live ? limit : 0x7fffffff);
       float m = -INFINITY, l = 0.0f;
       int distrust = 0;                               // > 1: the optimistic pass is skipped
-      bool settled = false;                           // every row of the warp has a maximum
+      bool settled = false;                           // every row of the warp that has a token has a maximum
       const f32x2_t scale2 = pack2(p.score_scale, p.score_scale);
 #pragma unroll 1
       for (int hh = 0; hh < 2 * g.n_tiles; ++hh) {
@@ -431,7 +434,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const f32x2_t acc = weigh(sr[0], m, [](int, float*) {}, by_hand, pk);
             const float2 a = unpack2(fadd2(acc, weigh(sr[1], m, [](int, float*) {}, by_hand, pk + 16)));
             const float sum = a.x + a.y;
-            done = !__any_sync(0xffffffffu, !(sum <= kTileSumMax) || high > 16.0f);
+            done = (__ballot_sync(0xffffffffu, !(sum <= kTileSumMax) || high > 16.0f) & live_rows) == 0;
             if (done) {
               l += sum;
               tmem_st32(t_sh, pk);
@@ -454,7 +457,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               }
             }
             const bool need = top > m + (attempt ? kTileRefusedLazy : kTileLazy) || (m == -INFINITY && top > m);
-            const bool moved = __any_sync(0xffffffffu, need);
+            const bool moved = (__ballot_sync(0xffffffffu, need) & live_rows) != 0;
             if (!attempt && hh > 0) distrust = moved ? min(distrust + 1, 4) : max(distrust - 1, 0);
             if (moved) {
               if (hh > 0) {
@@ -474,7 +477,7 @@ sage_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               }
               if (need) m = top;
             }
-            settled = !__any_sync(0xffffffffu, m == -INFINITY);
+            settled = (__ballot_sync(0xffffffffu, m == -INFINITY) & live_rows) == 0;
             const float base = m == -INFINITY ? 0.0f : m;            // (a row that has seen nothing yet)
 #pragma unroll 1
             for (int c = 0; c < kHalfKeys; c += 16) {                // (P of these columns goes where columns before them were)

@@ -130,3 +130,41 @@ def test_a_page_code_does_not_replace_a_wait():
         assert int(word) == 2 + 16 * 20 and int(mirror[0]) == 2 + 16 * 20
     finally:
         clear_status(dev)
+
+
+# ---------------------------------------------------------------- rows that belong to no token
+
+def fill_shared_memory(value, D, dtype, dev):
+    """A call that leaves `value` in the places of Q of every SM."""
+    heads = 320
+    cache = PagedKV.allocate(16, 16, heads, D, dtype=dtype)
+    q = torch.full((256, heads, D), value, dtype=dtype, device=dev)
+    i32 = dict(dtype=torch.int32, device=dev)
+    sageattn_paged(q, cache, torch.arange(16, **i32)[None], torch.full((1,), 256, **i32), cu_q=torch.tensor([0, 256], **i32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("group, D", [(3, 128), (5, 64), (12, 128), (1, 64)])
+def test_rows_without_a_token_change_nothing(group, D, dtype):
+    """Groups that do not divide a row tile, and a tile that reaches behind the last sequence: what stands in those rows (of an earlier
+    kernel, of the padding, of the next sequence) does not change a bit of the others."""
+    dev = torch.device("cuda", 0)
+    batch = PagedBatch([61, 75], [900, 333], 2 * group, 2, D, 16, "NHD", dtype, dev, seed=group)
+    table, lens = batch.args()
+    cache, cu = batch.cache(), batch.cu_q()
+    results = []
+    for filler in (0.0, float("nan"), 300.0, float("inf")):
+        for pad in (0.0, float("nan")):
+            q = torch.cat([batch.q, torch.full((200, 2 * group, D), pad, dtype=dtype)]).to(dev)
+            fill_shared_memory(filler, D, dtype, dev)
+            results.append(sageattn_paged(q, cache, table, lens, cu_q=cu, return_lse=True))
+    check_status(dev)
+    for o, lse in results:
+        compare(batch, o[:batch.T], lse[:batch.T])
+        assert torch.equal(o, results[0][0]) and torch.equal(lse, results[0][1])
+    # a neighbour that is not a number
+    sick = batch.q.clone()
+    sick[61:] = float("nan")
+    o, lse = sageattn_paged(sick.to(dev), cache, table, lens, cu_q=cu, return_lse=True)
+    assert torch.equal(o[:61], results[0][0][:61]) and torch.equal(lse[:61], results[0][1][:61])
