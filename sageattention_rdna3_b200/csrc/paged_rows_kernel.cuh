@@ -464,7 +464,7 @@ sage_paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         }
         const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) out[c] *= inv;
+        for (int c = 0; c < 4; ++c) out[c] = sum == 0.0f ? 0.0f : out[c] * inv;    // (of a row without keys: 0 * V)
         if (g.slot >= 0) {
           const long long at = (static_cast<long long>(blockIdx.x) * 2 + g.slot) * kRows + r;
           store_floats(p.part_o + at * D + col, out);

@@ -183,6 +183,8 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
     ``paged_kv_append``; ``max_q``, if the program knows it, is an upper bound of the new tokens of one sequence and helps to choose
     the kernel.  ``is_causal`` aligns the last new token with the last key (a token sees the keys up to its own
     position); without it every token sees all keys of its sequence.  A row without keys is zero, its log-sum-exp -inf.
+    Keys that a row does not see may be anything; values that are not finite reach the rows of the same step and sequence that
+    share a tile of keys with them (0 * inf), as they do in a product of matrices.
 
     shared_pages: ``[n]`` int32.  The first ``n * page_size`` keys of every sequence stand in these pages (a system
     prompt, one question with many answers); they are read once for the whole batch, and the first n columns of ``page_table``

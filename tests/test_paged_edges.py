@@ -168,3 +168,21 @@ def test_rows_without_a_token_change_nothing(group, D, dtype):
     sick[61:] = float("nan")
     o, lse = sageattn_paged(sick.to(dev), cache, table, lens, cu_q=cu, return_lse=True)
     assert torch.equal(o[:61], results[0][0][:61]) and torch.equal(lse[:61], results[0][1][:61])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("q_lens, kv_lens", [([6, 1], [2, 50]), ([100, 1], [30, 50]), ([700], [500])])
+def test_a_row_without_keys_is_zero_whatever_v_holds(q_lens, kv_lens, value):
+    dev = torch.device("cuda", 0)
+    batch = PagedBatch(q_lens, kv_lens, 8, 2, 64, 16, "HND", F16, dev)
+    batch.v[0][:] = value
+    batch._put(0, 0, kv_lens[0], batch.k[0], batch.v[0])
+    table, lens = batch.args()
+    for max_q in (None, 1):
+        o, lse = sageattn_paged(batch.q.to(dev), batch.cache(), table, lens, cu_q=batch.cu_q(), max_q=max_q, return_lse=True)
+        check_status(dev)
+        blind = q_lens[0] - kv_lens[0]
+        assert (lse[:blind] == float("-inf")).all() and torch.isfinite(lse[blind:]).all()
+        assert torch.equal(o[:blind], torch.zeros_like(o[:blind]))
+        assert not torch.isfinite(o[blind:q_lens[0]]).any() and torch.isfinite(o[q_lens[0]:]).all()
