@@ -59,7 +59,8 @@ typedef struct sage_paged_kv {
  * new tokens included: new token i of n has position kv_lens[b] - n + i, and key j stands in slot j % page_size of page
  * page_table[b * table_stride + j / page_size].  All four arrays are int32 on the device.  Entries of the table behind the
  * last key are not looked at.  cu_q that leaves [0, T] or falls is clipped; rows that belong to no sequence are not written
- * (by sage_paged_append: zeroed). */
+ * (by sage_paged_append: zeroed).  Without cu_q a kv_lens of 0 is a slot that is not in use: nothing is stored for it, and
+ * its rows are zero. */
 typedef struct sage_paged_batch {
   const int32_t* page_table;
   int64_t table_stride;

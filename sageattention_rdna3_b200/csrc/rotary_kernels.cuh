@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) sage_paged_appe
   }
   int q0, q1;
   p.batch.tokens(b, &q0, &q1);
-  const bool belongs = token >= q0 && token < q1;
+  // (without cu_q a sequence of length 0 is a slot that is not in use: its row belongs to no sequence)
+  const bool belongs = token >= q0 && token < q1 && (searched || p.batch.kv_lens[b] != 0);
   const long long at = belongs ? static_cast<long long>(p.batch.kv_lens[b]) - (q1 - token) : 0;
   long long page = -1;
   int slot = 0;
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kRotaryBlocks) sage_paged_appe
 #pragma unroll
     for (int u = 0; u < kHeadsInFlight; ++u) {
       if (h + u >= h1 || out[u] == nullptr) continue;
-      if (!belongs) {                                 // a row of q behind the last sequence
+      if (!belongs) {                                 // a row of q that belongs to no sequence
 #pragma unroll
         for (int i = 0; i < Group<T>::kVec; ++i) g[u].a[i] = g[u].b[i] = make_uint4(0, 0, 0, 0);
       } else if (turned && h + u < heads_turned) {

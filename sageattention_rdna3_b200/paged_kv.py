@@ -127,7 +127,8 @@ def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table
     rotary: k is turned on its way, and q (``[T, Hq, D]``) too: the turned q is returned, a new tensor.  The position is the one in
     the sequence, on every axis, unless ``positions`` (``[T]`` or ``[T, axes]``, int32 / int64) gives others.
 
-    Rows that belong to no sequence (T may be padded) are not stored, and zero in the returned q.  A page index
+    Rows that belong to no sequence (T may be padded) are not stored, and zero in the returned q; without ``cu_q`` also those of
+    length 0, slots of a batch that are not in use.  A page index
     outside the cache, a position outside the page table or more new tokens than ``kv_lens`` says are not stored either; they
     are reported like the errors of ``sageattn``, by the next call or ``check_status()``.  Two sequences that share a page
     must not append to it at once, and k, v and q must not lie in the cache."""

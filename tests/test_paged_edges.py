@@ -186,3 +186,38 @@ def test_a_row_without_keys_is_zero_whatever_v_holds(q_lens, kv_lens, value):
         assert (lse[:blind] == float("-inf")).all() and torch.isfinite(lse[blind:]).all()
         assert torch.equal(o[:blind], torch.zeros_like(o[:blind]))
         assert not torch.isfinite(o[blind:q_lens[0]]).any() and torch.isfinite(o[q_lens[0]:]).all()
+
+
+# ---------------------------------------------------------------- slots that are not in use
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("aligned", [True, False])
+def test_slots_that_are_not_in_use(aligned):
+    """Without cu_q a sequence of length 0 is a slot that is not in use: nothing stored, nothing reported, its rows zero."""
+    dev = torch.device("cuda", 0)
+    batch = PagedBatch([1] * 5, [20, 1, 33, 1, 16], 4, 2, 64, 16, "NHD", F16, dev)
+    table, lens = batch.args()
+    lens[1] = lens[3] = 0
+    rope = rotary_axes(64, 64)
+    joint = torch.randn(5, 8, 64 if aligned else 68, device=dev).to(F16)[..., :64]       # (else copied, by the way through Python)
+    q, k, v = joint[:, :4], joint[:, 4:6], joint[:, 6:]
+    cache, plain = batch.cache(), batch.cache()
+    used = [0, 2, 4]
+    want = paged_kv_append(plain, k[used], v[used], table[used], lens[used], rotary=rope, q=q[used])
+    for positions in (None, torch.arange(5, device=dev)):
+        got = paged_kv_append(cache, k, v, table, lens, rotary=rope, q=q, positions=positions)
+        check_status(dev)
+        assert torch.equal(got[[1, 3]], torch.zeros_like(got[[1, 3]]))
+        if positions is None:
+            assert torch.equal(got[used], want)
+            for x, y in ((cache.k_pages, plain.k_pages), (cache.v_pages, plain.v_pages)):
+                assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+            o, lse = sageattn_paged(got, cache, table, lens, return_lse=True)
+            assert torch.equal(o[[1, 3]], torch.zeros_like(o[[1, 3]])) and (lse[[1, 3]] == float("-inf")).all()
+            assert torch.equal(o[used], sageattn_paged(want, plain, table[used], lens[used]))
+    check_status(dev)
+    # a negative length is no slot
+    lens[1] = -1
+    paged_kv_append(cache, k, v, table, lens)
+    with pytest.raises(RuntimeError, match="device status 4"):
+        check_status(dev)
