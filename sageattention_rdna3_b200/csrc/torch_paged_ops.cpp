@@ -143,7 +143,11 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({positions, freq, axis});
     ctx->saved_data["args"] = std::vector<int64_t>{interleaved, layout, inverse};
-    return rotary(q, k, positions, freq, axis, interleaved, layout, inverse);
+    auto out = rotary(q, k, positions, freq, axis, interleaved, layout, inverse);
+    // (a result of what needs no gradient needs none either)
+    if (!q.requires_grad()) ctx->mark_non_differentiable({out[0]});
+    else if (k.has_value() && !k->requires_grad()) ctx->mark_non_differentiable({out[1]});
+    return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
@@ -152,12 +156,13 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     auto turn = [&](const at::Tensor& a, const c10::optional<at::Tensor>& b) {
       return RotaryNode::apply(a, b, saved[0], saved[1], saved[2], args[0], args[1], args[2] == 0 ? 1 : 0);
     };
-    const bool has_k = grads.size() > 1 && grads[1].defined();
-    if (grads[0].defined()) {
-      const auto d = turn(grads[0], has_k ? c10::optional<at::Tensor>(grads[1]) : c10::nullopt);
+    const bool want_q = grads[0].defined() && ctx->needs_input_grad(0);
+    const bool want_k = grads.size() > 1 && grads[1].defined() && ctx->needs_input_grad(1);
+    if (want_q) {
+      const auto d = turn(grads[0], want_k ? c10::optional<at::Tensor>(grads[1]) : c10::nullopt);
       dq = d[0];
-      if (has_k) dk = d[1];
-    } else if (has_k) {
+      if (want_k) dk = d[1];
+    } else if (want_k) {
       dk = turn(grads[1], c10::nullopt)[0];
     }
     return {dq, dk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};

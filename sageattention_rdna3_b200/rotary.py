@@ -92,7 +92,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     q: ``[B,H,S,D]`` ("HND") or ``[B,S,H,D]`` ("NHD"), fp16 / bf16 / fp32; k likewise with its own number of heads, or
     None (then only q is returned).  positions: int32 or int64 on the device, ``[S]`` or ``[B,S]`` for one axis, else
     ``[S, axes]`` or ``[B, S, axes]``; any integers, negative ones too.  Returns new tensors; the arithmetic is fp32 with
-    one rounding at the end.  Differentiable in q and k (reverse mode, any order).  Forward and backward can be captured in one
+    one rounding at the end.  Differentiable in q and k (reverse mode, any order); the result of one that needs no gradient needs
+    none.  Forward and backward can be captured in one
     CUDA graph; as with every operator of torch, no graph of the same leaves that was recorded outside may be alive then: its
     nodes accumulate on their own stream, which a capture cannot join."""
     assert isinstance(rotary, RotaryAxes), "rotary must come from rotary_axes()."
