@@ -134,6 +134,14 @@ at::Tensor vector_aligned(const at::Tensor& t) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// The operator below autograd: through the dispatcher where a mode wants to see it.
+std::vector<at::Tensor> rotary_below(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& positions, const at::Tensor& freq,
+                                     const at::Tensor& axis, int64_t interleaved, int64_t layout, int64_t inverse) {
+  if (!c10::impl::TorchDispatchModeTLS::any_modes_set()) return rotary(q, k, positions, freq, axis, interleaved, layout, inverse);
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("sageattention::rotary", "").typed<decltype(rotary)>();
+  return op.call(q, k, positions, freq, axis, interleaved, layout, inverse);
+}
+
 // The gradient of a rotation is the rotation the other way.  (In Python the same node cost 40 us of host time.)
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const c10::optional<at::Tensor>& k,
@@ -143,7 +151,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({positions, freq, axis});
     ctx->saved_data["args"] = std::vector<int64_t>{interleaved, layout, inverse};
-    auto out = rotary(q, k, positions, freq, axis, interleaved, layout, inverse);
+    auto out = rotary_below(q, k, positions, freq, axis, interleaved, layout, inverse);
     // (a result of what needs no gradient needs none either)
     if (!q.requires_grad()) ctx->mark_non_differentiable({out[0]});
     else if (k.has_value() && !k->requires_grad()) ctx->mark_non_differentiable({out[1]});

@@ -65,3 +65,29 @@ def test_second_derivatives_of_a_frozen_input():
     w = H.randn((1, 2, 9, 64), 4, torch.float32, dev)
     (dg,) = torch.autograd.grad(dq, (g,), (w,))
     assert torch.equal(dg, apply_rotary(w, None, pos, rope))
+
+
+@pytest.mark.gpu
+def test_dispatch_modes_see_the_rotation():
+    """... forward and backward, not only what it allocates."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            Names.seen.append(func.__name__)
+            return func(*args, **(kwargs or {}))
+
+    dev = torch.device("cuda", 0)
+    rope, pos = rotary_axes(64, 64), torch.arange(9, device=dev)
+    x = H.randn((1, 2, 9, 64), 1, torch.float32, dev)
+    want = apply_rotary(x, None, pos, rope)
+    leaf = x.clone().requires_grad_()
+    (dwant,) = torch.autograd.grad(apply_rotary(leaf, None, pos, rope), (leaf,), (x,))
+    with Names():
+        assert torch.equal(apply_rotary(x, None, pos, rope), want)
+        assert Names.seen.count("rotary.default") == 1
+        (got,) = torch.autograd.grad(apply_rotary(leaf, None, pos, rope), (leaf,), (x,))
+        assert Names.seen.count("rotary.default") == 3
+    assert torch.equal(got, dwant)
