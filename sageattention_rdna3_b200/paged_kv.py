@@ -19,6 +19,7 @@ from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import _native
 from .core import _LAYOUT_CODE, _prepare_status, _raise_pending, _register, _status_word, check_status
@@ -112,6 +113,7 @@ def _check_rows(cache: PagedKV, name: str, t: torch.Tensor, heads: Optional[int]
         f"{name} must have the dtype and device of the cache.")
     assert not (torch.is_grad_enabled() and t.requires_grad), (
         f"{name} requires a gradient: the paged cache has none (detach it, or call under torch.no_grad()).")
+    assert fwAD.unpack_dual(t).tangent is None, f"{name} has a tangent: the paged cache has no derivative in forward mode either."
 
 
 def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,

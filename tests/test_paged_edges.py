@@ -221,3 +221,98 @@ def test_slots_that_are_not_in_use(aligned):
     paged_kv_append(cache, k, v, table, lens)
     with pytest.raises(RuntimeError, match="device status 4"):
         check_status(dev)
+
+
+# ---------------------------------------------------------------- tangents, modes, subclasses
+
+def refused(fn, *args, match="gradient|tangent", **kwargs):
+    with pytest.raises(AssertionError, match=match):
+        fn(*args, **kwargs)
+
+
+def test_tangents_are_refused():
+    """The cache has no derivative in either mode: a dual tensor is refused, not stripped of its tangent."""
+    cache = PagedKV.allocate(4, 16, 2, 64, dtype=F16, device="cpu")
+    table, lens = torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    q, k = torch.zeros(3, 4, 64, dtype=F16), torch.zeros(3, 2, 64, dtype=F16)
+    with fwAD.dual_level():
+        dq, dk = fwAD.make_dual(q, torch.ones_like(q)), fwAD.make_dual(k, torch.ones_like(k))
+        refused(sageattn_paged, dq, cache, table, lens)
+        refused(paged_kv_append, cache, dk, k, table, lens)
+        refused(paged_kv_append, cache, k, dk, table, lens)
+        refused(paged_kv_append, cache, k, k, table, lens, q=dq, rotary=rotary_axes(64, 64, device="cpu"))
+
+
+class Marked(torch.Tensor):
+    """A subclass that sees every function called on it."""
+    seen = 0
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        Marked.seen += 1
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+@pytest.mark.gpu
+def test_the_short_ways_leave_what_is_not_plain():
+    """Modes, subclasses, dual tensors, vmap: none of them is passed by."""
+    import sageattention_rdna3_b200._C as C
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+    dev = torch.device("cuda", 0)
+    batch = PagedBatch([1, 1], [20, 40], 4, 2, 64, 16, "NHD", F16, dev)
+    table, lens = batch.args()
+    cache, q = batch.cache(), batch.q.to(dev)
+    k = H.randn((2, 2, 64), 1, F16, dev)
+    rope = rotary_axes(64, 64)
+    x, pos = H.randn((1, 2, 8, 64), 2, torch.float32, dev), torch.arange(8, device=dev)
+    want, turned = sageattn_paged(q, cache, table, lens), apply_rotary(x, None, pos, rope)
+    table_args = (rope.freq, rope.axis, 1, False)
+
+    def attn(q):
+        return C.paged_attn_plain(q, cache.k_pages, cache.v_pages, "NHD", table, lens, None, None, True, None, False, None)
+
+    def append(k):
+        return C.paged_append_plain(cache.k_pages, cache.v_pages, "NHD", k, k, table, lens, None, None, None, None, 0, False, None)
+
+    def rotary(x):
+        return C.rotary_plain(x, None, pos, *table_args, 64, "HND")
+
+    assert torch.equal(attn(q), want) and append(k) is True and torch.equal(rotary(x), turned)
+    want = sageattn_paged(q, cache, table, lens)
+
+    class Functions(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    class Dispatched(TorchDispatchMode):
+        names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            Dispatched.names.append(func.__name__)
+            return func(*args, **(kwargs or {}))
+
+    for mode in (Functions, Dispatched):
+        with mode():
+            assert attn(q) is None and append(k) is None and rotary(x) is None
+            assert torch.equal(sageattn_paged(q, cache, table, lens), want)
+            paged_kv_append(cache, k, k, table, lens)
+            assert torch.equal(apply_rotary(x, None, pos, rope), turned)
+    assert {"paged_attn.default", "paged_append.default", "rotary.default"} <= set(Dispatched.names)
+    marked = [t.as_subclass(Marked) for t in (q, k, x)]
+    assert attn(marked[0]) is None and append(marked[1]) is None and rotary(marked[2]) is None
+    # a parameter is a tensor that needs a gradient: refused by the cache, turned with a gradient behind it
+    assert attn(torch.nn.Parameter(q)) is None and append(torch.nn.Parameter(k)) is None
+    assert rotary(torch.nn.Parameter(x)).requires_grad and torch.equal(rotary(torch.nn.Parameter(x)), turned)
+    with fwAD.dual_level():
+        dual = [fwAD.make_dual(t, torch.ones_like(t)) for t in (q, k, x)]
+        assert attn(dual[0]) is None and append(dual[1]) is None and rotary(dual[2]) is None
+        refused(sageattn_paged, dual[0], cache, table, lens)
+        refused(paged_kv_append, cache, dual[1], k, table, lens)
+        with pytest.raises(RuntimeError):                                    # no forward derivative either
+            apply_rotary(dual[2], None, pos, rope)
+    with pytest.raises(RuntimeError):                                        # no batching rule
+        torch.func.vmap(lambda t: sageattn_paged(t, cache, table, lens))(q[None].repeat(2, 1, 1, 1))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: apply_rotary(t, None, pos, rope))(x[None].repeat(2, 1, 1, 1, 1))
+    check_status(dev)
