@@ -19,6 +19,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdlib>
+#include <numeric>
 #include <vector>
 
 #include "../../include/sage_paged_b200.h"
@@ -281,6 +282,43 @@ std::vector<at::Tensor> paged_append(at::Tensor& k_pages, at::Tensor& v_pages, i
   return out;
 }
 
+// First and last byte of a tensor, and whether two of them can share any.
+struct Bytes {
+  int64_t lo, hi;
+  explicit Bytes(const at::Tensor& t) : lo(reinterpret_cast<int64_t>(t.data_ptr())), hi(lo + t.element_size()) {
+    for (int64_t i = 0; i < t.dim(); ++i) hi += (t.size(i) - 1) * t.stride(i) * static_cast<int64_t>(t.element_size());
+  }
+};
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const Bytes x(a), y(b);
+  return x.hi <= y.lo || y.hi <= x.lo;
+}
+
+// Rows `a` and `b`, [T, H, D] both, known to lie between one another: true if no row of one meets a row of the other.  It is enough
+// that they keep to different parts of a period in memory: that of all their rows (slots of a head), of a token, or of a head.
+bool rows_apart(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t T = a.size(0), H = a.size(1), D = a.size(2), size = a.element_size();
+  const int64_t distance = (reinterpret_cast<int64_t>(b.data_ptr()) - reinterpret_cast<int64_t>(a.data_ptr())) / size;
+  const int64_t st = T > 1 ? a.stride(0) : 0, sh = H > 1 ? a.stride(1) : 0;
+  if ((T > 1 && b.stride(0) != st) || (H > 1 && b.stride(1) != sh)) return false;
+  auto separate = [&](int64_t period, int64_t length) {          // `length` values from a multiple of `period` and from `distance` on
+    if (period <= 0) return false;
+    const int64_t d = (distance % period + period) % period;
+    return d >= length && d + length <= period;
+  };
+  return separate(std::gcd(st, sh), D) || separate(st, (H - 1) * sh + D) || separate(sh, (T - 1) * st + D);
+}
+
+// Each row of q is read by the thread blocks that write the same row of o and no others: o may be q, but not a shifted q.
+void check_output(const at::Tensor& o, const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages) {
+  at::assert_no_internal_overlap(o);
+  bool same = o.data_ptr() == q.data_ptr();
+  for (int64_t i = 0; i < 3; ++i) same = same && (o.size(i) <= 1 || o.stride(i) == q.stride(i));
+  TORCH_CHECK(same || apart(o, q) || rows_apart(o, q), "the output must be q or share no memory with it: they overlap");
+  TORCH_CHECK(apart(o, k_pages) && apart(o, v_pages), "the output must share no memory with the cache: they overlap");
+}
+
 // paged_attn(Tensor query, Tensor(a!) output, Tensor k_pages, Tensor v_pages, int tensor_layout, Tensor page_table, Tensor kv_lens,
 //            Tensor? cu_q, int max_q, int is_causal, float sm_scale, Tensor? lse, Tensor? shared_pages, int zero_rest, Tensor status) -> ()
 void paged_attn(const at::Tensor& q, at::Tensor& o, const at::Tensor& k_pages, const at::Tensor& v_pages, int64_t layout,
@@ -292,11 +330,7 @@ void paged_attn(const at::Tensor& q, at::Tensor& o, const at::Tensor& k_pages, c
   check_rows(q, k_pages, -1, "query");
   check_rows(o, k_pages, q.size(1), "output");
   TORCH_CHECK(o.size(0) == q.size(0), "query and output differ in length");
-  // Each row of q is read by the thread blocks that write the same row of o and no others: o may be q, but not a shifted q.
-  at::assert_no_internal_overlap(o);
-  at::assert_no_partial_overlap(o, q);
-  at::assert_no_overlap(o, k_pages);
-  at::assert_no_overlap(o, v_pages);
+  check_output(o, q, k_pages, v_pages);
   const sage_paged_batch_t batch = batch_of(page_table, kv_lens, cu_q, q.size(0), k_pages);
   const int Hq = size_of(q.size(1), "heads"), longest = size_of(max_q, "max_q");
   int n_shared = 0;

@@ -223,6 +223,36 @@ def test_slots_that_are_not_in_use(aligned):
         check_status(dev)
 
 
+# ---------------------------------------------------------------- results that overlap
+
+@pytest.mark.gpu
+def test_overlaps_of_strided_results_are_refused():
+    """q and out as slices of one joint projection: heads that another block still reads must not be written."""
+    dev = torch.device("cuda", 0)
+    batch = PagedBatch([1, 1, 1], [20, 300, 5], 4, 2, 64, 16, "NHD", F16, dev)
+    table, lens = batch.args()
+    cache = batch.cache()
+    want = sageattn_paged(batch.q.to(dev), cache, table, lens)
+    joint = torch.zeros(4, 12, 64, dtype=F16, device=dev)
+    by_head = torch.zeros(12, 4, 64, dtype=F16, device=dev).transpose(0, 1)
+    pairs = torch.zeros(3, 4, 2, 64, dtype=F16, device=dev)
+    for q, out in ((joint[:3, :4], joint[:3, 1:5]), (joint[:3, :4], joint[1:, :4]), (joint[:3, :4], joint[1:, 3:7]),
+                   (by_head[:3, :4], by_head[:3, 2:6]), (by_head[:3, :4], by_head[1:, :4]),
+                   (joint[:3, :4], joint.view(-1, 64)[:12].view(3, 4, 64))):
+        with pytest.raises(RuntimeError, match="overlap|memory"):
+            sageattn_paged(q, cache, table, lens, out=out)
+    both = torch.zeros(6, 2, 16, 2, 64, dtype=F16, device=dev)
+    pool = PagedKV(both[:, 0], both[:, 1])
+    with pytest.raises(RuntimeError, match="overlap|memory"):
+        sageattn_paged(batch.q[:, :2].to(dev), pool, table, lens, out=both[0, 0, 4:7])
+    # neighbours that only lie between each other are none
+    for q, out in ((joint[:3, :4], joint[:3, 4:8]), (joint[:3, 8:], joint[1:, :4]), (by_head[:3, :4], by_head[:3, 4:8]),
+                   (by_head[:3, :4], by_head[1:, 8:]), (pairs[:, :, 0], pairs[:, :, 1]), (joint[:3, :4], joint[:3, :4])):
+        q.copy_(batch.q)
+        assert torch.equal(sageattn_paged(q, cache, table, lens, out=out), want)
+    check_status(dev)
+
+
 # ---------------------------------------------------------------- tangents, modes, subclasses
 
 def refused(fn, *args, match="gradient|tangent", **kwargs):
