@@ -240,6 +240,11 @@ void check_rows(const at::Tensor& t, const at::Tensor& k_pages, int64_t heads, c
   check_vectors(t, name);
 }
 
+// Counts a change of `t` in place: a backward pass that kept it is refused then.  (Tensors made for inference count none.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // paged_append(Tensor(a!) k_pages, Tensor(b!) v_pages, int tensor_layout, Tensor key, Tensor value, Tensor page_table, Tensor kv_lens,
 //              Tensor? cu_q, Tensor? query, Tensor? freq, Tensor? axis, int n_axes, int interleaved, Tensor? positions, Tensor status)
 // -> Tensor[]: the turned query, if one is given.  positions: [T, n_axes].
@@ -279,6 +284,8 @@ std::vector<at::Tensor> paged_append(at::Tensor& k_pages, at::Tensor& v_pages, i
                              q.has_value() ? size_of(q->size(1), "heads") : 0, turn ? &r : nullptr, status_of(status, k_pages),
                              current_stream(k_pages)),
            "paged_append");
+  written(k_pages);
+  written(v_pages);
   return out;
 }
 
@@ -353,6 +360,7 @@ void paged_attn(const at::Tensor& q, at::Tensor& o, const at::Tensor& k_pages, c
                            n_shared > 0 ? shared_pages->data_ptr<int32_t>() : nullptr, n_shared, zero_rest != 0,
                            status_of(status, k_pages), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, current_stream(k_pages)),
            "paged_attn");
+  written(o);
 }
 
 }  // namespace
@@ -582,6 +590,8 @@ PyObject* sage_paged_append_plain(PyObject*, PyObject* const* args, Py_ssize_t n
     check_rc(sage_paged_append(&cache, &batch, &ks, &vs, q != nullptr ? &qs : nullptr, q != nullptr ? &qo : nullptr,
                                q != nullptr ? size_of(q->size(1), "heads") : 0, freq != nullptr ? &r : nullptr, status, current_stream(*kp)),
              "paged_append");
+    written(*kp);
+    written(*vp);
   }
   if (q == nullptr) Py_RETURN_TRUE;
   return THPVariable_Wrap(out);

@@ -253,7 +253,32 @@ def test_overlaps_of_strided_results_are_refused():
     check_status(dev)
 
 
-# ---------------------------------------------------------------- tangents, modes, subclasses
+# ---------------------------------------------------------------- versions, tangents, modes, subclasses
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("aligned", [True, False])
+def test_what_is_written_counts_as_changed(aligned):
+    """Autograd refuses a backward pass whose saved tensors were written: the pages and `out` count their versions."""
+    dev = torch.device("cuda", 0)
+    cache = PagedKV.allocate(4, 16, 2, 64, dtype=F16)
+    table, lens = torch.arange(3, dtype=torch.int32, device=dev)[:, None], torch.ones(3, dtype=torch.int32, device=dev)
+    rows = torch.ones(3, 2, 64 if aligned else 68, dtype=F16, device=dev)[..., :64]
+    for _ in range(2):                                       # the second call on a device may take the short way
+        versions = cache.k_pages._version, cache.v_pages._version
+        paged_kv_append(cache, rows, rows, table, lens)
+        assert cache.k_pages._version > versions[0] and cache.v_pages._version > versions[1]
+    q = torch.ones(3, 4, 64, dtype=F16, device=dev, requires_grad=True)
+    x = q * 1.0
+    y = x * x                                                # keeps x
+    sageattn_paged(x.detach(), cache, table, lens, out=x.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        pages = PagedKV.allocate(4, 16, 2, 64, dtype=F16)
+    paged_kv_append(pages, rows, rows, table, lens)          # a cache made for inference may be used outside of it
+    sageattn_paged(torch.ones(3, 4, 64, dtype=F16, device=dev), pages, table, lens)
+    check_status(dev)
+
 
 def refused(fn, *args, match="gradient|tangent", **kwargs):
     with pytest.raises(AssertionError, match=match):
