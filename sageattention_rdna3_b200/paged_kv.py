@@ -106,14 +106,18 @@ def _table_of(rotary: Optional[RotaryAxes]) -> tuple:
     return (None, None, 0, False) if rotary is None else (rotary.freq, rotary.axis, len(rotary.axes), rotary.interleaved)
 
 
+def _check_no_derivative(name: str, t: torch.Tensor) -> None:
+    assert not (torch.is_grad_enabled() and t.requires_grad), (
+        f"{name} requires a gradient: the paged cache has none (detach it, or call under torch.no_grad()).")
+    assert fwAD.unpack_dual(t).tangent is None, f"{name} has a tangent: the paged cache has no derivative in forward mode either."
+
+
 def _check_rows(cache: PagedKV, name: str, t: torch.Tensor, heads: Optional[int] = None) -> None:
     assert t.dim() == 3 and t.size(2) == cache.head_dim and (heads is None or t.size(1) == heads), (
         f"{name} must be [T, {'heads' if heads is None else heads}, {cache.head_dim}], got {tuple(t.shape)}.")
     assert t.dtype == cache.k_pages.dtype and t.device == cache.k_pages.device, (
         f"{name} must have the dtype and device of the cache.")
-    assert not (torch.is_grad_enabled() and t.requires_grad), (
-        f"{name} requires a gradient: the paged cache has none (detach it, or call under torch.no_grad()).")
-    assert fwAD.unpack_dual(t).tangent is None, f"{name} has a tangent: the paged cache has no derivative in forward mode either."
+    _check_no_derivative(name, t)
 
 
 def paged_kv_append(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -221,6 +225,7 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
     if out is not None:
         assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, (
             "out must have the shape, dtype and device of q.")
+        _check_no_derivative("out", out)
         assert out.stride(2) == 1 and out.data_ptr() % 16 == 0 and all(
             n <= 1 or (s % 8 == 0 and s > 0) for n, s in zip(out.shape[:2], out.stride()[:2])), (
             f"out needs a contiguous last dim, 16-byte aligned rows and a place for every row; got strides {out.stride()}.")

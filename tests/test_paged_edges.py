@@ -298,6 +298,14 @@ def test_tangents_are_refused():
         refused(paged_kv_append, cache, k, k, table, lens, q=dq, rotary=rotary_axes(64, 64, device="cpu"))
 
 
+def test_a_result_that_needs_a_gradient_is_refused():
+    cache = PagedKV.allocate(4, 16, 2, 64, dtype=F16, device="cpu")
+    table, lens = torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    q = torch.zeros(3, 4, 64, dtype=F16)
+    out = torch.zeros(3, 4, 64, dtype=F16, requires_grad=True)
+    refused(sageattn_paged, q, cache, table, lens, out=out)
+
+
 class Marked(torch.Tensor):
     """A subclass that sees every function called on it."""
     seen = 0
