@@ -244,7 +244,7 @@ def sageattn_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, kv
     if any(n > 1 and s == 0 for n, s in zip(q.shape, q.stride())):      # an expanded q
         q = q.contiguous()
     ops.paged_attn(_vector_aligned(q), out, cache.k_pages, cache.v_pages, _LAYOUT_CODE[cache.tensor_layout], page_table, kv_lens,
-                   cu_q, 0 if max_q is None else int(max_q), int(is_causal),
+                   cu_q, 0 if max_q is None else min(int(max_q), T), int(is_causal),
                    cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale), lse, shared_pages, int(zero_rest),
                    _status_word(dev))
     _check_if_asked(dev)

@@ -379,3 +379,15 @@ def test_the_short_ways_leave_what_is_not_plain():
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda t: apply_rotary(t, None, pos, rope))(x[None].repeat(2, 1, 1, 1, 1))
     check_status(dev)
+
+
+# ---------------------------------------------------------------- bounds
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_q", [2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 80])
+def test_an_upper_bound_may_be_any_number(max_q):
+    dev = torch.device("cuda", 0)
+    batch = PagedBatch([3, 1], [20, 40], 4, 2, 64, 16, "NHD", F16, dev)
+    table, lens = batch.args()
+    args = (batch.q.to(dev), batch.cache(), table, lens)
+    assert torch.equal(sageattn_paged(*args, cu_q=batch.cu_q(), max_q=max_q), sageattn_paged(*args, cu_q=batch.cu_q()))
