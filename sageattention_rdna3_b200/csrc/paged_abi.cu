@@ -345,7 +345,7 @@ int sage_apply_rotary(const sage_strided_t* q, const sage_strided_t* q_out, cons
   SAGE_REQUIRE(rotary->positions != nullptr, "rotary: null positions");
   const int unit = dtype == SAGE_DTYPE_F32 ? 4 : 8;
   for (const sage_strided_t* t : {q, q_out, k, k_out}) {
-    if (t == nullptr || ((t == q || t == q_out) && Hq == 0)) continue;
+    if (t == nullptr || (t == q || t == q_out ? Hq : Hkv) == 0) continue;
     SAGE_REQUIRE(t->ptr != nullptr && aligned16(t->ptr) && stride_ok(t->stride_b, unit) && stride_ok(t->stride_h, unit) && stride_ok(t->stride_s, unit),
                  "rotary: tensors need a 16-byte aligned base and strides that are multiples of 16 bytes");
   }

@@ -91,3 +91,17 @@ def test_dispatch_modes_see_the_rotation():
         (got,) = torch.autograd.grad(apply_rotary(leaf, None, pos, rope), (leaf,), (x,))
         assert Names.seen.count("rotary.default") == 3
     assert torch.equal(got, dwant)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_heads_that_are_not_there(layout):
+    dev = torch.device("cuda", 0)
+    rope, pos = rotary_axes(64, 64), torch.arange(9, device=dev)
+    q = H.randn((2, 9, 9, 64), 1, torch.float16, dev)
+    none = torch.empty((2, 0, 9, 64) if layout == "HND" else (2, 9, 0, 64), dtype=torch.float16, device=dev)
+    want = apply_rotary(q, None, pos, rope, tensor_layout=layout)
+    rq, rk = apply_rotary(q, none, pos, rope, tensor_layout=layout)
+    assert torch.equal(rq, want) and rk.shape == none.shape
+    rq, rk = apply_rotary(none, q, pos, rope, tensor_layout=layout)
+    assert torch.equal(rk, want) and rq.shape == none.shape
