@@ -246,7 +246,7 @@ void written(const at::Tensor& t) {
 }
 
 // paged_append(Tensor(a!) k_pages, Tensor(b!) v_pages, int tensor_layout, Tensor key, Tensor value, Tensor page_table, Tensor kv_lens,
-//              Tensor? cu_q, Tensor? query, Tensor? freq, Tensor? axis, int n_axes, int interleaved, Tensor? positions, Tensor status)
+//              Tensor? cu_q, Tensor? query, Tensor? freq, Tensor? axis, int n_axes, int interleaved, Tensor? positions, Tensor(c!) status)
 // -> Tensor[]: the turned query, if one is given.  positions: [T, n_axes].
 std::vector<at::Tensor> paged_append(at::Tensor& k_pages, at::Tensor& v_pages, int64_t layout, const at::Tensor& k, const at::Tensor& v,
                                      const at::Tensor& page_table, const at::Tensor& kv_lens, const c10::optional<at::Tensor>& cu_q,
@@ -327,7 +327,7 @@ void check_output(const at::Tensor& o, const at::Tensor& q, const at::Tensor& k_
 }
 
 // paged_attn(Tensor query, Tensor(a!) output, Tensor k_pages, Tensor v_pages, int tensor_layout, Tensor page_table, Tensor kv_lens,
-//            Tensor? cu_q, int max_q, int is_causal, float sm_scale, Tensor? lse, Tensor? shared_pages, int zero_rest, Tensor status) -> ()
+//            Tensor? cu_q, int max_q, int is_causal, float sm_scale, Tensor(b!)? lse, Tensor? shared_pages, int zero_rest, Tensor(c!) status) -> ()
 void paged_attn(const at::Tensor& q, at::Tensor& o, const at::Tensor& k_pages, const at::Tensor& v_pages, int64_t layout,
                 const at::Tensor& page_table, const at::Tensor& kv_lens, const c10::optional<at::Tensor>& cu_q, int64_t max_q,
                 int64_t is_causal, double sm_scale, const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& shared_pages,
@@ -370,10 +370,10 @@ TORCH_LIBRARY_FRAGMENT(sageattention, m) {
         "int inverse) -> Tensor[]");
   m.def("paged_append(Tensor(a!) k_pages, Tensor(b!) v_pages, int tensor_layout, Tensor key, Tensor value, Tensor page_table, "
         "Tensor kv_lens, Tensor? cu_q, Tensor? query, Tensor? freq, Tensor? axis, int n_axes, int interleaved, Tensor? positions, "
-        "Tensor status) -> Tensor[]");
+        "Tensor(c!) status) -> Tensor[]");
   m.def("paged_attn(Tensor query, Tensor(a!) output, Tensor k_pages, Tensor v_pages, int tensor_layout, Tensor page_table, "
-        "Tensor kv_lens, Tensor? cu_q, int max_q, int is_causal, float sm_scale, Tensor? lse, Tensor? shared_pages, int zero_rest, "
-        "Tensor status) -> ()");
+        "Tensor kv_lens, Tensor? cu_q, int max_q, int is_causal, float sm_scale, Tensor(b!)? lse, Tensor? shared_pages, int zero_rest, "
+        "Tensor(c!) status) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(sageattention, AutogradCUDA, m) {

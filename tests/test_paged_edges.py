@@ -381,7 +381,7 @@ def test_the_short_ways_leave_what_is_not_plain():
     check_status(dev)
 
 
-# ---------------------------------------------------------------- bounds
+# ---------------------------------------------------------------- bounds and schemas
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("max_q", [2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 80])
@@ -391,3 +391,11 @@ def test_an_upper_bound_may_be_any_number(max_q):
     table, lens = batch.args()
     args = (batch.q.to(dev), batch.cache(), table, lens)
     assert torch.equal(sageattn_paged(*args, cu_q=batch.cu_q(), max_q=max_q), sageattn_paged(*args, cu_q=batch.cu_q()))
+
+
+def test_schemas_say_what_is_written():
+    ops = _native.load_ops()
+    for op, names in ((ops.paged_append, {"k_pages", "v_pages", "status"}), (ops.paged_attn, {"output", "lse", "status"})):
+        schema = op.default._schema
+        assert {a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write} == names
+        assert schema.is_mutable
