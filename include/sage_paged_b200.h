@@ -27,7 +27,8 @@ extern "C" {
 
 /* Rotary positions.  The pairs of a head, (x[i], x[i + pairs]) or, interleaved, (x[2i], x[2i+1]), are turned by
  * freq[i] * positions[token][axis[i]].  freq is the angle per position in turns, as a fraction of 2^64: the product with
- * an integer position wraps at whole turns and is exact for positions of any size.  pairs is a multiple of 8;
+ * an integer position wraps at whole turns and is exact, so that only the rounding of freq itself (half of 2^-64 turns at best)
+ * grows with the position.  pairs is a multiple of 8;
  * what a head has behind its pairs is copied. */
 typedef struct sage_rotary {
   const uint64_t* freq;              /* [pairs], 16-byte aligned */

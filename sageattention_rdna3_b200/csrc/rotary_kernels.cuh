@@ -6,7 +6,8 @@
 //
 // The angle.  A position of 10^6 times a frequency in fp32 is off by up to 0.06 radians.  Here the frequency is a
 // fraction of a turn in units of 2^-64; a 64-bit product with the integer position wraps at whole turns by itself, and
-// its upper 32 bits are the angle, exact to 2^-32 turns wherever the token stands, without a range reduction.
+// its upper 32 bits are the angle, to 2^-32 turns of that product, without a range reduction.  The frequency itself is rounded to 2^-64:
+// at position p that is p 2^-65 turns more.
 //
 // The split.  A thread owns 8 pairs of a token (16-byte loads of both halves), computes their 8 angles once and walks over
 // a slice of the heads with them, two heads in flight: with one head per thread the sines take longer than the memory.
@@ -116,7 +117,7 @@ __device__ __forceinline__ long long position_at(const Rotary& r, long long offs
 
 // cos and sin of 2 pi t / 2^32 for two angles.  The nearest quarter turn is taken off in integers, which leaves r in
 // [-1/8, 1/8] turns, exact to fp32; there sin(2 pi r) = r S(r^2) and cos(2 pi r) = C(r^2) with polynomials of degree 3 and 4, fitted for
-// the smallest largest error (1.2e-9 and 5e-11; 1e-7 with fp32 arithmetic).  Two angles at a time in packed arithmetic this is
+// the smallest largest error (1.2e-9 and 9.5e-11; 1e-7 with fp32 arithmetic).  Two angles at a time in packed arithmetic this is
 // half the instructions of sincospif, and the sines are what the kernel computes most.
 __device__ __forceinline__ void sincos_turns(uint32_t t0, uint32_t t1, float* s0, float* s1, float* c0, float* c1) {
   const uint32_t q0 = (t0 + 0x20000000u) >> 30, q1 = (t1 + 0x20000000u) >> 30;

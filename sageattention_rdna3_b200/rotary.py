@@ -10,7 +10,8 @@ gradient another:
 """
 from __future__ import annotations
 
-import math
+import decimal
+import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple, Union
 
@@ -40,6 +41,26 @@ class RotaryAxes:
         return sum(self.axes)
 
 
+@functools.lru_cache(maxsize=8)
+def _pi(digits: int) -> decimal.Decimal:
+    """pi to `digits` digits, by the arithmetic-geometric mean (Gauss, Legendre)."""
+    with decimal.localcontext(decimal.Context(prec=digits + 10)):
+        a, b, t, p = decimal.Decimal(1), decimal.Decimal("0.5").sqrt(), decimal.Decimal("0.25"), 1
+        for _ in range(digits.bit_length() + 1):              # twice the digits each time
+            mean = (a + b) / 2
+            a, b, t, p = mean, (a * b).sqrt(), t - p * (a - mean) ** 2, 2 * p
+        return (a + b) ** 2 / (4 * t)
+
+
+def _turn_units(frequencies) -> list:
+    """Frequencies in radians per position (decimals) as turns in units of 2^-64, the nearest one, as int64 holds them."""
+    digits = 50 + max(0, max(f.adjusted() for f in frequencies))      # whole turns are taken off: 20 digits are left, and some
+    with decimal.localcontext(decimal.Context(prec=digits)):
+        per_radian = 2 ** 63 / _pi(digits)
+        units = [int((f * per_radian).to_integral_value()) % 2 ** 64 for f in frequencies]
+    return [u - 2 ** 64 if u >= 2 ** 63 else u for u in units]
+
+
 def rotary_axes(head_dim: int, axes: Union[int, Sequence[int]], base: Union[float, Sequence[float]] = 10000.0,
                 interleaved: bool = False, inv_freq: Optional[Sequence[float]] = None,
                 device: Union[torch.device, int, str, None] = None) -> RotaryAxes:
@@ -49,8 +70,8 @@ def rotary_axes(head_dim: int, axes: Union[int, Sequence[int]], base: Union[floa
     multiple of 16 and at most ``head_dim``; the values behind them stay as they are).  Pair i of an axis of width w has the
     frequency ``base ** (-2 i / w)`` radians per position; ``base`` may be one number per axis, and ``inv_freq`` (one
     number per pair, the pairs of axis 0 first) takes its place.  Pairs are ``(x[i], x[i + rotary_dim / 2])``, or
-    neighbours ``(x[2i], x[2i + 1])`` with ``interleaved``.  The frequencies keep 64 bits, so that positions
-    far from zero lose nothing."""
+    neighbours ``(x[2i], x[2i + 1])`` with ``interleaved``.  A frequency is kept as the nearest of 2^64 parts
+    of a turn: the angle at position p is off by at most p * 2^-65 turns for that (at 2^40 positions 1.9e-7 radians)."""
     widths = (axes,) if isinstance(axes, int) else tuple(int(w) for w in axes)
     assert head_dim in (64, 128), f"head_dim must be 64 or 128, got {head_dim}."
     assert 1 <= len(widths) <= MAX_AXES, f"1 to {MAX_AXES} axes, got {len(widths)}."
@@ -61,16 +82,18 @@ def rotary_axes(head_dim: int, axes: Union[int, Sequence[int]], base: Union[floa
     if inv_freq is None:
         bases = [float(base)] * len(widths) if isinstance(base, (int, float)) else [float(b) for b in base]
         assert len(bases) == len(widths) and all(b > 0 for b in bases), "base must be positive: one number, or one per axis."
-        inv_freq = [b ** (-2.0 * i / w) for b, w in zip(bases, widths) for i in range(w // 2)]
+        with decimal.localcontext(decimal.Context(prec=40)):
+            values = []
+            for b, w in zip(bases, widths):                  # (powers by products: a power of its own for each took 2 ms)
+                step, f = decimal.Decimal(b) ** (decimal.Decimal(-2) / w), decimal.Decimal(1)
+                for _ in range(w // 2):
+                    values.append(f)
+                    f = f * step
     else:
-        inv_freq = [float(f) for f in inv_freq]
-        assert len(inv_freq) == total // 2, f"inv_freq must have one number per pair ({total // 2}), got {len(inv_freq)}."
-    assert all(math.isfinite(f) for f in inv_freq), "frequencies must be finite."
-    freq = []
-    for f in inv_freq:
-        turns = f / (2.0 * math.pi)
-        units = int((turns - math.floor(turns)) * 2.0 ** 64) % 2 ** 64
-        freq.append(units - 2 ** 64 if units >= 2 ** 63 else units)
+        values = [decimal.Decimal(float(f)) for f in inv_freq]
+        assert len(values) == total // 2, f"inv_freq must have one number per pair ({total // 2}), got {len(values)}."
+    assert all(f.is_finite() for f in values), "frequencies must be finite."
+    freq = _turn_units(values)
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else (
         torch.device("cuda", device) if isinstance(device, int) else torch.device(device))
     return RotaryAxes(head_dim, widths, bool(interleaved), torch.tensor(freq, dtype=torch.int64).to(dev),

@@ -1,9 +1,86 @@
 """Edges of apply_rotary: inputs of which only some need a gradient, heads that are not there, positions of any size."""
+from fractions import Fraction
+
 import pytest
 import torch
 
 import helpers as H
 from sageattention_rdna3_b200 import PagedKV, apply_rotary, check_status, paged_kv_append, rotary_axes
+from test_rotary import partner_sum, rotate64, tolerance
+
+DIGITS = 400                                          # binary digits behind the point
+PI_DIGITS = 1200                                      # ... of pi: 2^997 radians are still to be known to 2^-64 turns
+
+
+def _pi():
+    """pi by Machin's formula, 16 arctan(1/5) - 4 arctan(1/239), within 2^-PI_DIGITS."""
+    one = 1 << (PI_DIGITS + 20)
+
+    def arctan_inverse(n):
+        total, power, k = 0, one // n, 0
+        while power:
+            total += (power if k % 2 == 0 else -power) // (2 * k + 1)
+            power //= n * n
+            k += 1
+        return total
+    return Fraction(16 * arctan_inverse(5) - 4 * arctan_inverse(239), one)
+
+
+PI = _pi()
+
+
+def _root(x, n):
+    """x ** (1/n) of a fraction, within 2^-DIGITS, by bisection on integers."""
+    scaled = (x.numerator << (n * DIGITS)) // x.denominator
+    lo, hi = 0, 1 << (DIGITS + max(1, x.numerator.bit_length()))
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        if mid ** n <= scaled:
+            lo = mid
+        else:
+            hi = mid
+    return Fraction(lo, 1 << DIGITS)
+
+
+def frequencies(base, width):
+    """base ** (-2 i / width), i < width / 2, as fractions."""
+    step = _root(Fraction(base), width // 2)          # base ** (2 / width)
+    return [1 / step ** i for i in range(width // 2)]
+
+
+def units_off(stored, radians):
+    """How far a stored frequency is from the true one, in units of 2^-64 turns."""
+    d = (Fraction(int(stored) % 2 ** 64) - radians / (2 * PI) * 2 ** 64) % 2 ** 64
+    return float(min(d, 2 ** 64 - d))
+
+
+def test_frequencies_keep_64_bits():
+    """A stored frequency is the nearest of its 2^64 values to the formula's: half a unit."""
+    rope = rotary_axes(128, (32, 48, 48), base=(10000.0, 500000.0, 100.0), device="cpu")
+    want = frequencies(10000, 32) + frequencies(500000, 48) + frequencies(100, 48)
+    assert max(units_off(f, w) for f, w in zip(rope.freq, want)) <= 0.500001
+    rope = rotary_axes(128, 128, device="cpu")
+    assert max(units_off(f, w) for f, w in zip(rope.freq, frequencies(10000, 128))) <= 0.500001
+    own = [0.1, -0.1, 1e-7, -1e-7, 3.0, 1234.5, -2.0 ** -70, 0.0, 1e18, 2.0 ** -64, 1.0, -1.0, 0.7, 1e-19, 6.283185307179586, 1e300]
+    rope = rotary_axes(64, 32, inv_freq=own, device="cpu")
+    assert max(units_off(f, Fraction(w)) for f, w in zip(rope.freq, own)) <= 0.500001
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top", [2 ** 31, 2 ** 40])
+def test_positions_far_from_zero(top):
+    """The kernel's angle is within 2^-32 turns of position times stored frequency, and that is half a unit of 2^-64 turns
+    off: 2 pi (2^-32 + position 2^-65) radians beyond what fp32 does to every angle."""
+    dev = torch.device("cuda", 0)
+    pos = [top - 1, top // 2 + 7, top - 12345, -top + 1, top // 3]
+    freqs = frequencies(10000, 64)
+    turns = [[(p * f / (2 * PI)) % 1 for f in freqs] for p in pos]
+    phase = torch.tensor([[float(t * 2 * PI if t < Fraction(1, 2) else (t - 1) * 2 * PI) for t in row] for row in turns], dtype=torch.float64)
+    x = H.randn((1, 2, len(pos), 64), 5, torch.float32, dev)
+    y = apply_rotary(x, None, torch.tensor(pos, dtype=torch.int64, device=dev), rotary_axes(64, 64)).cpu().double()
+    want = rotate64(x.cpu(), phase[None, None], False)
+    tol = tolerance(x.cpu(), want, 32, False, torch.float32) + 6.2832 * (2.0 ** -32 + top * 2.0 ** -65) * partner_sum(x.cpu(), 32, False)
+    assert ((y - want).abs() - tol).max() <= 0
 
 
 def allocations(fn):
