@@ -58,7 +58,7 @@ typedef struct sage_paged_kv {
 /* A batch of B sequences whose T new tokens lie one behind the other: those of sequence b are rows
  * [cu_q[b], cu_q[b+1]), or row b alone if cu_q is NULL (then T == B).  kv_lens[b] counts all keys of the sequence, the
  * new tokens included: new token i of n has position kv_lens[b] - n + i, and key j stands in slot j % page_size of page
- * page_table[b * table_stride + j / page_size].  All four arrays are int32 on the device.  Entries of the table behind the
+ * page_table[b * table_stride + j / page_size].  All four arrays are int32 on the device and stay as they are until the call has completed.  Entries of the table behind the
  * last key are not looked at.  cu_q that leaves [0, T] or falls is clipped; rows that belong to no sequence are not written
  * (by sage_paged_append: zeroed).  Without cu_q a kv_lens of 0 is a slot that is not in use: nothing is stored for it, and
  * its rows are zero. */

@@ -8,7 +8,9 @@
 // step.  A span that covers part of an item leaves its result in a slot of the workspace (slot 1 the head of an item, slot 0
 // anything else: at most one of each per CTA) and a header that tells the merge kernels which parts follow.  Every CTA works
 // this out for itself from kv_lens and cu_q, by a block-wide prefix sum; nothing is communicated and the order of all sums is
-// fixed.
+// fixed.  Both are read more than once.  A program that changes them before the call is through gets numbers that mean
+// nothing, but every walk ends and every access stays in its tensor: what is derived from a sequence comes from one reading of it, and
+// walks end with the last sequence and the last CTA.
 #pragma once
 
 #include "paged_common.cuh"
@@ -225,7 +227,7 @@ __device__ __forceinline__ Span find_span(const AttnParams& p, SpanScratch* scra
     while (true) {
       seq = seq_at(p, b);
       const long long steps = steps_of(p, seq);
-      if (s.t < before + steps) break;
+      if (s.t < before + steps || b + 1 == last) break;        // (the latter if lengths change meanwhile)
       before += steps;
       ++b;
     }
@@ -290,7 +292,8 @@ struct SegmentIter {
 #pragma unroll 1
       while (s.t >= s.before + steps) {               // (sequences without new tokens have no steps)
         s.before += steps;
-        find(++s.b);
+        if (++s.b >= n_seqs(p)) return g;
+        find(s.b);
       }
       if (head < 0) {                                 // the head by division, its row tile step by step
         head = static_cast<int>(floor_div(s.t - s.before, seq.head_steps));
@@ -331,7 +334,7 @@ struct SegmentIter {
         // the CTA that has the first step of the last tile
         const long long e = item_end - cost, longer = s.extra * (s.share + 1);
         const long long c = e < longer ? floor_div(e, s.share + 1) : s.extra + floor_div(e - longer, s.share);
-        g.n_parts = static_cast<int>(c) - static_cast<int>(blockIdx.x) + 1;
+        g.n_parts = min(static_cast<int>(c), s.ctas - 1) - static_cast<int>(blockIdx.x) + 1;
       }
       s.t = stop;
     }

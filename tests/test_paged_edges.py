@@ -188,6 +188,42 @@ def test_a_row_without_keys_is_zero_whatever_v_holds(q_lens, kv_lens, value):
         assert not torch.isfinite(o[blind:q_lens[0]]).any() and torch.isfinite(o[q_lens[0]:]).all()
 
 
+# ---------------------------------------------------------------- lengths that change too early
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_len, shared", [(1, 0), (60, 0), (1, 64)])
+def test_lengths_that_change_during_a_call(q_len, shared):
+    """A program's mistake, which gives numbers without a meaning: the calls end all the same, write their own rows only, and those
+    behind them are right."""
+    dev = torch.device("cuda", 0)
+    n = 40
+    batch = PagedBatch([q_len] * n, [shared + q_len + (173 * i) % 900 for i in range(n)], 4, 2, 64, 16, "NHD", F16, dev, shared=shared)
+    table, lens = batch.args()
+    table[:, :shared // 16] = 0
+    table.clamp_(0, batch.n_pages - 1)                        # (any length up to the width of the table finds pages)
+    cache, cu, room = batch.cache(), batch.cu_q(), torch.full((batch.T + 8, 4, 64), 7.0, dtype=F16, device=dev)
+    args = dict(cu_q=cu, max_q=q_len, shared_pages=batch.shared_pages())
+    q = batch.q.to(dev)
+    want = sageattn_paged(q, cache, table, lens, **args)
+    good, good_cu = lens.clone(), cu.clone()
+    g = torch.Generator(device=dev).manual_seed(1)
+    other = torch.randint(0, table.size(1) * 16, (64, n), generator=g, device=dev, dtype=torch.int32)
+    rows = torch.randint(0, batch.T + 1, (64, n + 1), generator=g, device=dev, dtype=torch.int32).sort(dim=1).values.to(torch.int32)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(200):
+        with torch.cuda.stream(side):
+            lens.copy_(other[i % 64])
+            cu.copy_(rows[(i * 7) % 64])
+        sageattn_paged(q, cache, table, lens, out=room[4:-4], **args)
+    torch.cuda.synchronize()
+    assert (room[:4] == 7.0).all() and (room[-4:] == 7.0).all()
+    check_status(dev)
+    lens.copy_(good)
+    cu.copy_(good_cu)
+    assert torch.equal(sageattn_paged(q, cache, table, lens, **args), want)
+
+
 # ---------------------------------------------------------------- slots that are not in use
 
 @pytest.mark.gpu
